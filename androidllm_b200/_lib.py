@@ -33,6 +33,45 @@ class ProjSrc(ctypes.Structure):
                 ("in_", ctypes.c_int), ("in_real", ctypes.c_int)]
 
 
+class PagedKVView(ctypes.Structure):
+    _fields_ = [("k_dev", ctypes.c_void_p), ("v_dev", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int)]
+
+
+class SeqBatchView(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_seq", "n_rows", "max_rows", "table_rows", "table_pages",
+                                            "page_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("row_start_dev", "kv_len_dev", "page_table_dev", "slots_dev")]
+
+
+class RopeAppendArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q_dev", "k_dev", "v_dev")] + \
+               [(n, ctypes.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")] + \
+               [("q_out_dev", ctypes.c_void_p), ("qo_row", ctypes.c_int64), ("qo_head", ctypes.c_int64),
+                ("heads", ctypes.c_int), ("q_norm_dev", ctypes.c_void_p), ("k_norm_dev", ctypes.c_void_p),
+                ("eps", ctypes.c_float), ("rope_dev", ctypes.c_void_p), ("rope_dtype", ctypes.c_int),
+                ("rope_rows", ctypes.c_int), ("rot_dim", ctypes.c_int), ("interleaved", ctypes.c_int)]
+
+
+class AttnPagedArgs(ctypes.Structure):
+    _fields_ = [("q_dev", ctypes.c_void_p), ("q_row", ctypes.c_int64), ("q_head", ctypes.c_int64),
+                ("out_dev", ctypes.c_void_p), ("out_row", ctypes.c_int64), ("out_head", ctypes.c_int64),
+                ("lse_dev", ctypes.c_void_p), ("lse_row", ctypes.c_int64), ("heads", ctypes.c_int),
+                ("window", ctypes.c_int), ("scale", ctypes.c_float), ("work_dev", ctypes.c_void_p),
+                ("work_bytes", ctypes.c_size_t)]
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_seq", "n_rows", "k_max", "vocab")] + \
+               [("row_start_dev", ctypes.c_void_p), ("logits_dev", ctypes.c_void_p),
+                ("logits_dtype", ctypes.c_int), ("logits_row", ctypes.c_int64),
+                ("draft_tokens_dev", ctypes.c_void_p), ("draft_probs_dev", ctypes.c_void_p),
+                ("q_seq", ctypes.c_int64), ("q_step", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("uniforms_dev", "temperature_dev", "min_p_dev", "tokens_dev",
+                                               "n_accepted_dev", "p_draft_dev")]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _PP = ctypes.POINTER(ctypes.c_void_p)
@@ -93,6 +132,12 @@ SIGNATURES = {
     "alm_ctx_set_dense_prefill": [_P, _I],
     "alm_model_dense_prefill": [_P, _P],
     "alm_model_max_pass_rows": [_P, _P],
+    "alm_ctx_create_on_stream": [_I, _P, _PP],
+    "alm_kv_view": [_P, _I, ctypes.POINTER(PagedKVView), _PP, _PI32, _PI32],
+    "alm_rope_append": [_P, _P, _P, _P],
+    "alm_attn_paged": [_P, _P, _P, _P],
+    "alm_attn_paged_work": [_P, _I, _I, _I, ctypes.POINTER(ctypes.c_size_t)],
+    "alm_verify": [_P, _P],
     "alm_forward_trace": [_P, _P, _P, _I, _I, _P, _I, _P, _P],
     "alm_spec_create": [_P, _P, _P, _P, _I, _PP],
     "alm_spec_destroy": [_P],

@@ -1,0 +1,590 @@
+// Attention of a pass's new rows over the paged cache (alm_attn_paged): the
+// mma.sync kernel for few rows a sequence, and the kernel that joins the
+// partial results of units cut between CTAs.  Instantiated for fp16
+// and bf16 in attn_paged_f16.cu and attn_paged_bf16.cu.
+//
+//   o_i = sum_j exp(c (s_ij - m_i)) v_j / sum_j exp(c (s_ij - m_i)),  s = q.k,
+//   c = scale, over the positions j that row i sees; m_i = max_j s_ij.
+//
+// One pass over K and V with a running maximum and sum (rescaled when the
+// maximum grows).  A decode or verify pass reads far more K/V bytes than
+// it computes on, so HBM bounds it: the CTAs share all tiles evenly
+// (attn_sched.cuh), each streams its run of tiles through a ring of
+// shared-memory stages filled with cp.async across unit borders, and the rows
+// of the query heads that share a K/V head are one matrix operand, so K and V
+// are read once for all of them.
+//
+// CTA: 8 warps as WM x WK.  Warp (wm, wk) computes rows 16 wm .. 16 wm + 15
+// on the wk-th slice of each tile, with its own running statistics;
+// the WK slices are merged at a unit's end through the stage just consumed.
+#pragma once
+#include "attn_sched.cuh"
+
+namespace alm {
+
+constexpr int kPagedThreads = 256;
+constexpr int kPagedWarps = kPagedThreads / kWarp;
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<half> {
+  ALM_DEV static uint32_t pack(float a, float b) {
+    half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  ALM_DEV static float up(half h) { return __half2float(h); }
+  ALM_DEV static half down(float f) { return __float2half_rn(f); }
+  ALM_DEV static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma16816(d, a[0], a[1], a[2], a[3], b0, b1);
+  }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+  ALM_DEV static uint32_t pack(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  ALM_DEV static float up(__nv_bfloat16 h) { return __bfloat162float(h); }
+  ALM_DEV static __nv_bfloat16 down(float f) { return __float2bfloat16_rn(f); }
+  ALM_DEV static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+ALM_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+ALM_DEV void ldmatrix_x4_trans(uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3, uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(a) : "memory");
+}
+ALM_DEV void ldmatrix_x4_at(uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3, uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(a) : "memory");
+}
+// 16 bytes, or zeros where `bytes` is 0
+ALM_DEV void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+ALM_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+ALM_DEV void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <int HD, int WM>
+struct PagedShape {
+  static constexpr int kTile = HD > 128 ? 64 : 128;        // positions a tile
+  static constexpr int kWK = kPagedWarps / WM;
+  static constexpr int kNP = kTile / kWK;                  // positions a warp and tile
+  static constexpr int kChunk = kNP < 64 ? kNP : 64;       // ... and step
+  static constexpr int kRows = 16 * WM;
+  // rows padded by 16 bytes: an odd number of 16-byte units, so that the 8
+  // rows of an ldmatrix matrix lie in 8 different bank groups
+  static constexpr int kPitch = HD * 2 + 16;
+  static constexpr int kStageBytes = 2 * kTile * kPitch;
+  static constexpr int kStages = HD <= 64 ? 6 : HD <= 96 ? 4 : 3;
+  // merge of the WK slices: 128 fp32 rows of HD / kPasses + 8 columns in one stage
+  static constexpr int kPasses = HD > 128 ? 4 : 1;
+  static constexpr int kMergePitch = HD / kPasses + 8;
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes;
+  static_assert(128 * kMergePitch * 4 <= kStageBytes, "merge fits a stage");
+  static_assert(kNP >= 16, "a warp's slice holds a k16 step");
+};
+
+// Partial result of a CTA's first (which = 0) or last (1) unit: kRows rows of
+// HD fp32 sums, then their maxima, then their sums of weights.
+template <int HD>
+ALM_DEV float* partial_at(char* work, int rows, int cta, int which) {
+  return reinterpret_cast<float*>(work) + (static_cast<size_t>(cta) * 2 + which) * rows * (HD + 2);
+}
+
+// One row by one warp straight from the formula, skipping every position the
+// row does not see: for rows whose sums are not finite, since a hidden
+// position's infinity or NaN times a zero weight spoils a matrix product.
+template <typename T, int HD>
+__device__ __noinline__ void row_by_formula(const AttnPaged& a, const PagedKV& kv, const Unit& u, int tok, int head,
+                                            int p_lo, int p_hi, float (&o)[HD / 32], float& m, float& l) {
+  const int lane = threadIdx.x % kWarp;
+  const T* q = reinterpret_cast<const T*>(a.q + (u.row0 + tok) * a.q_row + head * a.q_head);
+  float qv[HD / 32];
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) {
+    qv[i] = Elem<T>::up(q[lane + 32 * i]);
+    o[i] = 0.f;
+  }
+  m = kNegInf;
+  l = 0.f;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int p = p_lo; p <= p_hi; ++p) {
+      const int pi = page_of(kv, p);
+      const int page = u.pages ? __ldg(u.pages + pi) : -1;
+      const bool ok = page >= 0 && page < kv.n_pages;
+      const size_t off = ok ? kv_offset(kv, page, u.h, p - pi * kv.page_size) : 0;
+      const T* k = reinterpret_cast<const T*>(kv.k) + off;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) s = fmaf(qv[i], ok ? Elem<T>::up(k[lane + 32 * i]) : 0.f, s);
+      s = warp_sum(s);
+      if (pass == 0) {
+        m = fmaxf(m, s);
+        continue;
+      }
+      const float w = ex2((s - m) * a.scale_log2);
+      l += w;
+      const T* v = reinterpret_cast<const T*>(kv.v) + off;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) o[i] = fmaf(w, ok ? Elem<T>::up(v[lane + 32 * i]) : 0.f, o[i]);
+    }
+  }
+}
+
+template <typename T, int HD, int WM>
+__global__ void __launch_bounds__(kPagedThreads, 1)
+attn_paged_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv, int* err) {
+  using S = PagedShape<HD, WM>;
+  constexpr int kTile = S::kTile, kWK = S::kWK, kNP = S::kNP, kChunk = S::kChunk, kRows = S::kRows;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ SchedShared sched;
+  __shared__ float st_m[kWK][kRows], st_l[kWK][kRows];
+  __shared__ float row_m[kRows], row_l[kRows];
+  __shared__ int row_bad[kRows];
+
+  grid_dep_launch();
+  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
+  const int wm = warp % WM, wk = warp / WM, g = lane / 4, t4 = lane % 4;
+  const int tpu = kRows / a.group;
+  const int cta = blockIdx.x;
+  sched_init<kTile>(
+      b, kv, tpu, a.window, a.min_rows, a.max_rows, sched,
+      [&](long long total) {
+        const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
+        return cta < n ? share(total, cta, n) : -1ll;
+      },
+      [] { __syncthreads(); });
+  const long long total = sched.total;
+  const int n_cta = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
+  if (cta >= n_cta) return;
+  const long long x0 = share(total, cta, n_cta), x1 = share(total, cta + 1, n_cta);
+
+  Unit u = unit_at<kTile>(b, kv, tpu, a.window, sched.found_seq, sched.found_at, x0);
+  // the loader's walk, kStages - 1 tiles ahead of the computation's
+  Unit lu = u;
+  int lt = static_cast<int>(x0 - u.start);
+  long long lx = x0;
+  const uint32_t smem0 = smem_addr(smem);
+  constexpr int kUnits16 = HD / 8;   // 16-byte units of a K or V row
+  bool bad_page = false;
+
+  auto load_tile = [&](int stage) {
+    if (lx < x1) {
+      const uint32_t dst = smem0 + stage * S::kStageBytes;
+      const int base = (lu.t0 + lt) * kTile;
+      constexpr int kIter = kTile * kUnits16 / kPagedThreads;
+#pragma unroll
+      for (int i = 0; i < kIter; ++i) {
+        const int idx = tid + i * kPagedThreads;
+        const int r = idx / kUnits16, c = idx % kUnits16;
+        const int pos = base + r;
+        const int pi = page_of(kv, pos);
+        const bool in = pos < lu.n_kv;
+        const int page = in && lu.pages ? __ldg(lu.pages + pi) : -1;
+        const bool ok = page >= 0 && page < kv.n_pages;
+        bad_page |= in && !ok;
+        const size_t off = (ok ? kv_offset(kv, page, lu.h, pos - pi * kv.page_size) + c * 8 : 0) * sizeof(T);
+        cp_async16(dst + r * S::kPitch + c * 16, kv.k + off, ok ? 16 : 0);
+        cp_async16(dst + (kTile + r) * S::kPitch + c * 16, kv.v + off, ok ? 16 : 0);
+      }
+      ++lx;
+      if (++lt == lu.n_tile && lx < x1) {
+        next_unit<kTile>(b, kv, tpu, a.window, a.min_rows, a.max_rows, lu);
+        lt = 0;
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S::kStages - 1; ++i) load_tile(i);
+
+  int t = static_cast<int>(x0 - u.start);
+  int t_first = t;   // first tile of the unit computed here
+  uint32_t qf[HD / 16][4];
+  float o[HD / 8][4];
+  float m[2], l[2];
+  int hi[2];
+  auto begin_unit = [&] {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = wm * 16 + g + 8 * j;
+      const int tok = row / a.group, hh = row - tok * a.group;
+      const bool live = tok < u.n_tok;
+      hi[j] = live ? u.pos0 + tok : -1;
+      const char* q = a.q + (u.row0 + tok) * a.q_row + (u.h * a.group + hh) * a.q_head;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        qf[k][j] = live ? __ldg(reinterpret_cast<const unsigned*>(q + (16 * k + 2 * t4) * 2)) : 0u;
+        qf[k][j + 2] = live ? __ldg(reinterpret_cast<const unsigned*>(q + (16 * k + 8 + 2 * t4) * 2)) : 0u;
+      }
+      m[j] = kNegInf;
+      l[j] = 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[n][j] = 0.f;
+  };
+  begin_unit();
+
+  int stage = 0;
+  for (long long x = x0; x < x1; ++x) {
+    cp_async_wait<S::kStages - 2>();
+    __syncthreads();
+    load_tile(stage == 0 ? S::kStages - 1 : stage - 1);
+    const uint32_t kb = smem0 + stage * S::kStageBytes, vb = kb + kTile * S::kPitch;
+#pragma unroll 1
+    for (int c0 = 0; c0 < kNP; c0 += kChunk) {
+      const int r0 = wk * kNP + c0;                    // first row of the chunk in the stage
+      const int p0 = (u.t0 + t) * kTile + r0;          // ... and its position
+      float s[kChunk / 8][4];
+#pragma unroll
+      for (int n = 0; n < kChunk / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+        for (int n = 0; n < kChunk / 8; n += 2) {
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4_at(b0, b1, b2, b3,
+                         kb + (r0 + n * 8 + (lane & 7) + ((lane >> 4) & 1) * 8) * S::kPitch +
+                             (2 * k + ((lane >> 3) & 1)) * 16);
+          Elem<T>::mma(s[n], qf[k], b0, b1);
+          Elem<T>::mma(s[n + 1], qf[k], b2, b3);
+        }
+      // positions that some row of the block does not see
+      if (p0 + kChunk - 1 > u.pos0 || (a.window > 0 && p0 <= u.pos0 + u.n_tok - 1 - a.window)) {
+#pragma unroll
+        for (int n = 0; n < kChunk / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int p = p0 + n * 8 + 2 * t4 + (j & 1);
+            const bool seen = p <= hi[j >> 1] && (a.window == 0 || p > hi[j >> 1] - a.window);
+            s[n][j] = seen ? s[n][j] : kNegInf;
+          }
+      }
+      float mc[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float x_ = m[j];
+#pragma unroll
+        for (int n = 0; n < kChunk / 8; ++n) x_ = fmaxf(x_, fmaxf(s[n][2 * j], s[n][2 * j + 1]));
+        x_ = fmaxf(x_, __shfl_xor_sync(0xffffffffu, x_, 1));
+        x_ = fmaxf(x_, __shfl_xor_sync(0xffffffffu, x_, 2));
+        const float base = x_ == kNegInf ? 0.f : x_;   // nothing seen yet: every weight is exp(-inf)
+        const float f = ex2((m[j] - base) * a.scale_log2);
+        m[j] = x_;
+        mc[j] = base * a.scale_log2;
+        l[j] *= f;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+          o[n][2 * j] *= f;
+          o[n][2 * j + 1] *= f;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kChunk / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[n][j] = ex2(fmaf(s[n][j], a.scale_log2, -mc[j >> 1]));
+          l[j >> 1] += s[n][j];
+        }
+#pragma unroll
+      for (int k = 0; k < kChunk / 16; ++k) {
+        // weights in [0, 1] rounded to the cache's type for the tensor core:
+        // half a step each, as the output's own rounding, averaged over the row
+        const uint32_t p[4] = {Elem<T>::pack(s[2 * k][0], s[2 * k][1]), Elem<T>::pack(s[2 * k][2], s[2 * k][3]),
+                               Elem<T>::pack(s[2 * k + 1][0], s[2 * k + 1][1]),
+                               Elem<T>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
+#pragma unroll
+        for (int n = 0; n < HD / 8; n += 2) {
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4_trans(b0, b1, b2, b3,
+                            vb + (r0 + k * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * S::kPitch +
+                                (n + (lane >> 4)) * 16);
+          Elem<T>::mma(o[n], p, b0, b1);
+          Elem<T>::mma(o[n + 1], p, b2, b3);
+        }
+      }
+    }
+    if (t + 1 < u.n_tile && x + 1 < x1) {
+      ++t;
+      if (++stage == S::kStages) stage = 0;
+      continue;
+    }
+
+    // the unit's end, or the share's: merge the WK slices through this stage
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
+      l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
+      if (t4 == 0) {
+        st_m[wk][wm * 16 + g + 8 * j] = m[j];
+        st_l[wk][wm * 16 + g + 8 * j] = l[j];
+      }
+    }
+    if (tid < kRows) row_bad[tid] = 0;
+    __syncthreads();
+    if (tid < kRows) {
+      float mm = kNegInf, ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) mm = fmaxf(mm, st_m[w][tid]);
+      const float base = mm == kNegInf ? 0.f : mm;
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) ll += st_l[w][tid] * ex2((st_m[w][tid] - base) * a.scale_log2);
+      row_m[tid] = mm;
+      row_l[tid] = ll;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float mm = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kWK; ++w) mm = fmaxf(mm, st_m[w][wm * 16 + g + 8 * j]);
+      const float f = ex2((m[j] - (mm == kNegInf ? 0.f : mm)) * a.scale_log2);
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n) {
+        o[n][2 * j] *= f;
+        o[n][2 * j + 1] *= f;
+      }
+    }
+    float* buf = reinterpret_cast<float*>(smem + stage * S::kStageBytes);
+    const bool whole = u.start >= x0 && u.start + u.n_tile <= x1;
+    float* part = partial_at<HD>(a.work, kRows, cta, u.start >= x0 ? 1 : 0);
+    constexpr int kCols = HD / S::kPasses;
+    bool any_bad = false;
+#pragma unroll
+    for (int ps = 0; ps < S::kPasses; ++ps) {
+#pragma unroll
+      for (int n = 0; n < kCols / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<float2*>(buf + (wk * kRows + wm * 16 + g + 8 * j) * S::kMergePitch + n * 8 + 2 * t4) =
+              make_float2(o[ps * (kCols / 8) + n][2 * j], o[ps * (kCols / 8) + n][2 * j + 1]);
+      __syncthreads();
+      for (int i = tid; i < kRows * (kCols / 4); i += kPagedThreads) {
+        const int row = i / (kCols / 4), c = (i % (kCols / 4)) * 4;
+        const int tok = row / a.group, hh = row - tok * a.group;
+        if (tok >= u.n_tok) continue;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWK; ++w) {
+          const float4 y = *reinterpret_cast<const float4*>(buf + (w * kRows + row) * S::kMergePitch + c);
+          v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+        }
+        const bool bad = !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < __int_as_float(0x7f800000)) ;
+        if (bad) {
+          row_bad[row] = 1;
+          any_bad = true;
+        }
+        const int col = ps * kCols + c;
+        if (whole) {
+          // no position seen: the sums are zero, and so is the row
+          const float inv = row_m[row] == kNegInf && row_l[row] == 0.f ? 0.f : 1.f / row_l[row];
+          uint2 w2 = make_uint2(Elem<T>::pack(v.x * inv, v.y * inv), Elem<T>::pack(v.z * inv, v.w * inv));
+          char* dst = a.out + (u.row0 + tok) * a.out_row + (u.h * a.group + hh) * a.out_head;
+          *reinterpret_cast<uint2*>(dst + col * 2) = w2;
+          if (a.lse && col == 0)
+            a.lse[(u.row0 + tok) * a.lse_row + u.h * a.group + hh] =
+                row_m[row] == kNegInf ? kNegInf
+                                      : (row_m[row] * a.scale_log2 + log2f(row_l[row])) * 0.693147180559945309f;
+        } else {
+          *reinterpret_cast<float4*>(part + row * HD + col) = v;
+          if (col == 0) {
+            part[kRows * HD + row] = row_m[row];
+            part[kRows * HD + kRows + row] = row_l[row];
+          }
+        }
+      }
+      if (ps + 1 < S::kPasses) __syncthreads();
+    }
+    if (__syncthreads_or(any_bad)) {
+      for (int row = warp; row < kRows; row += kPagedWarps) {
+        if (!row_bad[row]) continue;
+        const int tok = row / a.group, hh = row - tok * a.group, head = u.h * a.group + hh;
+        const int last = u.pos0 + tok;
+        const int p_lo = max((u.t0 + t_first) * kTile, a.window > 0 ? last - a.window + 1 : 0);
+        const int p_hi = min((u.t0 + t + 1) * kTile - 1, last);
+        float ov[HD / 32], mm, ll;
+        row_by_formula<T, HD>(a, kv, u, tok, head, p_lo, p_hi, ov, mm, ll);
+        T* dst = reinterpret_cast<T*>(a.out + (u.row0 + tok) * a.out_row + head * a.out_head);
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+          if (whole) dst[lane + 32 * i] = Elem<T>::down(p_hi < p_lo ? 0.f : ov[i] / ll);
+          else part[row * HD + lane + 32 * i] = ov[i];
+        }
+        if (lane == 0) {
+          if (!whole) {
+            part[kRows * HD + row] = mm;
+            part[kRows * HD + kRows + row] = ll;
+          } else if (a.lse) {
+            a.lse[(u.row0 + tok) * a.lse_row + head] = (mm * a.scale_log2 + log2f(ll)) * 0.693147180559945309f;
+          }
+        }
+      }
+    }
+    if (x + 1 < x1) {
+      next_unit<kTile>(b, kv, tpu, a.window, a.min_rows, a.max_rows, u);
+      t = t_first = 0;
+      begin_unit();
+    }
+    if (++stage == S::kStages) stage = 0;
+  }
+  if (bad_page) *err = 1;
+}
+
+// Joins the partial results of the unit that CTA blockIdx.x began and did not
+// finish: rows 8 blockIdx.y + warp.  Partials are added in CTA order.
+template <typename T, int HD, int TILE, int ROWS>
+__global__ void __launch_bounds__(kPagedThreads)
+attn_paged_join_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv) {
+  __shared__ SchedShared sched;
+  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+  const int tpu = ROWS / a.group, cta = blockIdx.x;
+  long long x0 = 0, x1 = 0;
+  sched_init<TILE>(
+      b, kv, tpu, a.window, a.min_rows, a.max_rows, sched,
+      [&](long long total) {
+        const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
+        if (cta >= n) return -1ll;
+        x0 = share(total, cta, n);
+        x1 = share(total, cta + 1, n);
+        return x1 - 1;
+      },
+      [] { __syncthreads(); });
+  const long long total = sched.total;
+  const int n_cta = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
+  Unit u;
+  bool mine = cta < n_cta && x1 < total;
+  if (mine) {
+    u = unit_at<TILE>(b, kv, tpu, a.window, sched.found_seq, sched.found_at, x1 - 1);
+    mine = u.start >= x0 && u.start + u.n_tile > x1;
+  }
+  grid_dep_wait();
+  if (!mine) return;
+  int last = cta + 1;   // the CTA that holds the unit's last tile
+  while (share(total, last + 1, n_cta) < u.start + u.n_tile) ++last;
+  const int row = blockIdx.y * kPagedWarps + warp;
+  const int tok = row / a.group, head = u.h * a.group + row - tok * a.group;
+  if (tok >= u.n_tok) return;
+  const int n = last - cta + 1;
+
+  auto part = [&](int i) { return partial_at<HD>(a.work, ROWS, cta + i, i == 0 ? 1 : 0); };
+  float m = kNegInf;
+  for (int i = lane; i < n; i += kWarp) m = fmaxf(m, __ldcg(part(i) + ROWS * HD + row));
+  m = warp_max(m);
+  const float base = m == kNegInf ? 0.f : m;
+  float l = 0.f, o[HD / 32];
+#pragma unroll
+  for (int j = 0; j < HD / 32; ++j) o[j] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += kWarp) {
+    float w = 0.f, li = 0.f;
+    if (i0 + lane < n) {
+      const float* p = part(i0 + lane) + ROWS * HD;
+      w = ex2((__ldcg(p + row) - base) * a.scale_log2);
+      li = __ldcg(p + ROWS + row);
+    }
+    const int k = min(kWarp, n - i0);
+#pragma unroll 8
+    for (int i = 0; i < k; ++i) {
+      const float f = __shfl_sync(0xffffffffu, w, i);
+      l = fmaf(__shfl_sync(0xffffffffu, li, i), f, l);
+      const float* p = part(i0 + i) + row * HD;
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) o[j] = fmaf(__ldcg(p + lane + 32 * j), f, o[j]);
+    }
+  }
+  const float inv = m == kNegInf && l == 0.f ? 0.f : 1.f / l;
+  T* dst = reinterpret_cast<T*>(a.out + (u.row0 + tok) * a.out_row + head * a.out_head);
+#pragma unroll
+  for (int j = 0; j < HD / 32; ++j) dst[lane + 32 * j] = Elem<T>::down(o[j] * inv);
+  if (a.lse && lane == 0)
+    a.lse[(u.row0 + tok) * a.lse_row + head] =
+        m == kNegInf ? kNegInf : (m * a.scale_log2 + log2f(l)) * 0.693147180559945309f;
+}
+
+template <typename T, int HD, int WM>
+cudaError_t paged_attr() {
+  return cudaFuncSetAttribute(attn_paged_kernel<T, HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              static_cast<int>(PagedShape<HD, WM>::kSmem));
+}
+template <typename T, int HD>
+cudaError_t paged_attr_hd() {
+  cudaError_t e = paged_attr<T, HD, 2>();
+  if constexpr (HD <= 128) {
+    if (e == cudaSuccess) e = paged_attr<T, HD, 1>();
+  }
+  if (e == cudaSuccess) e = paged_attr<T, HD, 4>();
+  if (e == cudaSuccess) e = paged_attr<T, HD, 8>();
+  return e;
+}
+template <typename T>
+cudaError_t paged_attr_all() {
+  cudaError_t e = paged_attr_hd<T, 32>();
+  if (e == cudaSuccess) e = paged_attr_hd<T, 64>();
+  if (e == cudaSuccess) e = paged_attr_hd<T, 96>();
+  if (e == cudaSuccess) e = paged_attr_hd<T, 128>();
+  if (e == cudaSuccess) e = paged_attr_hd<T, 256>();
+  return e;
+}
+
+template <typename T, int HD, int TILE, int ROWS>
+cudaError_t launch_join(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.n_cta, ROWS / kPagedWarps, 1);
+  cfg.blockDim = dim3(kPagedThreads, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<T, HD, TILE, ROWS>, a, b, kv);
+}
+
+template <typename T, int HD, int WM>
+cudaError_t launch_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st) {
+  using S = PagedShape<HD, WM>;
+  attn_paged_kernel<T, HD, WM><<<a.n_cta, kPagedThreads, S::kSmem, st>>>(a, b, kv, err);
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess ? e : launch_join<T, HD, S::kTile, S::kRows>(a, b, kv, st);
+}
+
+// The smallest row block that holds the longest sequence's rows: K and V are
+// read once per block of rows, and padding rows cost tensor work only.
+template <typename T, int HD>
+cudaError_t launch_paged_hd(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st) {
+  const long long rows = static_cast<long long>(b.max_rows) * a.group;
+  if constexpr (HD <= 128) {
+    if (rows <= 16) return launch_paged<T, HD, 1>(a, b, kv, err, st);
+  }
+  if (rows <= 32) return launch_paged<T, HD, 2>(a, b, kv, err, st);
+  if (rows <= 64) return launch_paged<T, HD, 4>(a, b, kv, err, st);
+  return launch_paged<T, HD, 8>(a, b, kv, err, st);
+}
+template <typename T>
+cudaError_t launch_paged_t(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st) {
+  switch (kv.head_dim) {
+    case 32: return launch_paged_hd<T, 32>(a, b, kv, err, st);
+    case 64: return launch_paged_hd<T, 64>(a, b, kv, err, st);
+    case 96: return launch_paged_hd<T, 96>(a, b, kv, err, st);
+    case 128: return launch_paged_hd<T, 128>(a, b, kv, err, st);
+    default: return launch_paged_hd<T, 256>(a, b, kv, err, st);
+  }
+}
+
+}  // namespace alm

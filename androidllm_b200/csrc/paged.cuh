@@ -1,0 +1,113 @@
+// Operators of a batched step on device data: argument structs and launchers
+// shared by paged_api.cu (entry points and checks), rope_append.cu,
+// attn_paged.cu, attn_paged_tc.cu and verify.cu.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace alm {
+
+// One layer's pages, (n_pages, kv_heads, page_size, head_dim) each.
+struct PagedKV {
+  char* k;
+  char* v;
+  int n_pages, page_size, page_shift;   // page_shift: log2(page_size), or -1
+  int kv_heads, head_dim;
+};
+
+// The pass's sequences (see alm_seq_batch).
+struct SeqBatch {
+  int n_seq, n_rows, max_rows;
+  int table_rows, table_pages, page_stride;
+  const int* row_start;
+  const int* kv_len;
+  const int* table;
+  const int* slots;
+};
+
+// What a sequence's entries say, clamped to what exists: rows [row0, row0 +
+// n_new), the last of n_kv positions (n_new > n_kv leaves rows at negative
+// positions), its row of the page table (null: no such row).
+struct Seq {
+  int row0, n_new, n_kv;
+  const int* pages;
+};
+
+ALM_DEV Seq load_seq(const SeqBatch& b, const PagedKV& kv, int s) {
+  Seq q;
+  const int lo = max(0, min(__ldg(b.row_start + s), b.n_rows));
+  const int hi = max(lo, min(__ldg(b.row_start + s + 1), b.n_rows));
+  q.row0 = lo;
+  q.n_new = hi - lo;
+  const long long cap = static_cast<long long>(b.table_pages) * kv.page_size;
+  const int len = max(0, __ldg(b.kv_len + s));
+  q.n_kv = len > cap ? static_cast<int>(cap) : len;
+  const int t = b.slots ? __ldg(b.slots + s) : s;
+  q.pages = t >= 0 && t < b.table_rows ? b.table + static_cast<size_t>(t) * b.page_stride : nullptr;
+  return q;
+}
+
+ALM_DEV int page_of(const PagedKV& kv, int pos) { return kv.page_shift >= 0 ? pos >> kv.page_shift : pos / kv.page_size; }
+
+// Element offset of (page, head, position) inside K or V.
+ALM_DEV size_t kv_offset(const PagedKV& kv, int page, int head, int in_page) {
+  return ((static_cast<size_t>(page) * kv.kv_heads + head) * kv.page_size + in_page) * kv.head_dim;
+}
+
+struct RopeAppend {
+  const char *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // bytes
+  char* q_out;
+  int64_t qo_row, qo_head;                               // bytes
+  int heads;
+  const char *q_norm, *k_norm;
+  float eps;
+  const char* rope;
+  int rope_rows, rot;
+};
+
+struct AttnPaged {
+  const char* q;
+  int64_t q_row, q_head;       // bytes
+  char* out;
+  int64_t out_row, out_head;   // bytes
+  float* lse;
+  int64_t lse_row;             // elements
+  int heads, group, window;
+  float scale_log2;            // scale * log2(e)
+  char* work;
+  int n_cta;                   // CTAs that share the tiles
+  int min_rows, max_rows;      // this launch computes the sequences with min_rows <= rows < max_rows
+};
+
+struct Verify {
+  int n_seq, n_rows, k_max, vocab;
+  const int* row_start;
+  const char* logits;
+  int64_t logits_row;          // bytes
+  int vec;                     // rows are 16-byte aligned
+  const int* draft;
+  const float* q;
+  int64_t q_seq, q_step;
+  const double* u;
+  const float* temperature;
+  const float* min_p;
+  int* tokens;
+  int* n_accepted;
+  float* p_draft;
+};
+
+// dtype: ALM_F16 / ALM_BF16 / ALM_F32
+cudaError_t launch_rope_append(const RopeAppend& a, const SeqBatch& b, const PagedKV& kv, int dtype, int rope_dtype,
+                               bool interleaved, int* err, cudaStream_t st);
+cudaError_t launch_attn_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int dtype, int* err,
+                              cudaStream_t st);
+cudaError_t launch_verify(const Verify& a, int dtype, cudaStream_t st);
+size_t attn_paged_work_bytes(int n_sms, int head_dim);
+cudaError_t paged_init_attrs();
+
+}  // namespace alm

@@ -19,6 +19,7 @@
 #include "kernels.cuh"
 
 namespace alm {
+cudaError_t paged_init_attrs();
 cudaError_t launch_spec_prep_draft(const int* state, int* cand, const int* d_argmax, int i, int* tokens,
                                    int* pos, int prev_row, int refresh, cudaStream_t st);
 cudaError_t launch_spec_prep_verify(const int* state, int* cand, const int* d_argmax, int k, int* tokens,
@@ -165,6 +166,10 @@ struct alm_ctx {
   TpP2p p2p;
   float* p2p_own = nullptr;
   bool p2p_ready = false, tp_p2p = false;
+  bool own_stream = true;       // false: the caller's (alm_ctx_create_on_stream)
+  // what operators on device data met out of range (host memory that the GPU
+  // writes; read and cleared by alm_ctx_sync)
+  int* range_err = nullptr;
 };
 
 struct alm_qweight {
@@ -1320,8 +1325,7 @@ extern "C" {
 const char* alm_last_error(void) { return g_err.c_str(); }
 int alm_abi_version(void) { return 100; }
 
-int alm_ctx_create(int device, alm_ctx** out) {
-  ALM_REQ(out != nullptr, "null out");
+static int ctx_create(int device, bool own_stream, cudaStream_t stream, alm_ctx** out) {
   int n = 0;
   ALM_CUDA(cudaGetDeviceCount(&n));
   ALM_REQ(device >= 0 && device < n, "no such CUDA device");
@@ -1333,6 +1337,7 @@ int alm_ctx_create(int device, alm_ctx** out) {
     if (e == cudaSuccess) e = attn_prefill_init_attrs();
     if (e == cudaSuccess) e = rows_init_attrs();
     if (e == cudaSuccess) e = sample_init_attrs();
+    if (e == cudaSuccess) e = paged_init_attrs();
     if (e != cudaSuccess) return fail(ALM_ERR_CUDA, std::string("kernel attributes: ") + cudaGetErrorString(e));
   }
   auto* c = new alm_ctx();
@@ -1361,12 +1366,34 @@ int alm_ctx_create(int device, alm_ctx** out) {
     const char* e7 = getenv("ALM_ATTN_FUSED");
     c->attn_fused = e7 && e7[0] == '1';
   }
-  if (cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking) != cudaSuccess) {
+  if (cudaHostAlloc(reinterpret_cast<void**>(&c->range_err), sizeof(int), cudaHostAllocMapped) != cudaSuccess) {
+    delete c;
+    return fail(ALM_ERR_CUDA, "pinned memory allocation failed");
+  }
+  *c->range_err = 0;
+  c->own_stream = own_stream;
+  c->stream = stream;
+  if (own_stream && cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking) != cudaSuccess) {
+    cudaFreeHost(c->range_err);
     delete c;
     return fail(ALM_ERR_CUDA, "stream creation failed");
   }
   *out = c;
   return ALM_OK;
+}
+
+int alm_ctx_create(int device, alm_ctx** out) {
+  ALM_REQ(out != nullptr, "null out");
+  return ctx_create(device, true, nullptr, out);
+}
+
+int alm_ctx_create_on_stream(int device, void* stream, alm_ctx** out) {
+  ALM_REQ(out != nullptr, "null out");
+  int before = 0;
+  const bool restore = cudaGetDevice(&before) == cudaSuccess;
+  const int rc = ctx_create(device, false, static_cast<cudaStream_t>(stream), out);
+  if (restore) cudaSetDevice(before);
+  return rc;
 }
 
 int alm_ctx_destroy(alm_ctx* ctx) {
@@ -1379,7 +1406,8 @@ int alm_ctx_destroy(alm_ctx* ctx) {
   dev_free(ctx->p2p_own);
   dev_free(ctx->p2p.counters);
   tp_comm_destroy(ctx->tp_comm);
-  cudaStreamDestroy(ctx->stream);
+  if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
+  cudaFreeHost(ctx->range_err);
   delete ctx;
   return ALM_OK;
 }
@@ -1498,6 +1526,10 @@ int alm_ctx_sync(alm_ctx* ctx) {
   ALM_REQ(ctx, "null ctx");
   DeviceGuard g(ctx->device);
   ALM_CUDA(cudaStreamSynchronize(ctx->stream));
+  if (*const_cast<volatile int*>(ctx->range_err) != 0) {
+    *ctx->range_err = 0;
+    return fail(ALM_ERR_RANGE, "a page, slot or position outside its range reached the device");
+  }
   return ALM_OK;
 }
 
@@ -3120,5 +3152,30 @@ int alm_internal_ctx(alm_ctx* ctx, int* device, cudaStream_t* stream) {
   ALM_REQ(ctx && device && stream, "null argument");
   *device = ctx->device;
   *stream = ctx->stream;
+  return ALM_OK;
+}
+
+int alm_internal_ctx_paged(alm_ctx* ctx, int* device, int* n_sms, cudaStream_t* stream, int** range_err) {
+  ALM_REQ(ctx, "null ctx");
+  *device = ctx->device;
+  *n_sms = ctx->n_sms;
+  *stream = ctx->stream;
+  *range_err = ctx->range_err;
+  return ALM_OK;
+}
+
+int alm_internal_kv(alm_kv* kv, int layer, alm_paged_kv* view, const int32_t** table, int* rows, int* pages) {
+  ALM_REQ(kv && view && table && rows && pages, "null argument");
+  ALM_REQ(layer >= 0 && layer < kv->n_layers, "layer out of range");
+  view->k_dev = kv->k + static_cast<size_t>(layer) * kv->layer_elems;
+  view->v_dev = kv->v + static_cast<size_t>(layer) * kv->layer_elems;
+  view->dtype = ALM_F16;
+  view->n_pages = kv->n_pages;
+  view->page_size = kv->page_size;
+  view->kv_heads = kv->kv_heads;
+  view->head_dim = kv->head_dim;
+  *table = kv->page_table;
+  *rows = kv->n_slots;
+  *pages = kv->pages_per_slot;
   return ALM_OK;
 }

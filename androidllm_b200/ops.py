@@ -9,7 +9,7 @@ import os
 import numpy as np
 
 from . import safetensors
-from ._lib import ModelConfig, ProjSrc, check, lib, ptr
+from ._lib import ModelConfig, PagedKVView, ProjSrc, check, lib, ptr
 
 PROJ_BASES = ("q", "k", "v", "o", "gate", "up", "down")   # androidllm/shard.py:111
 # ALM_OP_* codes of include/androidllm_b200.h, in order
@@ -27,15 +27,22 @@ def _f16(a):
 
 
 class Context:
-    """One device + one stream."""
+    """One device + one stream: its own, or the caller's (``stream``: a
+    cudaStream_t as an integer, 0 the legacy default stream), which must outlive
+    the context."""
 
-    def __init__(self, device=0):
+    def __init__(self, device=0, stream=None):
         h = ctypes.c_void_p()
-        check(lib.alm_ctx_create(int(device), ctypes.byref(h)))
+        if stream is None:
+            check(lib.alm_ctx_create(int(device), ctypes.byref(h)))
+        else:
+            check(lib.alm_ctx_create_on_stream(int(device), int(stream) or None, ctypes.byref(h)))
         self.h = h
         self.device = device
 
     def sync(self):
+        """Wait for the stream; raises ALMError (ALM_ERR_RANGE) when an operator
+        on device data (``paged``) met a page, slot or position out of range."""
         check(lib.alm_ctx_sync(self.h))
 
     def set_persistent(self, enable):
@@ -89,10 +96,12 @@ class Context:
 _DEFAULT = {}
 
 
-def default_context(device=0):
-    ctx = _DEFAULT.get(device)
+def default_context(device=0, stream=None):
+    """The process's context of a device, or of one of the caller's streams."""
+    key = device if stream is None else (device, int(stream))
+    ctx = _DEFAULT.get(key)
     if ctx is None or ctx.h is None:
-        ctx = _DEFAULT[device] = Context(device)
+        ctx = _DEFAULT[key] = Context(device, stream)
     return ctx
 
 
@@ -527,6 +536,24 @@ class DeviceKV:
         k, v = np.empty(shape, np.float16), np.empty(shape, np.float16)
         check(lib.alm_kv_read_slot(self.h, int(slot), int(layer), int(pos0), int(n), ptr(k), ptr(v)))
         return k, v
+
+    def view(self, layer):
+        """The layer's pages as a ``paged.PagedKV`` for the operators on device
+        data; valid while this cache is open."""
+        from . import paged
+        return paged.PagedKV.of_view(self._view(layer)[0], self)
+
+    def page_table(self):
+        """The page table on the device (a row per slot) for ``paged.SeqBatch``."""
+        from . import paged
+        _, table, rows, pages = self._view(0)
+        return paged.PageTable(table, rows, pages, self)
+
+    def _view(self, layer):
+        view, table, rows, pages = PagedKVView(), ctypes.c_void_p(), ctypes.c_int32(), ctypes.c_int32()
+        check(lib.alm_kv_view(self.h, int(layer), ctypes.byref(view), ctypes.byref(table), ctypes.byref(rows),
+                              ctypes.byref(pages)))
+        return view, table.value, rows.value, pages.value
 
     def set_pages(self, slot, pages):
         """Map slot's first len(pages) pages to the given physical pages."""

@@ -1,0 +1,315 @@
+"""Operators of a batched step on device data: norms, rotation and the cache
+write of new rows (``rope_append``), attention of ragged batches over a paged
+cache (``attn_paged``), acceptance of drafted tokens (``verify``).
+
+Tensors are device arrays of the caller: objects with ``data_ptr()``,
+``shape``, ``stride()`` and ``dtype`` (torch tensors), objects with
+``__cuda_array_interface__``, or ``DeviceArray`` views of memory of the
+library.  Nothing here waits for the GPU: the calls run on the context's
+stream (``ops.default_context(device, stream)`` gives a context on the
+caller's own stream), can be captured into a CUDA graph, and a captured call
+reads the lengths, page numbers and draws that its device arrays hold when it
+is replayed.  What the device finds out of range is reported by the next
+``Context.sync()``.
+"""
+import ctypes
+
+import numpy as np
+
+from ._lib import AttnPagedArgs, PagedKVView, RopeAppendArgs, SeqBatchView, VerifyArgs, check, lib
+from .ops import DeviceBuffer
+
+F16, BF16, F32 = 0, 1, 2          # ALM_F16, ALM_BF16, ALM_F32
+I32, F64 = "int32", "float64"
+# type codes by the spellings of torch dtypes, numpy dtypes and array-interface type strings
+_NAMES = {"float16": F16, "bfloat16": BF16, "float32": F32, "int32": I32, "float64": F64,
+          "<f2": F16, "<f4": F32, "<i4": I32, "<f8": F64}
+_CODES = {}                       # dtype object -> code
+_SIZES = {F16: 2, BF16: 2, F32: 4, I32: 4, F64: 8}
+
+
+class DeviceArray:
+    """A typed, shaped view of device memory of the library (``buf``: an
+    ``ops.DeviceBuffer``; ``offset`` in bytes; contiguous)."""
+
+    def __init__(self, buf, shape, dtype, offset=0):
+        self.buf, self.shape, self.dtype, self.offset = buf, tuple(int(n) for n in shape), dtype, int(offset)
+        size = _SIZES[_code(dtype)]
+        if self.offset < 0 or self.offset + int(np.prod(self.shape, dtype=np.int64)) * size > buf.nbytes:
+            raise ValueError("the view ends behind its buffer")
+
+    def data_ptr(self):
+        return self.buf.h.value + self.offset
+
+    def stride(self):
+        out, n = [], 1
+        for d in reversed(self.shape):
+            out.append(n)
+            n *= d
+        return tuple(reversed(out))
+
+
+def _code(dtype):
+    try:
+        return _CODES[dtype]
+    except (KeyError, TypeError):
+        pass
+    name = dtype if isinstance(dtype, str) else str(dtype)
+    code = _NAMES.get(name.replace("torch.", ""))
+    if code is None and not isinstance(dtype, str):
+        try:
+            code = _NAMES.get(np.dtype(dtype).name)
+        except TypeError:
+            pass
+    if code is None:
+        raise TypeError(f"unsupported element type {name}")
+    try:
+        _CODES[dtype] = code
+    except TypeError:
+        pass
+    return code
+
+
+def _array(a, what, codes, ndim, device=None):
+    """(pointer, type code, shape, strides in elements) of a device array."""
+    if hasattr(a, "data_ptr"):
+        dev = getattr(a, "device", None)
+        if dev is not None:
+            if getattr(dev, "type", "cuda") != "cuda":
+                raise ValueError(f"{what} must be on a CUDA device")
+            if device is not None and dev.index is not None and dev.index != device:
+                raise ValueError(f"{what} is on device {dev.index}, the context on device {device}")
+        p, shape, stride, code = a.data_ptr(), a.shape, a.stride(), _code(a.dtype)
+    elif hasattr(a, "__cuda_array_interface__"):
+        i = a.__cuda_array_interface__
+        p, shape, code = i["data"][0], tuple(i["shape"]), _code(i["typestr"])
+        size = _SIZES[code]
+        if i.get("strides") is None:
+            stride, n = [], 1
+            for d in reversed(shape):
+                stride.append(n)
+                n *= d
+            stride = tuple(reversed(stride))
+        else:
+            if any(s % size for s in i["strides"]):
+                raise ValueError(f"{what} has strides that are not whole elements")
+            stride = tuple(s // size for s in i["strides"])
+    else:
+        raise TypeError(f"{what} must be a device array (data_ptr() or __cuda_array_interface__)")
+    if code not in codes:
+        raise TypeError(f"{what} has an unsupported element type")
+    if len(shape) != ndim:
+        raise ValueError(f"{what} must have {ndim} dimensions")
+    return p, code, shape, stride
+
+
+def _dense(shape, stride):
+    n = 1
+    for d, s in zip(reversed(shape), reversed(stride)):
+        if d != 1 and s != n:
+            return False
+        n *= d
+    return True
+
+
+def _contiguous(a, what, codes, ndim, device=None):
+    p, code, shape, stride = _array(a, what, codes, ndim, device)
+    if not _dense(shape, stride):
+        raise ValueError(f"{what} must be contiguous")
+    return p, code, shape
+
+
+def _rows(a, what, code, n_rows, heads, dim, device):
+    """(pointer, row stride, head stride) of a (rows, heads, dim) array."""
+    p, _, shape, stride = _array(a, what, (code,), 3, device)
+    if shape[0] != n_rows or shape[2] != dim or (heads is not None and shape[1] != heads):
+        want = f"({n_rows}, {'heads' if heads is None else heads}, {dim})"
+        raise ValueError(f"{what} must be {want}, not {tuple(shape)}")
+    if stride[2] != 1 and dim > 1:
+        raise ValueError(f"{what} must be contiguous in its last dimension")
+    # a stride nothing is stepped with may be any number
+    return p, stride[0] if n_rows > 1 else 0, stride[1] if shape[1] > 1 else 0
+
+
+class PagedKV:
+    """One layer's pages: K and V (n_pages, kv_heads, page_size, head_dim),
+    contiguous, fp16 or bf16.  ``DeviceKV.view(layer)`` gives a model's own."""
+
+    def __init__(self, k, v, device=None):
+        kp, code, shape = _contiguous(k, "k", (F16, BF16), 4, device)
+        vp, vcode, vshape = _contiguous(v, "v", (F16, BF16), 4, device)
+        if vcode != code or tuple(vshape) != tuple(shape):
+            raise ValueError("k and v must have the same type and shape")
+        self.code = code
+        self.n_pages, self.kv_heads, self.page_size, self.head_dim = (int(n) for n in shape)
+        self.c = PagedKVView(kp, vp, code, self.n_pages, self.page_size, self.kv_heads, self.head_dim)
+        self.ref = ctypes.addressof(self.c)
+        self._keep = (k, v)
+
+    @classmethod
+    def of_view(cls, view, keep):
+        self = cls.__new__(cls)
+        self.code = view.dtype
+        self.n_pages, self.kv_heads = view.n_pages, view.kv_heads
+        self.page_size, self.head_dim = view.page_size, view.head_dim
+        self.c, self._keep = view, keep
+        self.ref = ctypes.addressof(view)
+        return self
+
+
+class PageTable:
+    """The page table of a model's cache (``DeviceKV.page_table()``): row s
+    holds slot s's page numbers."""
+
+    def __init__(self, pointer, rows, pages, keep):
+        self.pointer, self.rows, self.pages, self._keep = pointer, rows, pages, keep
+
+
+class SeqBatch:
+    """The sequences of one pass.  ``row_start`` (n_seq + 1, int32): sequence
+    s owns rows row_start[s] .. row_start[s + 1] - 1 of the packed row tensors;
+    they are the last of its ``kv_len[s]`` (int32) positions.  ``page_table``
+    (int32, a row per sequence, or per slot with ``slots``; or a
+    ``PageTable``): position p lies on page page_table[s][p // page_size].
+    ``n_rows``: rows of the packed tensors (rows behind the last sequence stay
+    as they are).  ``max_rows`` bounds the rows of one sequence; it chooses
+    the attention kernel.  All arrays stay on the device, so a captured pass
+    can be replayed with new contents."""
+
+    def __init__(self, row_start, kv_len, page_table, n_rows, max_rows=None, slots=None, device=None):
+        rp, _, rs = _contiguous(row_start, "row_start", (I32,), 1, device)
+        lp, _, ls = _contiguous(kv_len, "kv_len", (I32,), 1, device)
+        n_seq = int(ls[0])
+        if rs[0] != n_seq + 1:
+            raise ValueError("row_start must have one entry more than kv_len")
+        if isinstance(page_table, PageTable):
+            tp, rows, pages, step = page_table.pointer, page_table.rows, page_table.pages, page_table.pages
+        else:
+            tp, _, shape, stride = _array(page_table, "page_table", (I32,), 2, device)
+            rows, pages = int(shape[0]), int(shape[1])
+            if pages > 1 and stride[1] != 1:
+                raise ValueError("page_table must be contiguous in its last dimension")
+            step = int(stride[0]) if rows > 1 else pages
+            if step < pages:
+                raise ValueError("page_table rows must not overlap")
+        sp = None
+        if slots is not None:
+            sp, _, ss = _contiguous(slots, "slots", (I32,), 1, device)
+            if ss[0] != n_seq:
+                raise ValueError("slots must have an entry for every sequence")
+        elif rows < n_seq:
+            raise ValueError("page_table must have a row for every sequence")
+        self.n_seq, self.n_rows = n_seq, int(n_rows)
+        if self.n_rows < 0:
+            raise ValueError("n_rows must not be negative")
+        most = self.n_rows if max_rows is None else int(max_rows)
+        self.c = SeqBatchView(n_seq, self.n_rows, most, rows, pages, step, rp, lp, tp, sp)
+        self.ref = ctypes.addressof(self.c)
+        self._keep = (row_start, kv_len, page_table, slots)
+
+
+class AttnWorkspace:
+    """Work area of ``attn_paged`` (partial results of sequences that several
+    CTAs share), for any batch of these heads.  Calls that can overlap on the
+    GPU, graphs replayed on different streams among them, need one each."""
+
+    def __init__(self, ctx, heads, kv_heads, head_dim):
+        n = ctypes.c_size_t()
+        check(lib.alm_attn_paged_work(ctx.h, int(heads), int(kv_heads), int(head_dim), ctypes.byref(n)))
+        self.buf = DeviceBuffer(ctx, n.value)
+        self.pointer, self.nbytes = self.buf.h.value, n.value
+
+
+def rope_append(ctx, kv, seqs, q, k, v, rope, q_out, q_norm=None, k_norm=None, eps=1e-6, interleaved=False):
+    """alm_rope_append: norm (optional) and rotate the heads of q and k, write
+    q to ``q_out`` and K / V to the cache.  q, q_out (n_rows, heads, head_dim),
+    k, v (n_rows, kv_heads, head_dim): the cache's type, any row and head
+    strides that are multiples of 8; q_out may be q.  rope (positions,
+    rot_dim): [cos | sin], fp16, bf16 or fp32; interleaved rotates neighbours
+    (2i, 2i + 1) instead of halves (i, i + rot_dim / 2)."""
+    dev, n, d, code = ctx.device, seqs.n_rows, kv.head_dim, kv.code
+    qp, qr, qh = _rows(q, "q", code, n, None, d, dev)
+    kp, kr, kh = _rows(k, "k", code, n, kv.kv_heads, d, dev)
+    vp, vr, vh = _rows(v, "v", code, n, kv.kv_heads, d, dev)
+    heads = int(q.shape[1])
+    op, o_r, oh = _rows(q_out, "q_out", code, n, heads, d, dev)
+    rp, rcode, rs = _contiguous(rope, "rope", (F16, BF16, F32), 2, dev)
+    np_ = [None, None]
+    for i, (w, what) in enumerate(((q_norm, "q_norm"), (k_norm, "k_norm"))):
+        if w is not None:
+            np_[i], _, ws = _contiguous(w, what, (code,), 1, dev)
+            if ws[0] != d:
+                raise ValueError(f"{what} must have head_dim entries")
+    a = RopeAppendArgs(qp, kp, vp, qr, qh, kr, kh, vr, vh, op, o_r, oh, heads, np_[0], np_[1], eps, rp, rcode,
+                       rs[0], rs[1], 1 if interleaved else 0)
+    check(lib.alm_rope_append(ctx.h, kv.ref, seqs.ref, ctypes.addressof(a)))
+
+
+def attn_paged(ctx, kv, seqs, q, out, work, scale=None, window=0, lse=None):
+    """alm_attn_paged: out[r] = softmax(scale q[r] . K) V over the positions of
+    row r's sequence up to its own (the last ``window`` of them when window >
+    0).  q, out (n_rows, heads, head_dim) of the cache's type; scale defaults
+    to head_dim ** -0.5; lse (n_rows, heads) fp32 receives the log of the sum
+    of exponentials.  Rows that see nothing get zeros and -inf."""
+    dev, n, d, code = ctx.device, seqs.n_rows, kv.head_dim, kv.code
+    qp, qr, qh = _rows(q, "q", code, n, None, d, dev)
+    heads = int(q.shape[1])
+    op, o_r, oh = _rows(out, "out", code, n, heads, d, dev)
+    lp, ls = None, 0
+    if lse is not None:
+        lp, _, shape, stride = _array(lse, "lse", (F32,), 2, dev)
+        if shape[0] != n or shape[1] != heads or (heads > 1 and stride[1] != 1):
+            raise ValueError("lse must be (n_rows, heads), contiguous in its last dimension")
+        ls = stride[0]
+    a = AttnPagedArgs(qp, qr, qh, op, o_r, oh, lp, ls, heads, window, d ** -0.5 if scale is None else scale,
+                      work.pointer, work.nbytes)
+    check(lib.alm_attn_paged(ctx.h, kv.ref, seqs.ref, ctypes.addressof(a)))
+
+
+def verify(ctx, row_start, logits, draft_tokens, draft_probs, uniforms, temperature, tokens, n_accepted,
+           min_p=None, p_draft=None):
+    """alm_verify: accept drafted tokens while u q(x) < p(x), then draw from
+    the residual (or the bonus row), for a ragged batch.  row_start (n_seq + 1,
+    int32): sequence s owns rows row_start[s] .. row_start[s + 1] - 1 of logits
+    (n_rows, vocab): one per drafted token and one more.  draft_tokens (n_seq,
+    k_max) int32; draft_probs (n_seq, k_max, vocab) fp32 or None (certain
+    drafts); uniforms (n_seq, k_max + 1) float64; temperature, min_p (n_seq)
+    fp32, temperature <= 0 greedy.  Writes tokens (n_seq, k_max + 1) int32 (-1
+    behind the emitted ones), n_accepted (n_seq) int32 and p_draft (n_seq,
+    k_max) fp32."""
+    dev = ctx.device
+    lp, lcode, ls, lstride = _array(logits, "logits", (F16, BF16, F32), 2, dev)
+    n_rows, vocab = ls
+    if vocab > 1 and lstride[1] != 1:
+        raise ValueError("logits must be contiguous in the last dimension")
+    dp, _, ds = _contiguous(draft_tokens, "draft_tokens", (I32,), 2, dev)
+    n_seq, k = ds
+    rp, _, rs = _contiguous(row_start, "row_start", (I32,), 1, dev)
+    if rs[0] != n_seq + 1:
+        raise ValueError("row_start must have n_seq + 1 entries")
+    qp, q_seq, q_step = None, 0, 0
+    if draft_probs is not None:
+        qp, _, qs, qst = _array(draft_probs, "draft_probs", (F32,), 3, dev)
+        if tuple(qs) != (n_seq, k, vocab) or (vocab > 1 and qst[2] != 1):
+            raise ValueError("draft_probs must be (n_seq, k_max, vocab), contiguous in its last dimension")
+        q_seq, q_step = qst[0], qst[1]
+    up, _, us = _contiguous(uniforms, "uniforms", (F64,), 2, dev)
+    op, _, os_ = _contiguous(tokens, "tokens", (I32,), 2, dev)
+    if tuple(us) != (n_seq, k + 1) or tuple(os_) != (n_seq, k + 1):
+        raise ValueError("uniforms and tokens must be (n_seq, k_max + 1)")
+    tp, _, ts = _contiguous(temperature, "temperature", (F32,), 1, dev)
+    ap, _, as_ = _contiguous(n_accepted, "n_accepted", (I32,), 1, dev)
+    mp = pp = None
+    if min_p is not None:
+        mp, _, ms = _contiguous(min_p, "min_p", (F32,), 1, dev)
+        if ms[0] != n_seq:
+            raise ValueError("min_p must have n_seq entries")
+    if ts[0] != n_seq or as_[0] != n_seq:
+        raise ValueError("temperature and n_accepted must have n_seq entries")
+    if p_draft is not None:
+        pp, _, ps = _contiguous(p_draft, "p_draft", (F32,), 2, dev)
+        if tuple(ps) != (n_seq, k):
+            raise ValueError("p_draft must be (n_seq, k_max)")
+    a = VerifyArgs(n_seq, n_rows, k, vocab, rp, lp, lcode, lstride[0] if n_rows > 1 else vocab, dp, qp, q_seq, q_step,
+                   up, tp, mp, op, ap, pp)
+    check(lib.alm_verify(ctx.h, ctypes.addressof(a)))

@@ -46,7 +46,8 @@ enum {
   ALM_ERR_ARG = 1,    /* invalid argument (shape, range, null pointer) */
   ALM_ERR_CUDA = 2,   /* CUDA runtime error */
   ALM_ERR_STATE = 3,  /* object not ready (e.g. model layer missing) */
-  ALM_ERR_TOKEN = 4   /* a token id outside the vocabulary reached the device */
+  ALM_ERR_TOKEN = 4,  /* a token id outside the vocabulary reached the device */
+  ALM_ERR_RANGE = 5   /* a page, slot or position outside its range reached the device */
 };
 
 /* Human-readable description of the last error on this thread. */
@@ -58,7 +59,16 @@ ALM_API int alm_abi_version(void);
 /* Create a context (device + stream). */
 ALM_API int alm_ctx_create(int device, alm_ctx** out);
 ALM_API int alm_ctx_destroy(alm_ctx* ctx);
+/* Waits for the context's stream.  ALM_ERR_RANGE when an operator of the
+ * batched step (below) met a page, slot or position outside its range since
+ * the last alm_ctx_sync; the record is cleared. */
 ALM_API int alm_ctx_sync(alm_ctx* ctx);
+/* A context on the caller's CUDA stream (a cudaStream_t of `device`, NULL for
+ * the legacy default stream): the operators of the batched step are then
+ * ordered with the caller's own work and are captured with it.  The stream
+ * must outlive the context.  Models, whose speculative steps capture graphs,
+ * need a stream other than the legacy default one. */
+ALM_API int alm_ctx_create_on_stream(int device, void* stream, alm_ctx** out);
 /* Forwards of up to 8 rows as one persistent kernel (enable = 1) or as one
    launch per layer operation (enable = 0, the default; the environment
    variable ALM_PERSIST=1 turns the persistent kernel on at context creation).
@@ -394,6 +404,139 @@ ALM_API int alm_spec_set_rejection(alm_spec* s, int enable);
 ALM_API int alm_spec_set_uniforms(alm_spec* s, const double* uniforms_host, int n);
 /* Draws of the loaded stream consumed so far. */
 ALM_API int alm_spec_uniforms_used(alm_spec* s, int32_t* used);
+
+/* ---- operators of a batched step on device data ----------------------------------- */
+/* Element types of device tensors. */
+enum { ALM_F16 = 0, ALM_BF16 = 1, ALM_F32 = 2 };
+/* One layer's pages: k_dev and v_dev are (n_pages, kv_heads, page_size,
+ * head_dim) contiguous, 16-byte aligned, fp16 or bf16 (the layout of alm_kv).
+ * head_dim: 32, 64, 96, 128 or 256; page_size 1..65536. */
+typedef struct alm_paged_kv {
+  void *k_dev, *v_dev;
+  int dtype, n_pages, page_size, kv_heads, head_dim;
+} alm_paged_kv;
+/* The sequences of one pass, described on the device so that a captured
+ * graph can be replayed with new lengths.  Sequence s owns rows
+ * row_start_dev[s] .. row_start_dev[s + 1] - 1 of the packed row tensors
+ * (row_start_dev has n_seq + 1 entries, starts at 0 or above and does not
+ * decrease; a sequence may own no row) and they are the last of its
+ * kv_len_dev[s] positions.  Rows from row_start_dev[n_seq] to n_rows - 1
+ * belong to no sequence and are neither read nor written.  Position p of
+ * sequence s lies on page page_table_dev[t * page_stride + p / page_size]
+ * with t = s, or slots_dev[s] when slots_dev is not NULL; the table has
+ * table_rows rows of table_pages valid entries each, and positions behind
+ * table_pages * page_size do not exist.  max_rows: a bound on the rows of
+ * one sequence (it chooses the kernel; a sequence with more rows is still
+ * computed).  n_seq is at most 4096. */
+typedef struct alm_seq_batch {
+  int n_seq, n_rows, max_rows;
+  int table_rows, table_pages, page_stride;
+  const int32_t *row_start_dev, *kv_len_dev, *page_table_dev, *slots_dev;
+} alm_seq_batch;
+/* The pages of one layer of a model's cache and its page table (row s =
+ * slot s, *table_pages entries each, *table_rows rows), for the operators
+ * below.  The view stays valid until alm_kv_destroy. */
+ALM_API int alm_kv_view(alm_kv* kv, int layer, alm_paged_kv* view, const int32_t** page_table_dev, int* table_rows,
+                        int* table_pages);
+/* Head norms, position rotation and the cache write of a pass's new rows
+ * (no reference counterpart for batches; androidllm/models/llama.py:33-50,
+ * 108-115 rotates and writes one row).  q_dev (n_rows, heads, head_dim),
+ * k_dev and v_dev (n_rows, kv_heads, head_dim) have the cache's type,
+ * contiguous heads rows, and row / head strides in elements that are
+ * multiples of 8 (16-byte aligned vectors).  With q_norm_dev / k_norm_dev
+ * (head_dim, or NULL) each head is first divided by its root mean square
+ * (eps added to the mean) and multiplied by the weight.  rope_dev
+ * (rope_rows, rot_dim) holds cos for rot_dim / 2 angles, then sin, of every
+ * position, fp16, bf16 or fp32 (rope_dtype), 16-byte aligned; the first
+ * rot_dim (a multiple of 16, at most head_dim) values of a head are rotated:
+ * values i and i + rot_dim / 2 together, or 2i and 2i + 1 (interleaved = 1).
+ * q goes to q_out_dev (which may be q_dev itself with the same strides),
+ * K and unrotated V to the pages.  Arithmetic in fp32, rounded once.
+ * A row whose position is negative or not below rope_rows, or whose page is
+ * outside the table or the pool, is not written and is recorded for
+ * alm_ctx_sync.  Runs on the context's stream without waiting. */
+typedef struct alm_rope_append_args {
+  const void *q_dev, *k_dev, *v_dev;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;   /* strides in elements */
+  void* q_out_dev;
+  int64_t qo_row, qo_head;
+  int heads;
+  const void *q_norm_dev, *k_norm_dev;
+  float eps;
+  const void* rope_dev;
+  int rope_dtype, rope_rows, rot_dim, interleaved;
+} alm_rope_append_args;
+ALM_API int alm_rope_append(alm_ctx* ctx, const alm_paged_kv* kv, const alm_seq_batch* batch,
+                            const alm_rope_append_args* args);
+/* Attention of each sequence's rows over its positions in the cache
+ * (androidllm/models/llama.py:116-124 for many rows and sequences).  The row
+ * at position p sees positions max(0, p - window + 1) .. p (window = 0: 0 ..
+ * p).  heads is a multiple of kv_heads and at most 128 query heads share a
+ * K/V head.  q_dev and out_dev: (n_rows, heads, head_dim) of the cache's
+ * type, strides in elements, multiples of 8, 16-byte aligned; out_dev must
+ * not overlap q_dev.  lse_dev (optional, fp32, (n_rows, heads), row stride
+ * lse_row): log of the sum of exp(scale * q.k).  A row that sees no position
+ * (its position is negative) gets zeros and -inf.  Values behind a
+ * sequence's end and of pages of other sequences never reach a result, NaN
+ * and infinities included; nor does a value at a position that a row does not
+ * see.  A page outside the pool is read as zeros and recorded for
+ * alm_ctx_sync.  scale is positive.  work_dev: alm_attn_paged_work bytes, 256-byte
+ * aligned; calls that can overlap on the GPU, graphs replayed on
+ * different streams among them, need a work area each.  Runs on the
+ * context's stream without waiting; results do not change from run to run. */
+typedef struct alm_attn_paged_args {
+  const void* q_dev;
+  int64_t q_row, q_head;
+  void* out_dev;
+  int64_t out_row, out_head;
+  float* lse_dev;
+  int64_t lse_row;
+  int heads, window;
+  float scale;
+  void* work_dev;
+  size_t work_bytes;
+} alm_attn_paged_args;
+ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv, const alm_seq_batch* batch,
+                           const alm_attn_paged_args* args);
+/* Bytes of work area alm_attn_paged needs on this device for any batch. */
+ALM_API int alm_attn_paged_work(alm_ctx* ctx, int heads, int kv_heads, int head_dim, size_t* bytes);
+/* Acceptance of drafted tokens for a ragged batch (alm_accept's rule for
+ * many sequences, on device data, decided in 64 bits; androidllm/engine.py:
+ * 306-320 steps one sequence).  Sequence s owns logits rows row_start_dev[s]
+ * .. row_start_dev[s + 1] - 1 (fp16, bf16 or fp32, row stride logits_row): k
+ * rows that judge its k drafted tokens draft_tokens_dev[s * (k_max) + i], then
+ * one more; a sequence with no row emits nothing, rows that exceed k_max + 1
+ * are not looked at, k_max is at most 31.  draft_probs_dev[s * q_seq + i *
+ * q_step + x] (fp32) is the distribution token i was drawn from; NULL: the
+ * drafts are certain (probability 1 at the token).  uniforms_dev: k_max + 1
+ * draws in [0, 1) a sequence, one per drafted token and, at index k, the
+ * last draw.  p = softmax(l / temperature_dev[s]) of a row, without entries
+ * below min_p_dev[s] (or NULL: 0) times the largest.  Token i is accepted
+ * iff u_i q_i(x_i) < p_i(x_i); at the first refusal a token is drawn from
+ * max(0, p_i - q_i) (from p_i if that is zero everywhere), after k
+ * acceptances from p_k: the first index whose running sum exceeds the last
+ * draw times the total.  temperature <= 0 is greedy: the mass lies on the
+ * first largest logit.  NaN logits count as -inf, +inf logits share the mass
+ * among themselves; in a row without a finite or +inf logit nothing can be
+ * accepted or drawn, and the token is -1.  tokens_dev (n_seq, k_max + 1): the accepted tokens, the
+ * drawn one, then -1; n_accepted_dev (n_seq).  p_draft_dev (n_seq, k_max, or
+ * NULL): p_i(x_i), 0 behind k.  A drafted token outside the vocabulary has
+ * p = 0.  Runs on the context's stream without waiting. */
+typedef struct alm_verify_args {
+  int n_seq, n_rows, k_max, vocab;
+  const int32_t* row_start_dev;
+  const void* logits_dev;
+  int logits_dtype;
+  int64_t logits_row;
+  const int32_t* draft_tokens_dev;
+  const float* draft_probs_dev;
+  int64_t q_seq, q_step;
+  const double* uniforms_dev;
+  const float *temperature_dev, *min_p_dev;
+  int32_t *tokens_dev, *n_accepted_dev;
+  float* p_draft_dev;
+} alm_verify_args;
+ALM_API int alm_verify(alm_ctx* ctx, const alm_verify_args* args);
 
 /* ---- measurement ---------------------------------------------------------------- */
 /* Replay n_steps speculative steps back to back and time them with CUDA
