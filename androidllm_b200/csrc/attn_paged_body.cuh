@@ -162,7 +162,7 @@ attn_paged_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv, int* er
   const int tpu = kRows / a.group;
   const int cta = blockIdx.x;
   sched_init<kTile>(
-      b, kv, tpu, a.window, a.min_rows, a.max_rows, sched,
+      b, kv, tpu, a.window, sched,
       [&](long long total) {
         const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
         return cta < n ? share(total, cta, n) : -1ll;
@@ -187,23 +187,28 @@ attn_paged_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv, int* er
       const uint32_t dst = smem0 + stage * S::kStageBytes;
       const int base = (lu.t0 + lt) * kTile;
       constexpr int kIter = kTile * kUnits16 / kPagedThreads;
+      // the page numbers first, all in flight together
+      int page[kIter];
+#pragma unroll
+      for (int i = 0; i < kIter; ++i) {
+        const int pos = base + (tid + i * kPagedThreads) / kUnits16;
+        page[i] = pos < lu.n_kv && lu.pages ? __ldg(lu.pages + page_of(kv, pos)) : -1;
+      }
 #pragma unroll
       for (int i = 0; i < kIter; ++i) {
         const int idx = tid + i * kPagedThreads;
         const int r = idx / kUnits16, c = idx % kUnits16;
         const int pos = base + r;
-        const int pi = page_of(kv, pos);
-        const bool in = pos < lu.n_kv;
-        const int page = in && lu.pages ? __ldg(lu.pages + pi) : -1;
-        const bool ok = page >= 0 && page < kv.n_pages;
-        bad_page |= in && !ok;
-        const size_t off = (ok ? kv_offset(kv, page, lu.h, pos - pi * kv.page_size) + c * 8 : 0) * sizeof(T);
+        const bool ok = page[i] >= 0 && page[i] < kv.n_pages;
+        bad_page |= !ok && pos < lu.n_kv;
+        const size_t off =
+            (ok ? kv_offset(kv, page[i], lu.h, pos - page_of(kv, pos) * kv.page_size) + c * 8 : 0) * sizeof(T);
         cp_async16(dst + r * S::kPitch + c * 16, kv.k + off, ok ? 16 : 0);
         cp_async16(dst + (kTile + r) * S::kPitch + c * 16, kv.v + off, ok ? 16 : 0);
       }
       ++lx;
       if (++lt == lu.n_tile && lx < x1) {
-        next_unit<kTile>(b, kv, tpu, a.window, a.min_rows, a.max_rows, lu);
+        next_unit<kTile>(b, kv, tpu, a.window, lu);
         lt = 0;
       }
     }
@@ -438,7 +443,7 @@ attn_paged_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv, int* er
       }
     }
     if (x + 1 < x1) {
-      next_unit<kTile>(b, kv, tpu, a.window, a.min_rows, a.max_rows, u);
+      next_unit<kTile>(b, kv, tpu, a.window, u);
       t = t_first = 0;
       begin_unit();
     }
@@ -448,16 +453,17 @@ attn_paged_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv, int* er
 }
 
 // Joins the partial results of the unit that CTA blockIdx.x began and did not
-// finish: rows 8 blockIdx.y + warp.  Partials are added in CTA order.
-template <typename T, int HD, int TILE, int ROWS>
+// finish: rows 8 blockIdx.y + warp.  Partials are added in CTA order.  A unit's
+// ROWS rows are blocks of BLK rows, whole tokens each.
+template <typename T, int HD, int TILE, int ROWS, int BLK>
 __global__ void __launch_bounds__(kPagedThreads)
 attn_paged_join_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv) {
   __shared__ SchedShared sched;
   const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-  const int tpu = ROWS / a.group, cta = blockIdx.x;
+  const int tq = BLK / a.group, tpu = ROWS / BLK * tq, cta = blockIdx.x;
   long long x0 = 0, x1 = 0;
   sched_init<TILE>(
-      b, kv, tpu, a.window, a.min_rows, a.max_rows, sched,
+      b, kv, tpu, a.window, sched,
       [&](long long total) {
         const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
         if (cta >= n) return -1ll;
@@ -479,8 +485,8 @@ attn_paged_join_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv) {
   int last = cta + 1;   // the CTA that holds the unit's last tile
   while (share(total, last + 1, n_cta) < u.start + u.n_tile) ++last;
   const int row = blockIdx.y * kPagedWarps + warp;
-  const int tok = row / a.group, head = u.h * a.group + row - tok * a.group;
-  if (tok >= u.n_tok) return;
+  const int tk = row % BLK / a.group, tok = row / BLK * tq + tk, head = u.h * a.group + row % BLK - tk * a.group;
+  if (tk >= tq || tok >= u.n_tok) return;
   const int n = last - cta + 1;
 
   auto part = [&](int i) { return partial_at<HD>(a.work, ROWS, cta + i, i == 0 ? 1 : 0); };
@@ -542,7 +548,7 @@ cudaError_t paged_attr_all() {
   return e;
 }
 
-template <typename T, int HD, int TILE, int ROWS>
+template <typename T, int HD, int TILE, int ROWS, int BLK>
 cudaError_t launch_join(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.n_cta, ROWS / kPagedWarps, 1);
@@ -553,7 +559,7 @@ cudaError_t launch_join(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<T, HD, TILE, ROWS>, a, b, kv);
+  return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<T, HD, TILE, ROWS, BLK>, a, b, kv);
 }
 
 template <typename T, int HD, int WM>
@@ -561,7 +567,7 @@ cudaError_t launch_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& k
   using S = PagedShape<HD, WM>;
   attn_paged_kernel<T, HD, WM><<<a.n_cta, kPagedThreads, S::kSmem, st>>>(a, b, kv, err);
   const cudaError_t e = cudaGetLastError();
-  return e != cudaSuccess ? e : launch_join<T, HD, S::kTile, S::kRows>(a, b, kv, st);
+  return e != cudaSuccess ? e : launch_join<T, HD, S::kTile, S::kRows, S::kRows>(a, b, kv, st);
 }
 
 // The smallest row block that holds the longest sequence's rows: K and V are

@@ -1,0 +1,682 @@
+// Attention of many new rows over the paged cache (alm_attn_paged) on the
+// fifth-generation tensor cores; instantiated in attn_paged_tc_f16.cu and
+// attn_paged_tc_bf16.cu.  The mathematics and the sharing of tiles are those of
+// attn_paged_body.cuh; here 128 rows (tokens times the query heads of one K/V
+// head) are the M of a tcgen05.mma:
+//
+//   S (128 x 128 positions, tensor memory) = Q (shared memory) . K^T
+//   P = 2^(c S - c m), written over S as 16-bit values
+//   O (128 x head_dim, tensor memory) += P (tensor memory) . V
+//
+// Two streams alternate, so that one's softmax runs under the other's
+// products: with kNQ = 2 they are two 128-row blocks over the same K and V
+// tiles, with kNQ = 1 (at most 128 rows in a sequence) the even and the odd
+// tiles of one block, joined at the unit's end.
+//
+// Warps 0-3 and 4-7: softmax of stream 0 and 1, one row a thread.  Warp 8:
+// issues the products.  Warp 9: loads K and V tiles with TMA, one box per page
+// piece and 64 columns, into a ring of tiles in the order they are used.
+//
+// The reference maximum m follows the row's maximum only when that has grown
+// by more than kSlack (in powers of two): weights stay below 2^kSlack, and the
+// rescaling of O, which has to wait for the last product, is rare.  Tensor
+// and exponential units bound long chunks (at 128 x 128 x 128 both take
+// about 512 cycles of an SM), HBM short ones.
+#pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_paged_body.cuh"
+#include "tc.cuh"
+
+namespace alm {
+
+constexpr int kTcPagedThreads = 320;
+constexpr float kSlack = 8.f;
+
+template <int HD, int NQ>
+struct TcShape {
+  static constexpr int kTile = 128;
+  static constexpr int kChunks = HD / 64;                  // 128-byte column groups
+  static constexpr int kTileBytes = 128 * HD * 2;          // Q block, K or V tile
+  static constexpr int kSlots = HD == 128 ? (NQ == 2 ? 5 : 6) : 10;
+  static constexpr size_t kSmem = static_cast<size_t>(NQ + kSlots) * kTileBytes + 1024;
+  static constexpr int kColS = 0, kColO = 256, kTmemCols = 512;
+};
+
+struct TcShared {
+  SchedShared sched;
+  uint64_t full[10], empty[10];
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
+  uint32_t tmem;
+  int dead;      // a wait ran out: everybody leaves
+};
+
+ALM_DEV uint64_t sdesc128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return tc_sdesc(addr, lbo, sbo) | (static_cast<uint64_t>(2) << 61);   // SWIZZLE_128B
+}
+ALM_DEV void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc ? 1 : 0)
+      : "memory");
+}
+ALM_DEV void tc_ld32(uint32_t taddr, uint32_t (&d)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]),
+        "=r"(d[9]), "=r"(d[10]), "=r"(d[11]), "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15]), "=r"(d[16]),
+        "=r"(d[17]), "=r"(d[18]), "=r"(d[19]), "=r"(d[20]), "=r"(d[21]), "=r"(d[22]), "=r"(d[23]), "=r"(d[24]),
+        "=r"(d[25]), "=r"(d[26]), "=r"(d[27]), "=r"(d[28]), "=r"(d[29]), "=r"(d[30]), "=r"(d[31])
+      : "r"(taddr));
+}
+ALM_DEV void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      : "memory");
+}
+ALM_DEV void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+// Instruction descriptor: fp32 accumulator, A and B of type T, N wide; bmn: B
+// is stored with N contiguous (V: positions by head dimensions).
+template <typename T>
+constexpr uint32_t tc_idesc(int n, bool bmn) {
+  const uint32_t f = sizeof(T) == 2 && !std::is_same<T, half>::value ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((bmn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+template <typename T, int HD, int NQ>
+__global__ void __launch_bounds__(kTcPagedThreads, 1)
+attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                     const AttnPaged a, const SeqBatch b, const PagedKV kv, int box_rows, int* err) {
+  using S = TcShape<HD, NQ>;
+  extern __shared__ char smem_raw[];
+  __shared__ TcShared sh;
+  const uint32_t smem0 = (smem_addr(smem_raw) + 1023) & ~1023u;
+  char* const smem = smem_raw + (smem0 - smem_addr(smem_raw));
+  const uint32_t ring0 = smem0 + NQ * S::kTileBytes;
+  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
+  const int cta = blockIdx.x;
+  const int tq = 128 / a.group;      // tokens a 128-row block
+  const int tpu = NQ * tq;
+
+  grid_dep_launch();
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int i = 0; i < S::kSlots; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sh.q_full[i], NQ == 2 ? 128 : 256);
+        mbar_init(&sh.s_full[i], 1);
+        mbar_init(&sh.p_full[i], 128);
+        mbar_init(&sh.pv_done[i], 1);
+      }
+      sh.dead = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tc_alloc(&sh.tmem, S::kTmemCols);
+  } else if (warp < 8) {
+    sched_init<S::kTile>(
+        b, kv, tpu, a.window, sh.sched,
+        [&](long long total) {
+          const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
+          return cta < n ? share(total, cta, n) : -1ll;
+        },
+        [] { bar_sync(1, kSchedThreads); });
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const long long total = sh.sched.total;
+  const int n_cta = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
+  const long long x0 = cta < n_cta ? share(total, cta, n_cta) : 0;
+  const long long x1 = cta < n_cta ? share(total, cta + 1, n_cta) : 0;
+
+  volatile int* dead = &sh.dead;
+  // by whole warps, so that a wait that runs out ends for all lanes alike
+  auto gone = [&] { return __any_sync(0xffffffffu, *dead != 0) != 0; };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!gone() && !mbar_wait(bar, parity & 1)) {
+      *dead = 1;
+      *err = 2;
+    }
+    __syncwarp();
+  };
+
+  if (x0 < x1) {
+    Unit u = unit_at<S::kTile>(b, kv, tpu, a.window, sh.sched.found_seq, sh.sched.found_at, x0);
+    // this CTA's tiles [ta, tb) of the unit
+    int ta = static_cast<int>(x0 - u.start);
+    int tb = static_cast<int>(min(x1 - u.start, static_cast<long long>(u.n_tile)));
+    auto next = [&] {
+      next_unit<S::kTile>(b, kv, tpu, a.window, u);
+      ta = 0;
+      tb = static_cast<int>(min(x1 - u.start, static_cast<long long>(u.n_tile)));
+    };
+    auto more = [&] { return u.start + u.n_tile < x1; };
+
+    if (warp == 9) {
+      // ---- loads ---------------------------------------------------------------
+      int at = 0;
+      uint32_t round = 0;
+      bool bad = false;
+      const int rows_total = kv.n_pages * kv.kv_heads * kv.page_size;
+      const int n_box = 128 / box_rows * S::kChunks;
+      auto load = [&](const CUtensorMap* map, int t) {
+        // one box a lane: at most 128 / 8 pieces of at most 2 column groups
+        const int box = lane / S::kChunks, c = lane % S::kChunks;
+        const int pos = (u.t0 + t) * S::kTile + box * box_rows;
+        const bool in = lane < n_box && pos < u.n_kv;
+        const int pi = page_of(kv, pos);
+        const int page = in && u.pages ? __ldg(u.pages + pi) : -1;
+        const bool ok = page >= 0 && page < kv.n_pages;
+        bad |= in && !ok;
+        // a row behind the tensor's end reads zeros
+        const int y = ok ? (page * kv.kv_heads + u.h) * kv.page_size + pos - pi * kv.page_size : rows_total;
+        wait(&sh.empty[at], round ^ 1);
+        if (gone()) return;
+        if (lane == 0) mbar_expect_tx(&sh.full[at], S::kTileBytes);
+        __syncwarp();
+        if (lane < n_box)
+          tma_2d(ring0 + at * S::kTileBytes + c * (128 * 128) + box * box_rows * 128, map, c * 64, y, &sh.full[at]);
+        __syncwarp();
+        if (++at == S::kSlots) at = 0, round ^= 1;
+      };
+      if (NQ == 2) {
+        load(&k_map, ta);
+        for (bool go = true; go;) {
+          for (int t = ta; t < tb; ++t) {
+            load(&v_map, t);
+            if (t + 1 < tb) load(&k_map, t + 1);
+          }
+          go = more();
+          if (go) {
+            next();
+            load(&k_map, ta);
+          }
+        }
+      } else {
+        for (bool go = true; go;) {
+          load(&k_map, ta);
+          if (ta + 1 < tb) load(&k_map, ta + 1);
+          for (int t = ta; t < tb; ++t) {
+            load(&v_map, t);
+            if (t + 2 < tb) load(&k_map, t + 2);
+          }
+          go = more();
+          if (go) next();
+        }
+      }
+      if (bad) *err = 1;
+      // whatever happened, no copy is in flight when the CTA leaves: a slot's
+      // last fill is complete once its barrier has left that phase
+      if (gone()) {
+        for (int i = 0; i < S::kSlots; ++i) {
+          mbar_wait(&sh.full[i], 0);
+          mbar_wait(&sh.full[i], 1);
+        }
+      }
+    } else if (warp == 8) {
+      // ---- products ------------------------------------------------------------
+      const uint32_t id_s = tc_idesc<T>(128, false), id_o = tc_idesc<T>(HD, true);
+      int at = 0;
+      uint32_t round = 0;
+      uint32_t n_p[2] = {0, 0}, n_q[2] = {0, 0};
+      auto step_ring = [&] {
+        if (++at == S::kSlots) at = 0, round ^= 1;
+      };
+      // S of stream i from the K tile in the current slot
+      auto qk = [&](int i) {
+        if (lane == 0) {
+          const uint32_t qa = smem0 + (NQ == 2 ? i : 0) * S::kTileBytes, ka = ring0 + at * S::kTileBytes;
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
+            tc_mma_ss(tmem + S::kColS + i * 128, sdesc128(qa + off, 16, 1024), sdesc128(ka + off, 16, 1024), id_s,
+                      k > 0);
+          }
+          tc_commit(&sh.s_full[i]);
+        }
+        __syncwarp();
+      };
+      // O of stream i += P . V tile in the current slot
+      auto pv = [&](int i, bool acc) {
+        if (lane == 0) {
+          const uint32_t va = ring0 + at * S::kTileBytes;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)   // 16 positions: two groups of 8 rows of 128 bytes
+            tc_mma_ts(tmem + S::kColO + i * HD, tmem + S::kColS + i * 128 + 8 * k,
+                      sdesc128(va + k * 2048, 128 * 128, 1024), id_o, acc || k > 0);
+          tc_commit(&sh.pv_done[i]);
+        }
+        __syncwarp();
+      };
+      auto release = [&] {
+        if (lane == 0) tc_commit(&sh.empty[at]);
+        __syncwarp();
+        step_ring();
+      };
+      // The V tile t: rows behind the sequence's end that came with its last
+      // page hold anything, and a zero weight times NaN is NaN: clear them.
+      auto v_ready = [&](int t) {
+        wait(&sh.full[at], round);
+        const int base = (u.t0 + t) * S::kTile;
+        if (base + S::kTile > u.n_kv && !gone()) {
+          const int r0 = max(u.n_kv - base, 0);
+          const int r1 = min(S::kTile, (r0 + box_rows - 1) / box_rows * box_rows);
+          char* v = smem + (NQ + at) * S::kTileBytes;
+          for (int i = lane; i < (r1 - r0) * 8; i += kWarp)
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+              *reinterpret_cast<uint4*>(v + c * (128 * 128) + (r0 + i / 8) * 128 + (i % 8) * 16) =
+                  make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        tc_fence_after();
+      };
+      auto k_ready = [&] {
+        wait(&sh.full[at], round);
+        tc_fence_after();
+      };
+      auto p_ready = [&](int i) {
+        wait(&sh.p_full[i], n_p[i]++);
+        tc_fence_after();
+      };
+      auto q_ready = [&](int i) {
+        wait(&sh.q_full[i], n_q[i]++);
+        tc_fence_after();
+      };
+      if (NQ == 2) {
+        q_ready(0);
+        k_ready();
+        qk(0);
+        q_ready(1);
+        qk(1);
+        release();
+        for (bool go = true; go && !gone();) {
+          const bool last_unit = !more();
+          for (int t = ta; t < tb && !gone(); ++t) {
+            const int v_at = at;
+            const uint32_t v_round = round;
+            const bool another = t + 1 < tb || !last_unit;
+            p_ready(0);
+            v_ready(t);
+            pv(0, t > ta);
+            step_ring();
+            if (another) {
+              if (t + 1 == tb) q_ready(0);
+              k_ready();
+              qk(0);
+            }
+            const int k_at = at;
+            const uint32_t k_round = round;
+            p_ready(1);
+            at = v_at, round = v_round;
+            pv(1, t > ta);
+            release();
+            at = k_at, round = k_round;
+            if (another) {
+              if (t + 1 == tb) q_ready(1);
+              qk(1);
+              release();
+            }
+          }
+          go = !last_unit;
+          if (go) next();
+        }
+      } else {
+        for (bool go = true; go && !gone();) {
+          q_ready(0);
+          k_ready();
+          qk(0);
+          release();
+          if (ta + 1 < tb) {
+            k_ready();
+            qk(1);
+            release();
+          }
+          for (int t = ta; t < tb && !gone(); ++t) {
+            const int i = (t - ta) & 1;
+            p_ready(i);
+            v_ready(t);
+            pv(i, t - ta >= 2);
+            release();
+            if (t + 2 < tb) {
+              k_ready();
+              qk(i);
+              release();
+            }
+          }
+          go = more();
+          if (go) next();
+        }
+      }
+    } else {
+      // ---- softmax -------------------------------------------------------------
+      const int st = warp / 4;                         // stream
+      const int r = tid % 128;                         // row of the block = lane of tensor memory
+      const uint32_t t_s = tc_addr(tmem + S::kColS + st * 128, (warp % 4) * 32, 0);
+      const uint32_t t_o = tc_addr(tmem + S::kColO + st * HD, (warp % 4) * 32, 0);
+      const int blk = NQ == 2 ? st : 0;                // 128-row block of the unit
+      uint32_t n_s = 0;                                // tiles of this stream so far
+
+      // Q block `blk` into shared memory, 16 bytes a thread and step, in the
+      // swizzled layout TMA gives K (row r at 128 r, its 16-byte column c at c ^ (r mod 8))
+      auto load_q = [&] {
+        constexpr int kUnits = HD / 8;
+        char* q_s = smem + blk * S::kTileBytes;
+        constexpr int kStep = NQ == 2 ? 128 : 256;
+        const int t0 = NQ == 2 ? r : tid;
+#pragma unroll 4
+        for (int i = t0; i < 128 * kUnits; i += kStep) {
+          const int row = i / kUnits, c = i % kUnits;
+          const int tk = row / a.group, tok = blk * tq + tk, head = u.h * a.group + row - tk * a.group;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (tk < tq && tok < u.n_tok)
+            v = __ldg(reinterpret_cast<const uint4*>(a.q + (u.row0 + tok) * a.q_row + head * a.q_head) + c);
+          *reinterpret_cast<uint4*>(q_s + (c / 8) * (128 * 128) + row * 128 + ((c % 8) ^ (row % 8)) * 16) = v;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&sh.q_full[blk]);
+      };
+      load_q();
+      for (bool go = true; go;) {
+        const Unit cu = u;
+        const int ca = ta, cb = tb;
+        const int tk = r / a.group, tok = blk * tq + tk, head = cu.h * a.group + r - tk * a.group;
+        const bool live = tk < tq && tok < cu.n_tok;
+        const int hi = live ? cu.pos0 + tok : -1;       // last position the row sees
+        // of the block: the first token's position and the last's
+        const int pos_a = cu.pos0 + blk * tq, pos_b = min(pos_a + tq, cu.pos0 + cu.n_tok) - 1;
+        const bool any_live = __any_sync(0xffffffffu, live);
+        float m = kNegInf, l = 0.f;
+        int n_mine = 0;
+        for (int t = ca + (NQ == 1 ? st : 0); t < cb; t += NQ == 1 ? 2 : 1) {
+          wait(&sh.s_full[st], n_s);
+          tc_fence_after();
+          if (any_live) {
+            uint32_t sr[4][32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tc_ld32(t_s + 32 * i, sr[i]);
+            tc_wait_ld();
+            const int p0 = (cu.t0 + t) * S::kTile;
+            if (p0 + S::kTile - 1 > pos_a || (a.window > 0 && p0 <= pos_b - a.window)) {
+              const int lo = a.window > 0 ? hi - a.window + 1 : 0;
+#pragma unroll
+              for (int i = 0; i < 128; ++i) {
+                const int p = p0 + i;
+                if (p > hi || p < lo) sr[i / 32][i % 32] = 0xff800000u;
+              }
+            }
+            float top[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              top[i] = __uint_as_float(sr[i][0]);
+#pragma unroll
+              for (int j = 1; j < 32; ++j) top[i] = fmaxf(top[i], __uint_as_float(sr[i][j]));
+            }
+            const float row_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            if (n_mine == 0) {
+              m = row_top;
+            } else {
+              const bool grow = row_top > m && !((row_top - m) * a.scale_log2 <= kSlack);
+              if (__any_sync(0xffffffffu, grow)) {
+                const float base = grow ? row_top : m;
+                const float f = grow ? ex2((m - base) * a.scale_log2) : 1.f;
+                m = base;
+                l *= f;
+                wait(&sh.pv_done[st], n_s - 1);
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                  uint32_t ov[32];
+                  tc_ld32(t_o + 32 * c, ov);
+                  tc_wait_ld();
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * f);
+                  tc_st32(t_o + 32 * c, ov);
+                }
+                tc_wait_st();
+              }
+            }
+            const float mc = m == kNegInf ? 0.f : m * a.scale_log2;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t pr[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const int e = 64 * h + 2 * j;
+                const float p = ex2(fmaf(__uint_as_float(sr[e / 32][e % 32]), a.scale_log2, -mc));
+                const float q = ex2(fmaf(__uint_as_float(sr[e / 32][e % 32 + 1]), a.scale_log2, -mc));
+                sum[j & 1] += p;
+                sum[2 + (j & 1)] += q;
+                pr[j] = Elem<T>::pack(p, q);
+              }
+              tc_st32(t_s + 32 * h, pr);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc_wait_st();
+          }
+          tc_fence_before();
+          mbar_arrive(&sh.p_full[st]);
+          ++n_s;
+          ++n_mine;
+        }
+
+        // the next unit's Q as soon as nothing reads this one's: S of the last
+        // tile has been seen, so its product is done
+        go = more();
+        if (NQ == 1) bar_sync(2, 256);
+        if (go) {
+          next();
+          load_q();
+        }
+
+        // ---- the unit's end ------------------------------------------------------
+        if (n_mine > 0) {
+          wait(&sh.pv_done[st], n_s - 1);
+          tc_fence_after();
+        }
+        const bool whole = cu.start >= x0 && cu.start + cu.n_tile <= x1;
+        float* part = partial_at<HD>(a.work, NQ * 128, cta, cu.start >= x0 ? 1 : 0) ;
+        // stream 1 of a single block leaves its sums in global memory for stream 0
+        float* half_sum = NQ == 1 ? partial_at<HD>(a.work, 128, a.n_cta + cta, 0) : nullptr;
+        const bool two = NQ == 1 && cb - ca >= 2;
+        if (NQ == 1 && st == 1) {
+          if (two) {
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t ov[32];
+              tc_ld32(t_o + 32 * c, ov);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; j += 4)
+                *reinterpret_cast<uint4*>(half_sum + r * HD + 32 * c + j) =
+                    make_uint4(ov[j], ov[j + 1], ov[j + 2], ov[j + 3]);
+            }
+            half_sum[128 * HD + r] = m;
+            half_sum[128 * HD + 128 + r] = l;
+          }
+          tc_fence_before();
+          bar_sync(2, 256);
+          continue;
+        }
+        float f0 = 1.f, f1 = 0.f;
+        if (NQ == 1) {
+          bar_sync(2, 256);
+          if (two) {
+            const float m1 = half_sum[128 * HD + r], l1 = half_sum[128 * HD + 128 + r];
+            const float mm = fmaxf(m, m1), base = mm == kNegInf ? 0.f : mm;
+            f0 = ex2((m - base) * a.scale_log2);
+            f1 = ex2((m1 - base) * a.scale_log2);
+            l = l * f0 + l1 * f1;
+            m = mm;
+          }
+        }
+        const bool none = m == kNegInf && l == 0.f;
+        const float inv = whole ? (none ? 0.f : 1.f / l) : 1.f;
+        const float w0 = f0 * inv, w1 = f1 * inv;
+        char* dst = a.out + (cu.row0 + tok) * a.out_row + head * a.out_head;
+        const int prow = blk * 128 + r;
+        bool odd = false;
+        if (any_live) {
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t ov[32];
+            tc_ld32(t_o + 32 * c, ov);
+            tc_wait_ld();
+            float o[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(ov[j]) * w0;
+            if (two && live) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(half_sum + r * HD + 32 * c + j);
+                o[j] = fmaf(y.x, w1, o[j]), o[j + 1] = fmaf(y.y, w1, o[j + 1]);
+                o[j + 2] = fmaf(y.z, w1, o[j + 2]), o[j + 3] = fmaf(y.w, w1, o[j + 3]);
+              }
+            }
+            float zero = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) zero = fmaf(0.f, o[j], zero);   // NaN if any is NaN or infinite
+            odd |= zero != 0.f;
+            if (!live) continue;
+            if (whole) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 8)
+                *reinterpret_cast<uint4*>(dst + (32 * c + j) * 2) =
+                    make_uint4(Elem<T>::pack(o[j], o[j + 1]), Elem<T>::pack(o[j + 2], o[j + 3]),
+                               Elem<T>::pack(o[j + 4], o[j + 5]), Elem<T>::pack(o[j + 6], o[j + 7]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; j += 4)
+                *reinterpret_cast<float4*>(part + prow * HD + 32 * c + j) =
+                    make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            }
+          }
+        }
+        tc_fence_before();
+        if (live) {
+          if (!whole) {
+            part[NQ * 128 * HD + prow] = m;
+            part[NQ * 128 * HD + NQ * 128 + prow] = l;
+          } else if (a.lse) {
+            a.lse[(cu.row0 + tok) * a.lse_row + head] =
+                none ? kNegInf : (m * a.scale_log2 + log2f(l)) * 0.693147180559945309f;
+          }
+        }
+        // rows whose sums are not finite, by the formula
+        unsigned todo = __ballot_sync(0xffffffffu, odd && live);
+        while (todo) {
+          const int src = __ffs(todo) - 1;
+          todo &= todo - 1;
+          const int tok_s = __shfl_sync(0xffffffffu, tok, src), head_s = __shfl_sync(0xffffffffu, head, src);
+          const int row_s = __shfl_sync(0xffffffffu, prow, src);
+          const int last = cu.pos0 + tok_s;
+          const int p_lo = max((cu.t0 + ca) * S::kTile, a.window > 0 ? last - a.window + 1 : 0);
+          const int p_hi = min((cu.t0 + cb) * S::kTile - 1, last);
+          float ov[HD / 32], mm, ll;
+          row_by_formula<T, HD>(a, kv, cu, tok_s, head_s, p_lo, p_hi, ov, mm, ll);
+          T* d = reinterpret_cast<T*>(a.out + (cu.row0 + tok_s) * a.out_row + head_s * a.out_head);
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) {
+            if (whole) d[lane + 32 * i] = Elem<T>::down(p_hi < p_lo ? 0.f : ov[i] / ll);
+            else part[row_s * HD + lane + 32 * i] = ov[i];
+          }
+          if (lane == 0) {
+            if (!whole) {
+              part[NQ * 128 * HD + row_s] = mm;
+              part[NQ * 128 * HD + NQ * 128 + row_s] = ll;
+            } else if (a.lse) {
+              a.lse[(cu.row0 + tok_s) * a.lse_row + head_s] =
+                  (mm * a.scale_log2 + log2f(ll)) * 0.693147180559945309f;
+            }
+          }
+        }
+      }
+    }
+  }
+  // a wait that ran out has left products in flight: give them time, then free
+  __syncthreads();
+  if (*dead && tid == 0) {
+    mbar_wait(&sh.pv_done[0], 0), mbar_wait(&sh.pv_done[0], 1);
+    mbar_wait(&sh.pv_done[1], 0), mbar_wait(&sh.pv_done[1], 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tc_dealloc(tmem, S::kTmemCols);
+  }
+}
+
+// ---- host --------------------------------------------------------------------
+PFN_cuTensorMapEncodeTiled_v12000 cu_tensor_map_encoder();
+
+// K or V as rows of head_dim elements, read as boxes of box_rows rows x 64 columns.
+template <typename T>
+bool encode_pages(CUtensorMap* map, const char* p, const PagedKV& kv, int box_rows) {
+  const PFN_cuTensorMapEncodeTiled_v12000 enc = cu_tensor_map_encoder();
+  if (enc == nullptr) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(kv.head_dim),
+                        static_cast<cuuint64_t>(kv.n_pages) * kv.kv_heads * kv.page_size};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(kv.head_dim) * sizeof(T)};
+  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(map, std::is_same<T, half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+             const_cast<char*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows of a TMA box: the largest power of two that divides the page, at most a tile.
+inline int page_box_rows(const PagedKV& kv) { return std::min(kv.page_size & -kv.page_size, 128); }
+
+// What the tensor-core kernels take: pages of whole 8-row pieces (the swizzle's
+// period), head dimensions of 64 or 128, and a row index that fits a TMA coordinate.
+inline bool tc_paged_fits(const PagedKV& kv) {
+  return (kv.head_dim == 64 || kv.head_dim == 128) && kv.page_size % 8 == 0 &&
+         static_cast<long long>(kv.n_pages) * kv.kv_heads * kv.page_size < (1ll << 31) - 256;
+}
+
+template <typename T, int HD, int NQ>
+cudaError_t launch_tc(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st) {
+  using S = TcShape<HD, NQ>;
+  CUtensorMap km, vm;
+  const int box = page_box_rows(kv);
+  if (!encode_pages<T>(&km, kv.k, kv, box) || !encode_pages<T>(&vm, kv.v, kv, box)) return cudaErrorInvalidValue;
+  attn_paged_tc_kernel<T, HD, NQ><<<a.n_cta, kTcPagedThreads, S::kSmem, st>>>(km, vm, a, b, kv, box, err);
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess ? e : launch_join<T, HD, S::kTile, NQ * 128, 128>(a, b, kv, st);
+}
+
+template <typename T>
+cudaError_t launch_tc_t(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int nq, int* err, cudaStream_t st) {
+  if (kv.head_dim == 64)
+    return nq == 2 ? launch_tc<T, 64, 2>(a, b, kv, err, st) : launch_tc<T, 64, 1>(a, b, kv, err, st);
+  return nq == 2 ? launch_tc<T, 128, 2>(a, b, kv, err, st) : launch_tc<T, 128, 1>(a, b, kv, err, st);
+}
+
+template <typename T>
+cudaError_t tc_paged_attrs() {
+  auto set = [](auto* f, size_t n) {
+    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(n));
+  };
+  cudaError_t e = set(attn_paged_tc_kernel<T, 64, 1>, TcShape<64, 1>::kSmem);
+  if (e == cudaSuccess) e = set(attn_paged_tc_kernel<T, 64, 2>, TcShape<64, 2>::kSmem);
+  if (e == cudaSuccess) e = set(attn_paged_tc_kernel<T, 128, 1>, TcShape<128, 1>::kSmem);
+  if (e == cudaSuccess) e = set(attn_paged_tc_kernel<T, 128, 2>, TcShape<128, 2>::kSmem);
+  return e;
+}
+
+}  // namespace alm

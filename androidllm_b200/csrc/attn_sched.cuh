@@ -45,8 +45,6 @@ ALM_DEV void block_tiles(const Seq& q, int tpu, int window, int mb, int& t0, int
   if (last < 0) t0 = 0;
 }
 
-ALM_DEV bool seq_in(const Seq& q, int min_rows, int max_rows) { return q.n_new >= min_rows && q.n_new < max_rows; }
-
 // Tiles of one K/V head of sequence q, by one thread.
 template <int TILE>
 ALM_DEV long long seq_tiles(const Seq& q, int tpu, int window) {
@@ -65,8 +63,8 @@ constexpr int kManyBlocks = 8;
 // The line's length and the sequence that holds place goal(total): every one
 // of the first kSchedThreads threads calls it; sync() is their barrier.
 template <int TILE, typename Goal, typename Sync>
-ALM_DEV void sched_init(const SeqBatch& b, const PagedKV& kv, int tpu, int window, int min_rows, int max_rows,
-                        SchedShared& sh, Goal goal, Sync sync) {
+ALM_DEV void sched_init(const SeqBatch& b, const PagedKV& kv, int tpu, int window, SchedShared& sh, Goal goal,
+                        Sync sync) {
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
   // thread t sums sequences [t per, (t + 1) per); per is 1 up to 256 sequences
   const int per = (b.n_seq + kSchedThreads - 1) / kSchedThreads;
@@ -75,7 +73,7 @@ ALM_DEV void sched_init(const SeqBatch& b, const PagedKV& kv, int tpu, int windo
     q.n_new = 0;
     q.n_kv = 0;
     if (s < b.n_seq) q = load_seq(b, kv, s);
-    const bool in = q.n_new > 0 && seq_in(q, min_rows, max_rows);
+    const bool in = q.n_new > 0;
     const bool many = in && q.n_new > kManyBlocks * tpu;
     long long n = in && !many ? seq_tiles<TILE>(q, tpu, window) : 0;
     unsigned todo = __ballot_sync(0xffffffffu, many);
@@ -182,13 +180,13 @@ ALM_DEV Unit unit_at(const SeqBatch& b, const PagedKV& kv, int tpu, int window, 
 
 // The next unit on the line (there is one).
 template <int TILE>
-ALM_DEV void next_unit(const SeqBatch& b, const PagedKV& kv, int tpu, int window, int min_rows, int max_rows, Unit& u) {
+ALM_DEV void next_unit(const SeqBatch& b, const PagedKV& kv, int tpu, int window, Unit& u) {
   u.start += u.n_tile;
   if (++u.h < kv.kv_heads) return;
   u.h = 0;
   Seq q = load_seq(b, kv, u.s);
   ++u.mb;
-  while (u.mb * tpu >= q.n_new || !seq_in(q, min_rows, max_rows)) {
+  while (u.mb * tpu >= q.n_new) {
     u.mb = 0;
     ++u.s;
     if (u.s >= b.n_seq) return;   // behind the line's end: the caller does not use it

@@ -81,7 +81,6 @@ struct AttnPaged {
   float scale_log2;            // scale * log2(e)
   char* work;
   int n_cta;                   // CTAs that share the tiles
-  int min_rows, max_rows;      // this launch computes the sequences with min_rows <= rows < max_rows
 };
 
 struct Verify {
@@ -104,8 +103,6 @@ struct Verify {
 // dtype: ALM_F16 / ALM_BF16 / ALM_F32
 cudaError_t launch_rope_append(const RopeAppend& a, const SeqBatch& b, const PagedKV& kv, int dtype, int rope_dtype,
                                bool interleaved, int* err, cudaStream_t st);
-cudaError_t launch_attn_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int dtype, int* err,
-                              cudaStream_t st);
 cudaError_t launch_verify(const Verify& a, int dtype, cudaStream_t st);
 size_t attn_paged_work_bytes(int n_sms, int head_dim);
 cudaError_t paged_init_attrs();

@@ -18,18 +18,31 @@ cudaError_t launch_attn_paged_f16(const AttnPaged& a, const SeqBatch& b, const P
 cudaError_t launch_attn_paged_bf16(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st);
 cudaError_t attn_paged_attrs_f16();
 cudaError_t attn_paged_attrs_bf16();
+bool attn_paged_tc_fits(const PagedKV& kv);
+cudaError_t launch_attn_paged_tc_f16(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int nq, int* err,
+                                     cudaStream_t st);
+cudaError_t launch_attn_paged_tc_bf16(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int nq, int* err,
+                                      cudaStream_t st);
+cudaError_t attn_paged_tc_attrs_f16();
+cudaError_t attn_paged_tc_attrs_bf16();
 cudaError_t verify_init_attrs();
 
 cudaError_t paged_init_attrs() {
   cudaError_t e = attn_paged_attrs_f16();
   if (e == cudaSuccess) e = attn_paged_attrs_bf16();
+  if (e == cudaSuccess) e = attn_paged_tc_attrs_f16();
+  if (e == cudaSuccess) e = attn_paged_tc_attrs_bf16();
   if (e == cudaSuccess) e = verify_init_attrs();
   return e;
 }
 
+// Sequences of more rows than this (tokens times the heads that share a K/V
+// head) take the tcgen05 kernel.
+constexpr long long kTcMinRows = 32;
+
 // Two partial results a CTA, of the largest row block.
 size_t attn_paged_work_bytes(int n_sms, int head_dim) {
-  return static_cast<size_t>(n_sms) * 2 * 128 * (head_dim + 2) * sizeof(float);
+  return static_cast<size_t>(n_sms) * 2 * 256 * (head_dim + 2) * sizeof(float);
 }
 }  // namespace alm
 
@@ -207,11 +220,16 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   a.scale_log2 = v->scale * 1.4426950408889634f;
   a.work = static_cast<char*>(v->work_dev);
   a.n_cta = n_sms;
-  a.min_rows = 1;
-  a.max_rows = 0x7fffffff;
   OnDevice on(device);
-  return cuda_status(kv_->dtype == ALM_BF16 ? launch_attn_paged_bf16(a, b, kv, err, st)
-                                            : launch_attn_paged_f16(a, b, kv, err, st),
+  const long long rows = static_cast<long long>(b.max_rows) * a.group;
+  const bool bf = kv_->dtype == ALM_BF16;
+  if (rows > kTcMinRows && attn_paged_tc_fits(kv)) {
+    const int nq = rows > 128 ? 2 : 1;
+    return cuda_status(bf ? launch_attn_paged_tc_bf16(a, b, kv, nq, err, st)
+                          : launch_attn_paged_tc_f16(a, b, kv, nq, err, st),
+                       "attn_paged");
+  }
+  return cuda_status(bf ? launch_attn_paged_bf16(a, b, kv, err, st) : launch_attn_paged_f16(a, b, kv, err, st),
                      "attn_paged");
 }
 

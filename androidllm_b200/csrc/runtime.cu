@@ -1526,8 +1526,9 @@ int alm_ctx_sync(alm_ctx* ctx) {
   ALM_REQ(ctx, "null ctx");
   DeviceGuard g(ctx->device);
   ALM_CUDA(cudaStreamSynchronize(ctx->stream));
-  if (*const_cast<volatile int*>(ctx->range_err) != 0) {
+  if (const int e = *const_cast<volatile int*>(ctx->range_err); e != 0) {
     *ctx->range_err = 0;
+    if (e == 2) return fail(ALM_ERR_CUDA, "a wait inside the attention kernel ran out");
     return fail(ALM_ERR_RANGE, "a page, slot or position outside its range reached the device");
   }
   return ALM_OK;

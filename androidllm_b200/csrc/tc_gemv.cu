@@ -1147,6 +1147,9 @@ cudaError_t tc_set_attrs() {
 
 }  // namespace
 
+// the same for other translation units
+PFN_cuTensorMapEncodeTiled_v12000 cu_tensor_map_encoder() { return tensor_map_encoder(); }
+
 cudaError_t tc_gemv_init_attrs() {
   cudaError_t e = tc_set_attrs<4>();
   if (e == cudaSuccess) e = tc_set_attrs<8>();
