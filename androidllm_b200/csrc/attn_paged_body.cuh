@@ -109,10 +109,10 @@ ALM_DEV float* partial_at(char* work, int rows, int cta, int which) {
 // row does not see: for rows whose sums are not finite, since a hidden
 // position's infinity or NaN times a zero weight spoils a matrix product.
 template <typename T, int HD>
-__device__ __noinline__ void row_by_formula(const AttnPaged& a, const PagedKV& kv, const Unit& u, int tok, int head,
-                                            int p_lo, int p_hi, float (&o)[HD / 32], float& m, float& l) {
+__device__ __noinline__ void row_by_formula(const AttnPaged& a, const PagedKV& kv, const int* pages, int kv_head, int row,
+                                            int head, int p_lo, int p_hi, float (&o)[HD / 32], float& m, float& l) {
   const int lane = threadIdx.x % kWarp;
-  const T* q = reinterpret_cast<const T*>(a.q + (u.row0 + tok) * a.q_row + head * a.q_head);
+  const T* q = reinterpret_cast<const T*>(a.q + row * a.q_row + head * a.q_head);
   float qv[HD / 32];
 #pragma unroll
   for (int i = 0; i < HD / 32; ++i) {
@@ -124,9 +124,9 @@ __device__ __noinline__ void row_by_formula(const AttnPaged& a, const PagedKV& k
   for (int pass = 0; pass < 2; ++pass) {
     for (int p = p_lo; p <= p_hi; ++p) {
       const int pi = page_of(kv, p);
-      const int page = u.pages ? __ldg(u.pages + pi) : -1;
+      const int page = pages ? __ldg(pages + pi) : -1;
       const bool ok = page >= 0 && page < kv.n_pages;
-      const size_t off = ok ? kv_offset(kv, page, u.h, p - pi * kv.page_size) : 0;
+      const size_t off = ok ? kv_offset(kv, page, kv_head, p - pi * kv.page_size) : 0;
       const T* k = reinterpret_cast<const T*>(kv.k) + off;
       float s = 0.f;
 #pragma unroll
@@ -147,7 +147,8 @@ __device__ __noinline__ void row_by_formula(const AttnPaged& a, const PagedKV& k
 
 template <typename T, int HD, int WM>
 __global__ void __launch_bounds__(kPagedThreads, 1)
-attn_paged_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv, int* err) {
+attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ SeqBatch b,
+                  const __grid_constant__ PagedKV kv, int* err) {
   using S = PagedShape<HD, WM>;
   constexpr int kTile = S::kTile, kWK = S::kWK, kNP = S::kNP, kChunk = S::kChunk, kRows = S::kRows;
   extern __shared__ __align__(128) char smem[];
@@ -425,7 +426,7 @@ attn_paged_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv, int* er
         const int p_lo = max((u.t0 + t_first) * kTile, a.window > 0 ? last - a.window + 1 : 0);
         const int p_hi = min((u.t0 + t + 1) * kTile - 1, last);
         float ov[HD / 32], mm, ll;
-        row_by_formula<T, HD>(a, kv, u, tok, head, p_lo, p_hi, ov, mm, ll);
+        row_by_formula<T, HD>(a, kv, u.pages, u.h, u.row0 + tok, head, p_lo, p_hi, ov, mm, ll);
         T* dst = reinterpret_cast<T*>(a.out + (u.row0 + tok) * a.out_row + head * a.out_head);
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
@@ -457,7 +458,8 @@ attn_paged_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv, int* er
 // ROWS rows are blocks of BLK rows, whole tokens each.
 template <typename T, int HD, int TILE, int ROWS, int BLK>
 __global__ void __launch_bounds__(kPagedThreads)
-attn_paged_join_kernel(const AttnPaged a, const SeqBatch b, const PagedKV kv) {
+attn_paged_join_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ SeqBatch b,
+                       const __grid_constant__ PagedKV kv) {
   __shared__ SchedShared sched;
   const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
   const int tq = BLK / a.group, tpu = ROWS / BLK * tq, cta = blockIdx.x;

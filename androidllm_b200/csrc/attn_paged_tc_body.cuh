@@ -14,7 +14,7 @@
 // tiles of one block, joined at the unit's end.
 //
 // Warps 0-3 and 4-7: softmax of stream 0 and 1, one row a thread.  Warp 8:
-// issues the products.  Warp 9: loads K and V tiles with TMA, one box per page
+// issues the products.  Warp 9 (10 and 11 idle): loads K and V tiles with TMA, one box per page
 // piece and 64 columns, into a ring of tiles in the order they are used.
 //
 // The reference maximum m follows the row's maximum only when that has grown
@@ -34,7 +34,12 @@
 
 namespace alm {
 
-constexpr int kTcPagedThreads = 320;
+// 12 warps launch with 168 registers a thread; the softmax warps (one row of S
+// a thread) then take kSoftRegs and the others keep kRestRegs:
+// 256 * 216 + 128 * 72 = 384 * 168.
+constexpr int kTcPagedThreads = 384;
+constexpr int kSoftRegs = 216, kRestRegs = 72;
+static_assert(256 * kSoftRegs + 128 * kRestRegs == kTcPagedThreads * 168, "the shares add up to the launch's registers");
 constexpr float kSlack = 8.f;
 
 template <int HD, int NQ>
@@ -95,7 +100,8 @@ constexpr uint32_t tc_idesc(int n, bool bmn) {
 template <typename T, int HD, int NQ>
 __global__ void __launch_bounds__(kTcPagedThreads, 1)
 attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                     const AttnPaged a, const SeqBatch b, const PagedKV kv, int box_rows, int* err) {
+                     const __grid_constant__ AttnPaged a, const __grid_constant__ SeqBatch b,
+                     const __grid_constant__ PagedKV kv, int box_rows, int* err) {
   using S = TcShape<HD, NQ>;
   extern __shared__ char smem_raw[];
   __shared__ TcShared sh;
@@ -151,18 +157,35 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     __syncwarp();
   };
 
-  if (x0 < x1) {
-    Unit u = unit_at<S::kTile>(b, kv, tpu, a.window, sh.sched.found_seq, sh.sched.found_at, x0);
-    // this CTA's tiles [ta, tb) of the unit
-    int ta = static_cast<int>(x0 - u.start);
-    int tb = static_cast<int>(min(x1 - u.start, static_cast<long long>(u.n_tile)));
-    auto next = [&] {
-      next_unit<S::kTile>(b, kv, tpu, a.window, u);
+  // Each role walks this CTA's part of the line by itself.
+  struct Walk {
+    Unit u;
+    int ta, tb;   // this CTA's tiles of the unit
+    long long x1;
+    ALM_DEV void start(const SeqBatch& b, const PagedKV& kv, int tpu, int window, const SchedShared& sc, long long x0,
+                       long long x1_) {
+      x1 = x1_;
+      u = unit_at<S::kTile>(b, kv, tpu, window, sc.found_seq, sc.found_at, x0);
+      ta = static_cast<int>(x0 - u.start);
+      tb = static_cast<int>(min(x1 - u.start, static_cast<long long>(u.n_tile)));
+    }
+    ALM_DEV void next(const SeqBatch& b, const PagedKV& kv, int tpu, int window) {
+      next_unit<S::kTile>(b, kv, tpu, window, u);
       ta = 0;
       tb = static_cast<int>(min(x1 - u.start, static_cast<long long>(u.n_tile)));
-    };
-    auto more = [&] { return u.start + u.n_tile < x1; };
+    }
+    ALM_DEV bool more() const { return u.start + u.n_tile < x1; }
+  };
 
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
+    if (x0 < x1 && warp <= 9) {
+    Walk w;
+    w.start(b, kv, tpu, a.window, sh.sched, x0, x1);
+    Unit& u = w.u;
+    int &ta = w.ta, &tb = w.tb;
+    auto next = [&] { w.next(b, kv, tpu, a.window); };
+    auto more = [&] { return w.more(); };
     if (warp == 9) {
       // ---- loads ---------------------------------------------------------------
       int at = 0;
@@ -224,7 +247,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           mbar_wait(&sh.full[i], 1);
         }
       }
-    } else if (warp == 8) {
+    } else {
       // ---- products ------------------------------------------------------------
       const uint32_t id_s = tc_idesc<T>(128, false), id_o = tc_idesc<T>(HD, true);
       int at = 0;
@@ -360,7 +383,17 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           if (go) next();
         }
       }
-    } else {
+    }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    if (x0 < x1) {
+      Walk w;
+      w.start(b, kv, tpu, a.window, sh.sched, x0, x1);
+      Unit& u = w.u;
+      int &ta = w.ta, &tb = w.tb;
+      auto next = [&] { w.next(b, kv, tpu, a.window); };
+      auto more = [&] { return w.more(); };
       // ---- softmax -------------------------------------------------------------
       const int st = warp / 4;                         // stream
       const int r = tid % 128;                         // row of the block = lane of tensor memory
@@ -586,7 +619,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           const int p_lo = max((cu.t0 + ca) * S::kTile, a.window > 0 ? last - a.window + 1 : 0);
           const int p_hi = min((cu.t0 + cb) * S::kTile - 1, last);
           float ov[HD / 32], mm, ll;
-          row_by_formula<T, HD>(a, kv, cu, tok_s, head_s, p_lo, p_hi, ov, mm, ll);
+          row_by_formula<T, HD>(a, kv, cu.pages, cu.h, cu.row0 + tok_s, head_s, p_lo, p_hi, ov, mm, ll);
           T* d = reinterpret_cast<T*>(a.out + (cu.row0 + tok_s) * a.out_row + head_s * a.out_head);
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) {
