@@ -175,16 +175,17 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
   const long long x0 = share(total, cta, n_cta), x1 = share(total, cta + 1, n_cta);
 
   Unit u = unit_at<kTile>(b, kv, tpu, a.window, sched.found_seq, sched.found_at, x0);
+  int t = u.from(x0), tb = u.upto(x1);   // this CTA's tiles of the unit: [t, tb)
+  if (t >= tb) return;                   // only places without a tile
   // the loader's walk, kStages - 1 tiles ahead of the computation's
   Unit lu = u;
-  int lt = static_cast<int>(x0 - u.start);
-  long long lx = x0;
+  int lt = t, ltb = tb;
   const uint32_t smem0 = smem_addr(smem);
   constexpr int kUnits16 = HD / 8;   // 16-byte units of a K or V row
   bool bad_page = false;
 
   auto load_tile = [&](int stage) {
-    if (lx < x1) {
+    if (lt < ltb) {
       const uint32_t dst = smem0 + stage * S::kStageBytes;
       const int base = (lu.t0 + lt) * kTile;
       constexpr int kIter = kTile * kUnits16 / kPagedThreads;
@@ -207,10 +208,10 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
         cp_async16(dst + r * S::kPitch + c * 16, kv.k + off, ok ? 16 : 0);
         cp_async16(dst + (kTile + r) * S::kPitch + c * 16, kv.v + off, ok ? 16 : 0);
       }
-      ++lx;
-      if (++lt == lu.n_tile && lx < x1) {
+      if (++lt == ltb && lu.more(x1)) {
         next_unit<kTile>(b, kv, tpu, a.window, lu);
         lt = 0;
+        ltb = lu.upto(x1);
       }
     }
     cp_async_commit();
@@ -218,7 +219,6 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) load_tile(i);
 
-  int t = static_cast<int>(x0 - u.start);
   int t_first = t;   // first tile of the unit computed here
   uint32_t qf[HD / 16][4];
   float o[HD / 8][4];
@@ -248,7 +248,7 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
   begin_unit();
 
   int stage = 0;
-  for (long long x = x0; x < x1; ++x) {
+  for (;;) {
     cp_async_wait<S::kStages - 2>();
     __syncthreads();
     load_tile(stage == 0 ? S::kStages - 1 : stage - 1);
@@ -328,13 +328,13 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
         }
       }
     }
-    if (t + 1 < u.n_tile && x + 1 < x1) {
+    if (t + 1 < tb) {
       ++t;
       if (++stage == S::kStages) stage = 0;
       continue;
     }
 
-    // the unit's end, or the share's: merge the WK slices through this stage
+    // the unit's end here: merge the WK slices through this stage
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
@@ -369,8 +369,8 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
       }
     }
     float* buf = reinterpret_cast<float*>(smem + stage * S::kStageBytes);
-    const bool whole = u.start >= x0 && u.start + u.n_tile <= x1;
-    float* part = partial_at<HD>(a.work, kRows, cta, u.start >= x0 ? 1 : 0);
+    const bool whole = t_first == 0 && tb == u.n_tile;
+    float* part = partial_at<HD>(a.work, kRows, cta, t_first == 0 ? 1 : 0);
     constexpr int kCols = HD / S::kPasses;
     bool any_bad = false;
 #pragma unroll
@@ -443,13 +443,14 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
         }
       }
     }
-    if (x + 1 < x1) {
-      next_unit<kTile>(b, kv, tpu, a.window, u);
-      t = t_first = 0;
-      begin_unit();
-    }
+    if (!u.more(x1)) break;
+    next_unit<kTile>(b, kv, tpu, a.window, u);
+    t = t_first = 0;
+    tb = u.upto(x1);
+    begin_unit();
     if (++stage == S::kStages) stage = 0;
   }
+  cp_async_wait<0>();
   if (bad_page) *err = 1;
 }
 
@@ -480,7 +481,7 @@ attn_paged_join_kernel(const __grid_constant__ AttnPaged a, const __grid_constan
   bool mine = cta < n_cta && x1 < total;
   if (mine) {
     u = unit_at<TILE>(b, kv, tpu, a.window, sched.found_seq, sched.found_at, x1 - 1);
-    mine = u.start >= x0 && u.start + u.n_tile > x1;
+    mine = u.start >= x0 && u.start < x1 && u.start + u.n_tile > x1;
   }
   grid_dep_wait();
   if (!mine) return;

@@ -14,8 +14,9 @@
 // tiles of one block, joined at the unit's end.
 //
 // Warps 0-3 and 4-7: softmax of stream 0 and 1, one row a thread.  Warp 8:
-// issues the products.  Warp 9 (10 and 11 idle): loads K and V tiles with TMA, one box per page
-// piece and 64 columns, into a ring of tiles in the order they are used.
+// issues the products.  Warp 9: loads K and V tiles with TMA, one box per page
+// piece and 64 columns, into a ring of tiles in the order they are used.  Warp
+// 10: loads Q.  Warp 11 is idle.
 //
 // The reference maximum m follows the row's maximum only when that has grown
 // by more than kSlack (in powers of two): weights stay below 2^kSlack, and the
@@ -36,9 +37,9 @@ namespace alm {
 
 // 12 warps launch with 168 registers a thread; the softmax warps (one row of S
 // a thread) then take kSoftRegs and the others keep kRestRegs:
-// 256 * 216 + 128 * 72 = 384 * 168.
+// 256 * 208 + 128 * 88 = 384 * 168.
 constexpr int kTcPagedThreads = 384;
-constexpr int kSoftRegs = 216, kRestRegs = 72;
+constexpr int kSoftRegs = 208, kRestRegs = 88;
 static_assert(256 * kSoftRegs + 128 * kRestRegs == kTcPagedThreads * 168, "the shares add up to the launch's registers");
 constexpr float kSlack = 8.f;
 
@@ -55,7 +56,7 @@ struct TcShape {
 struct TcShared {
   SchedShared sched;
   uint64_t full[10], empty[10];
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], pv_done[2];
   uint32_t tmem;
   int dead;      // a wait ran out: everybody leaves
 };
@@ -87,6 +88,35 @@ ALM_DEV void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t
       "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
       : "memory");
 }
+ALM_DEV void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+// Pairs of fp32 in one 64-bit register: one instruction for both.
+ALM_DEV uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+ALM_DEV void unpair(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r)); }
+ALM_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+ALM_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+ALM_DEV float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 ALM_DEV void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 // Instruction descriptor: fp32 accumulator, A and B of type T, N wide; bmn: B
@@ -100,6 +130,7 @@ constexpr uint32_t tc_idesc(int n, bool bmn) {
 template <typename T, int HD, int NQ>
 __global__ void __launch_bounds__(kTcPagedThreads, 1)
 attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                     const __grid_constant__ CUtensorMap q_map,
                      const __grid_constant__ AttnPaged a, const __grid_constant__ SeqBatch b,
                      const __grid_constant__ PagedKV kv, int box_rows, int* err) {
   using S = TcShape<HD, NQ>;
@@ -118,9 +149,10 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     if (lane == 0) {
       for (int i = 0; i < S::kSlots; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&sh.q_full[i], NQ == 2 ? 128 : 256);
+        mbar_init(&sh.q_full[i], 1);
+        mbar_init(&sh.q_empty[i], 1);
         mbar_init(&sh.s_full[i], 1);
-        mbar_init(&sh.p_full[i], 128);
+        mbar_init(&sh.p_full[i][0], 128), mbar_init(&sh.p_full[i][1], 128);
         mbar_init(&sh.pv_done[i], 1);
       }
       sh.dead = 0;
@@ -162,26 +194,27 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     Unit u;
     int ta, tb;   // this CTA's tiles of the unit
     long long x1;
-    ALM_DEV void start(const SeqBatch& b, const PagedKV& kv, int tpu, int window, const SchedShared& sc, long long x0,
+    // false: the share has only places without a tile
+    ALM_DEV bool start(const SeqBatch& b, const PagedKV& kv, int tpu, int window, const SchedShared& sc, long long x0,
                        long long x1_) {
       x1 = x1_;
       u = unit_at<S::kTile>(b, kv, tpu, window, sc.found_seq, sc.found_at, x0);
-      ta = static_cast<int>(x0 - u.start);
-      tb = static_cast<int>(min(x1 - u.start, static_cast<long long>(u.n_tile)));
+      ta = u.from(x0);
+      tb = u.upto(x1);
+      return ta < tb;
     }
     ALM_DEV void next(const SeqBatch& b, const PagedKV& kv, int tpu, int window) {
       next_unit<S::kTile>(b, kv, tpu, window, u);
       ta = 0;
-      tb = static_cast<int>(min(x1 - u.start, static_cast<long long>(u.n_tile)));
+      tb = u.upto(x1);
     }
-    ALM_DEV bool more() const { return u.start + u.n_tile < x1; }
+    ALM_DEV bool more() const { return u.more(x1); }
   };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
-    if (x0 < x1 && warp <= 9) {
     Walk w;
-    w.start(b, kv, tpu, a.window, sh.sched, x0, x1);
+    if (x0 < x1 && warp <= 10 && w.start(b, kv, tpu, a.window, sh.sched, x0, x1)) {
     Unit& u = w.u;
     int &ta = w.ta, &tb = w.tb;
     auto next = [&] { w.next(b, kv, tpu, a.window); };
@@ -247,6 +280,30 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           mbar_wait(&sh.full[i], 1);
         }
       }
+    } else if (warp == 10) {
+      // ---- Q: the tokens' heads of one K/V head are a box (columns, heads,
+      // tokens), which is the packed order of the block's rows; tokens of the
+      // next sequence that it may hold fill rows that nothing is written from
+      uint32_t n = 0;
+      const uint32_t bytes = static_cast<uint32_t>(tq * a.group) * 128 * S::kChunks;
+      for (bool go = true; go && !gone(); ++n) {
+        for (int i = 0; i < NQ; ++i) {
+          wait(&sh.q_empty[i], n ^ 1);
+          if (gone()) break;
+          if (lane == 0) {
+            mbar_expect_tx(&sh.q_full[i], bytes);
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+              tma_3d(smem0 + i * S::kTileBytes + c * (128 * 128), &q_map, c * 64, u.h * a.group, u.row0 + i * tq,
+                     &sh.q_full[i]);
+          }
+          __syncwarp();
+        }
+        go = more();
+        if (go) next();
+      }
+      if (gone())
+        for (int i = 0; i < NQ; ++i) mbar_wait(&sh.q_full[i], 0), mbar_wait(&sh.q_full[i], 1);
     } else {
       // ---- products ------------------------------------------------------------
       const uint32_t id_s = tc_idesc<T>(128, false), id_o = tc_idesc<T>(HD, true);
@@ -270,16 +327,29 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         }
         __syncwarp();
       };
-      // O of stream i += P . V tile in the current slot
+      // O of stream i += P . V tile in the current slot, in two halves of 64
+      // positions: the first product runs while the second half's weights are made
       auto pv = [&](int i, bool acc) {
-        if (lane == 0) {
-          const uint32_t va = ring0 + at * S::kTileBytes;
 #pragma unroll
-          for (int k = 0; k < 8; ++k)   // 16 positions: two groups of 8 rows of 128 bytes
-            tc_mma_ts(tmem + S::kColO + i * HD, tmem + S::kColS + i * 128 + 8 * k,
-                      sdesc128(va + k * 2048, 128 * 128, 1024), id_o, acc || k > 0);
-          tc_commit(&sh.pv_done[i]);
+        for (int h = 0; h < 2; ++h) {
+          wait(&sh.p_full[i][h], n_p[i]);
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t va = ring0 + at * S::kTileBytes;
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; ++k)   // 16 positions: two groups of 8 rows of 128 bytes
+              tc_mma_ts(tmem + S::kColO + i * HD, tmem + S::kColS + i * 128 + 8 * k,
+                        sdesc128(va + k * 2048, 128 * 128, 1024), id_o, acc || k > 0);
+          }
+          __syncwarp();
         }
+        ++n_p[i];
+        if (lane == 0) tc_commit(&sh.pv_done[i]);
+        __syncwarp();
+      };
+      // nothing reads Q block i any more
+      auto q_done = [&](int i) {
+        if (lane == 0) tc_commit(&sh.q_empty[i]);
         __syncwarp();
       };
       auto release = [&] {
@@ -310,10 +380,6 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         wait(&sh.full[at], round);
         tc_fence_after();
       };
-      auto p_ready = [&](int i) {
-        wait(&sh.p_full[i], n_p[i]++);
-        tc_fence_after();
-      };
       auto q_ready = [&](int i) {
         wait(&sh.q_full[i], n_q[i]++);
         tc_fence_after();
@@ -322,39 +388,39 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         q_ready(0);
         k_ready();
         qk(0);
+        if (ta + 1 == tb) q_done(0);
         q_ready(1);
         qk(1);
+        if (ta + 1 == tb) q_done(1);
         release();
-        for (bool go = true; go && !gone();) {
-          const bool last_unit = !more();
-          for (int t = ta; t < tb && !gone(); ++t) {
-            const int v_at = at;
-            const uint32_t v_round = round;
-            const bool another = t + 1 < tb || !last_unit;
-            p_ready(0);
-            v_ready(t);
-            pv(0, t > ta);
-            step_ring();
-            if (another) {
-              if (t + 1 == tb) q_ready(0);
-              k_ready();
-              qk(0);
-            }
-            const int k_at = at;
-            const uint32_t k_round = round;
-            p_ready(1);
-            at = v_at, round = v_round;
-            pv(1, t > ta);
-            release();
-            at = k_at, round = k_round;
-            if (another) {
-              if (t + 1 == tb) q_ready(1);
-              qk(1);
-              release();
-            }
+        bool first = true;   // tile t is the unit's first here
+        for (int t = ta; !gone();) {
+          const int v_at = at;
+          const uint32_t v_round = round;
+          const bool cross = t + 1 == tb, another = !cross || more();
+          v_ready(t);
+          pv(0, !first);
+          step_ring();
+          if (cross && another) next();
+          t = cross ? ta : t + 1;
+          if (another) {
+            if (cross) q_ready(0);
+            k_ready();
+            qk(0);
+            if (t + 1 == tb) q_done(0);
           }
-          go = !last_unit;
-          if (go) next();
+          const int k_at = at;
+          const uint32_t k_round = round;
+          at = v_at, round = v_round;
+          pv(1, !first);
+          release();
+          at = k_at, round = k_round;
+          if (!another) break;
+          if (cross) q_ready(1);
+          qk(1);
+          if (t + 1 == tb) q_done(1);
+          release();
+          first = cross;
         }
       } else {
         for (bool go = true; go && !gone();) {
@@ -367,9 +433,9 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
             qk(1);
             release();
           }
+          if (tb - ta <= 2) q_done(0);
           for (int t = ta; t < tb && !gone(); ++t) {
             const int i = (t - ta) & 1;
-            p_ready(i);
             v_ready(t);
             pv(i, t - ta >= 2);
             release();
@@ -377,6 +443,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
               k_ready();
               qk(i);
               release();
+              if (t + 3 == tb) q_done(0);
             }
           }
           go = more();
@@ -387,9 +454,8 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-    if (x0 < x1) {
-      Walk w;
-      w.start(b, kv, tpu, a.window, sh.sched, x0, x1);
+    Walk w;
+    if (x0 < x1 && w.start(b, kv, tpu, a.window, sh.sched, x0, x1)) {
       Unit& u = w.u;
       int &ta = w.ta, &tb = w.tb;
       auto next = [&] { w.next(b, kv, tpu, a.window); };
@@ -402,26 +468,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       const int blk = NQ == 2 ? st : 0;                // 128-row block of the unit
       uint32_t n_s = 0;                                // tiles of this stream so far
 
-      // Q block `blk` into shared memory, 16 bytes a thread and step, in the
-      // swizzled layout TMA gives K (row r at 128 r, its 16-byte column c at c ^ (r mod 8))
-      auto load_q = [&] {
-        constexpr int kUnits = HD / 8;
-        char* q_s = smem + blk * S::kTileBytes;
-        constexpr int kStep = NQ == 2 ? 128 : 256;
-        const int t0 = NQ == 2 ? r : tid;
-#pragma unroll 4
-        for (int i = t0; i < 128 * kUnits; i += kStep) {
-          const int row = i / kUnits, c = i % kUnits;
-          const int tk = row / a.group, tok = blk * tq + tk, head = u.h * a.group + row - tk * a.group;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (tk < tq && tok < u.n_tok)
-            v = __ldg(reinterpret_cast<const uint4*>(a.q + (u.row0 + tok) * a.q_row + head * a.q_head) + c);
-          *reinterpret_cast<uint4*>(q_s + (c / 8) * (128 * 128) + row * 128 + ((c % 8) ^ (row % 8)) * 16) = v;
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(&sh.q_full[blk]);
-      };
-      load_q();
+      uint32_t n_u = 0;                                // units so far
       for (bool go = true; go;) {
         const Unit cu = u;
         const int ca = ta, cb = tb;
@@ -453,11 +500,13 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
             float top[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              top[i] = __uint_as_float(sr[i][0]);
+              top[i] = fmax3(__uint_as_float(sr[i][0]), __uint_as_float(sr[i][1]), __uint_as_float(sr[i][2]));
 #pragma unroll
-              for (int j = 1; j < 32; ++j) top[i] = fmaxf(top[i], __uint_as_float(sr[i][j]));
+              for (int j = 3; j < 31; j += 2)
+                top[i] = fmax3(top[i], __uint_as_float(sr[i][j]), __uint_as_float(sr[i][j + 1]));
+              top[i] = fmaxf(top[i], __uint_as_float(sr[i][31]));
             }
-            const float row_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const float row_top = fmaxf(fmax3(top[0], top[1], top[2]), top[3]);
             if (n_mine == 0) {
               m = row_top;
             } else {
@@ -482,48 +531,52 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
               }
             }
             const float mc = m == kNegInf ? 0.f : m * a.scale_log2;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t c2 = pair(a.scale_log2, a.scale_log2), m2 = pair(-mc, -mc);
+            uint64_t sum[2] = {0, 0};   // (+0, +0)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               uint32_t pr[32];
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 const int e = 64 * h + 2 * j;
-                const float p = ex2(fmaf(__uint_as_float(sr[e / 32][e % 32]), a.scale_log2, -mc));
-                const float q = ex2(fmaf(__uint_as_float(sr[e / 32][e % 32 + 1]), a.scale_log2, -mc));
-                sum[j & 1] += p;
-                sum[2 + (j & 1)] += q;
+                float p, q;
+                unpair(fma2(pair(__uint_as_float(sr[e / 32][e % 32]), __uint_as_float(sr[e / 32][e % 32 + 1])), c2, m2),
+                       p, q);
+                p = ex2(p);
+                q = ex2(q);
+                sum[j & 1] = add2(sum[j & 1], pair(p, q));
                 pr[j] = Elem<T>::pack(p, q);
               }
               tc_st32(t_s + 32 * h, pr);
+              tc_wait_st();
+              tc_fence_before();
+              mbar_arrive(&sh.p_full[st][h]);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tc_wait_st();
+            float s0, s1, s2, s3;
+            unpair(sum[0], s0, s1);
+            unpair(sum[1], s2, s3);
+            l += (s0 + s1) + (s2 + s3);
+          } else {
+            mbar_arrive(&sh.p_full[st][0]);
+            mbar_arrive(&sh.p_full[st][1]);
           }
-          tc_fence_before();
-          mbar_arrive(&sh.p_full[st]);
           ++n_s;
           ++n_mine;
         }
 
-        // the next unit's Q as soon as nothing reads this one's: S of the last
-        // tile has been seen, so its product is done
         go = more();
-        if (NQ == 1) bar_sync(2, 256);
-        if (go) {
-          next();
-          load_q();
-        }
+        if (go) next();
 
         // ---- the unit's end ------------------------------------------------------
         if (n_mine > 0) {
           wait(&sh.pv_done[st], n_s - 1);
           tc_fence_after();
         }
-        const bool whole = cu.start >= x0 && cu.start + cu.n_tile <= x1;
-        float* part = partial_at<HD>(a.work, NQ * 128, cta, cu.start >= x0 ? 1 : 0) ;
-        // stream 1 of a single block leaves its sums in global memory for stream 0
-        float* half_sum = NQ == 1 ? partial_at<HD>(a.work, 128, a.n_cta + cta, 0) : nullptr;
+        const bool whole = ca == 0 && cb == cu.n_tile;
+        float* part = partial_at<HD>(a.work, NQ * 128, cta, ca == 0 ? 1 : 0);
+        // stream 1 of a single block leaves its sums in global memory for
+        // stream 0, in two places in turn: one is read while the next is written
+        float* half_sum = NQ == 1 ? partial_at<HD>(a.work, 128, a.n_cta + cta, n_u++ & 1) : nullptr;
         const bool two = NQ == 1 && cb - ca >= 2;
         if (NQ == 1 && st == 1) {
           if (two) {
@@ -677,18 +730,42 @@ inline int page_box_rows(const PagedKV& kv) { return std::min(kv.page_size & -kv
 
 // What the tensor-core kernels take: pages of whole 8-row pieces (the swizzle's
 // period), head dimensions of 64 or 128, and a row index that fits a TMA coordinate.
-inline bool tc_paged_fits(const PagedKV& kv) {
-  return (kv.head_dim == 64 || kv.head_dim == 128) && kv.page_size % 8 == 0 &&
+// Q strides are positive and below 2^40 bytes, as a tensor map's have to be.
+inline bool tc_paged_fits(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv) {
+  auto stride = [](int64_t bytes, int n) { return n <= 1 || (bytes > 0 && bytes < (1ll << 40)); };
+  return (kv.head_dim == 64 || kv.head_dim == 128) && kv.page_size % 8 == 0 && stride(a.q_head, a.heads) &&
+         stride(a.q_row, b.n_rows) &&
          static_cast<long long>(kv.n_pages) * kv.kv_heads * kv.page_size < (1ll << 31) - 256;
+}
+
+// Q as (columns, heads, rows): boxes of 64 columns x the heads of one K/V head
+// x the tokens of a block.
+template <typename T>
+bool encode_q(CUtensorMap* map, const AttnPaged& a, const SeqBatch& b, int head_dim) {
+  const PFN_cuTensorMapEncodeTiled_v12000 enc = cu_tensor_map_encoder();
+  if (enc == nullptr) return false;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(a.heads),
+                        static_cast<cuuint64_t>(b.n_rows)};
+  // (a stride that nothing is stepped with may be 0)
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.heads > 1 ? a.q_head : head_dim * 2),
+                           static_cast<cuuint64_t>(b.n_rows > 1 ? a.q_row : head_dim * 2)};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(128 / a.group)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, std::is_same<T, half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+             const_cast<char*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int HD, int NQ>
 cudaError_t launch_tc(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st) {
   using S = TcShape<HD, NQ>;
-  CUtensorMap km, vm;
+  CUtensorMap km, vm, qm;
   const int box = page_box_rows(kv);
-  if (!encode_pages<T>(&km, kv.k, kv, box) || !encode_pages<T>(&vm, kv.v, kv, box)) return cudaErrorInvalidValue;
-  attn_paged_tc_kernel<T, HD, NQ><<<a.n_cta, kTcPagedThreads, S::kSmem, st>>>(km, vm, a, b, kv, box, err);
+  if (!encode_pages<T>(&km, kv.k, kv, box) || !encode_pages<T>(&vm, kv.v, kv, box) ||
+      !encode_q<T>(&qm, a, b, HD))
+    return cudaErrorInvalidValue;
+  attn_paged_tc_kernel<T, HD, NQ><<<a.n_cta, kTcPagedThreads, S::kSmem, st>>>(km, vm, qm, a, b, kv, box, err);
   const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess ? e : launch_join<T, HD, S::kTile, NQ * 128, 128>(a, b, kv, st);
 }

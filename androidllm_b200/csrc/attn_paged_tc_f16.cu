@@ -7,5 +7,5 @@ cudaError_t launch_attn_paged_tc_f16(const AttnPaged& a, const SeqBatch& b, cons
   return launch_tc_t<half>(a, b, kv, nq, err, st);
 }
 cudaError_t attn_paged_tc_attrs_f16() { return tc_paged_attrs<half>(); }
-bool attn_paged_tc_fits(const PagedKV& kv) { return tc_paged_fits(kv); }
+bool attn_paged_tc_fits(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv) { return tc_paged_fits(a, b, kv); }
 }  // namespace alm

@@ -3,9 +3,10 @@
 // A unit is (sequence, block of up to `tpu` tokens, K/V head): its rows are
 // the tokens' query heads of that K/V head, its work the TILE-position tiles
 // its rows can see (one at least, so that rows that see nothing are written).
-// All units' tiles, in the order sequence, token block, head, tile, form one
-// line of T tiles; CTA i of n takes [T i / n, T (i + 1) / n).  Every CTA gets
-// the same share whatever the lengths are, with lengths that only the device
+// All units, in the order sequence, token block, head, lie on one line of T
+// places: kUnitCost places for what a unit costs beside its tiles (its first
+// scores, its result), then one a tile.  CTA i of n takes the tiles of places
+// [T i / n, T (i + 1) / n).  Every CTA gets the same share whatever the lengths are, with lengths that only the device
 // knows, and the split points depend on nothing but the batch, so results do
 // not change from run to run.  A unit cut by a share's end leaves one partial
 // result per CTA; a CTA owns at most two of those (its first and last unit).
@@ -15,6 +16,7 @@
 namespace alm {
 
 constexpr int kSchedThreads = 256;   // threads that run sched_init (warps 0 .. 7)
+constexpr int kUnitCost = 2;         // in tiles
 
 struct Unit {
   int s, mb, h;       // sequence, token block, K/V head
@@ -24,7 +26,12 @@ struct Unit {
   int n_kv;           // positions of the sequence
   const int* pages;
   int t0, n_tile;     // first tile and number of tiles
-  long long start;    // place of the first tile on the line
+  long long start;    // place of the first tile on the line (kUnitCost places after the unit's)
+  // whether the share's end x1 leaves tiles for a unit behind this one
+  ALM_DEV bool more(long long x1) const { return start + n_tile + kUnitCost < x1; }
+  // its tiles in a share [x0, x1): [from(x0), upto(x1))
+  ALM_DEV int from(long long x0) const { return x0 > start ? static_cast<int>(min(x0 - start, static_cast<long long>(n_tile))) : 0; }
+  ALM_DEV int upto(long long x1) const { return x1 > start ? static_cast<int>(min(x1 - start, static_cast<long long>(n_tile))) : 0; }
 };
 
 struct SchedShared {
@@ -45,14 +52,14 @@ ALM_DEV void block_tiles(const Seq& q, int tpu, int window, int mb, int& t0, int
   if (last < 0) t0 = 0;
 }
 
-// Tiles of one K/V head of sequence q, by one thread.
+// Places of one K/V head of sequence q, by one thread.
 template <int TILE>
 ALM_DEV long long seq_tiles(const Seq& q, int tpu, int window) {
   long long n = 0;
   for (int mb = 0; mb * tpu < q.n_new; ++mb) {
     int t0, nt;
     block_tiles<TILE>(q, tpu, window, mb, t0, nt);
-    n += nt;
+    n += nt + kUnitCost;
   }
   return n;
 }
@@ -87,7 +94,7 @@ ALM_DEV void sched_init(const SeqBatch& b, const PagedKV& kv, int tpu, int windo
       for (int mb = lane; mb * tpu < w.n_new; mb += kWarp) {
         int t0, nt;
         block_tiles<TILE>(w, tpu, window, mb, t0, nt);
-        part += nt;
+        part += nt + kUnitCost;
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
@@ -151,7 +158,7 @@ ALM_DEV Unit unit_at(const SeqBatch& b, const PagedKV& kv, int tpu, int window, 
     const int mb = mb0 + lane;
     int t0 = 0, nt = 0;
     if (mb * tpu < q.n_new) block_tiles<TILE>(q, tpu, window, mb, t0, nt);
-    long long sc = static_cast<long long>(nt) * kv.kv_heads;
+    long long sc = nt > 0 ? static_cast<long long>(nt + kUnitCost) * kv.kv_heads : 0;
     const long long mine = sc;
 #pragma unroll
     for (int o = 1; o < kWarp; o <<= 1) {
@@ -168,8 +175,8 @@ ALM_DEV Unit unit_at(const SeqBatch& b, const PagedKV& kv, int tpu, int window, 
     at += __shfl_sync(0xffffffffu, sc, kWarp - 1);
   }
   block_tiles<TILE>(q, tpu, window, u.mb, u.t0, u.n_tile);
-  u.h = min(static_cast<int>((g - at) / u.n_tile), kv.kv_heads - 1);
-  u.start = at + static_cast<long long>(u.h) * u.n_tile;
+  u.h = min(static_cast<int>((g - at) / (u.n_tile + kUnitCost)), kv.kv_heads - 1);
+  u.start = at + static_cast<long long>(u.h) * (u.n_tile + kUnitCost) + kUnitCost;
   u.row0 = q.row0 + u.mb * tpu;
   u.n_tok = min(tpu, q.n_new - u.mb * tpu);
   u.pos0 = q.n_kv - q.n_new + u.mb * tpu;
@@ -181,7 +188,7 @@ ALM_DEV Unit unit_at(const SeqBatch& b, const PagedKV& kv, int tpu, int window, 
 // The next unit on the line (there is one).
 template <int TILE>
 ALM_DEV void next_unit(const SeqBatch& b, const PagedKV& kv, int tpu, int window, Unit& u) {
-  u.start += u.n_tile;
+  u.start += u.n_tile + kUnitCost;
   if (++u.h < kv.kv_heads) return;
   u.h = 0;
   Seq q = load_seq(b, kv, u.s);

@@ -18,7 +18,7 @@ cudaError_t launch_attn_paged_f16(const AttnPaged& a, const SeqBatch& b, const P
 cudaError_t launch_attn_paged_bf16(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st);
 cudaError_t attn_paged_attrs_f16();
 cudaError_t attn_paged_attrs_bf16();
-bool attn_paged_tc_fits(const PagedKV& kv);
+bool attn_paged_tc_fits(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv);
 cudaError_t launch_attn_paged_tc_f16(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int nq, int* err,
                                      cudaStream_t st);
 cudaError_t launch_attn_paged_tc_bf16(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int nq, int* err,
@@ -223,7 +223,7 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   OnDevice on(device);
   const long long rows = static_cast<long long>(b.max_rows) * a.group;
   const bool bf = kv_->dtype == ALM_BF16;
-  if (rows > kTcMinRows && attn_paged_tc_fits(kv)) {
+  if (rows > kTcMinRows && attn_paged_tc_fits(a, b, kv)) {
     const int nq = rows > 128 ? 2 : 1;
     return cuda_status(bf ? launch_attn_paged_tc_bf16(a, b, kv, nq, err, st)
                           : launch_attn_paged_tc_f16(a, b, kv, nq, err, st),
