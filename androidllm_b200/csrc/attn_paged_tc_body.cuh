@@ -16,7 +16,7 @@
 // Warps 0-3 and 4-7: softmax of stream 0 and 1, one row a thread.  Warp 8:
 // issues the products.  Warp 9: loads K and V tiles with TMA, one box per page
 // piece and 64 columns, into a ring of tiles in the order they are used.  Warp
-// 10: loads Q.  Warp 11 is idle.
+// 10: loads Q.  Warp 11: clears V rows behind a sequence's end.
 //
 // The reference maximum m follows the row's maximum only when that has grown
 // by more than kSlack (in powers of two): weights stay below 2^kSlack, and the
@@ -37,9 +37,9 @@ namespace alm {
 
 // 12 warps launch with 168 registers a thread; the softmax warps (one row of S
 // a thread) then take kSoftRegs and the others keep kRestRegs:
-// 256 * 208 + 128 * 88 = 384 * 168.
+// 256 * 216 + 128 * 72 = 384 * 168.
 constexpr int kTcPagedThreads = 384;
-constexpr int kSoftRegs = 208, kRestRegs = 88;
+constexpr int kSoftRegs = 216, kRestRegs = 72;
 static_assert(256 * kSoftRegs + 128 * kRestRegs == kTcPagedThreads * 168, "the shares add up to the launch's registers");
 constexpr float kSlack = 8.f;
 
@@ -56,7 +56,8 @@ struct TcShape {
 struct TcShared {
   SchedShared sched;
   uint64_t full[10], empty[10];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], pv_done[2];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], pv_done[2], v_fix, v_fixed;
+  int v_slot;    // slot of the V tile to clear
   uint32_t tmem;
   int dead;      // a wait ran out: everybody leaves
 };
@@ -117,6 +118,13 @@ ALM_DEV float fmax3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// One lane of a converged warp.  (With this instruction, unlike a test of the
+// lane number, the compiler knows that one thread runs what follows.)
+ALM_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
 ALM_DEV void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 // Instruction descriptor: fp32 accumulator, A and B of type T, N wide; bmn: B
@@ -125,6 +133,19 @@ template <typename T>
 constexpr uint32_t tc_idesc(int n, bool bmn) {
   const uint32_t f = sizeof(T) == 2 && !std::is_same<T, half>::value ? 1u : 0u;
   return (1u << 4) | (f << 7) | (f << 10) | ((bmn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+// The rest of a wait whose first look failed: true when the phase completed.
+ALM_DEV bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
+  const unsigned long long t0 = global_ns();
+  for (unsigned i = 0; i < kSpinLimit; ++i) {
+    if (mbar_try_wait_suspend(bar, parity)) return true;
+    if (*dead) return false;
+    if (global_ns() - t0 > kWaitLimitNs) break;
+  }
+  *dead = 1;
+  *err = 2;
+  return false;
 }
 
 template <typename T, int HD, int NQ>
@@ -155,6 +176,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         mbar_init(&sh.p_full[i][0], 128), mbar_init(&sh.p_full[i][1], 128);
         mbar_init(&sh.pv_done[i], 1);
       }
+      mbar_init(&sh.v_fix, 1), mbar_init(&sh.v_fixed, 1);
       sh.dead = 0;
       fence_mbar_init();
     }
@@ -179,14 +201,19 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
   const long long x1 = cta < n_cta ? share(total, cta + 1, n_cta) : 0;
 
   volatile int* dead = &sh.dead;
-  // by whole warps, so that a wait that runs out ends for all lanes alike
-  auto gone = [&] { return __any_sync(0xffffffffu, *dead != 0) != 0; };
+  // Waits are bounded: one that runs out marks the CTA dead, and every role leaves.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (!gone() && !mbar_wait(bar, parity & 1)) {
-      *dead = 1;
-      *err = 2;
-    }
-    __syncwarp();
+    return mbar_try_wait(bar, parity & 1) || slow_wait(bar, parity & 1, dead, err);
+  };
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) {   // the same answer for the whole warp
+    const bool ok = wait(bar, parity);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
+  // The V tile that holds the sequence's end, when its last page piece goes on
+  // behind it: those rows hold anything, and a zero weight times NaN is NaN,
+  // so warp 11 clears them.
+  auto v_to_fix = [&](const Unit& u, int t) {
+    return (u.t0 + t + 1) * S::kTile > u.n_kv && u.n_kv % box_rows != 0 && u.n_kv > (u.t0 + t) * S::kTile;
   };
 
   // Each role walks this CTA's part of the line by itself.
@@ -214,7 +241,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
     Walk w;
-    if (x0 < x1 && warp <= 10 && w.start(b, kv, tpu, a.window, sh.sched, x0, x1)) {
+    if (x0 < x1 && w.start(b, kv, tpu, a.window, sh.sched, x0, x1)) {
     Unit& u = w.u;
     int &ta = w.ta, &tb = w.tb;
     auto next = [&] { w.next(b, kv, tpu, a.window); };
@@ -223,7 +250,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       // ---- loads ---------------------------------------------------------------
       int at = 0;
       uint32_t round = 0;
-      bool bad = false;
+      bool bad = false, quit = false;
       const int rows_total = kv.n_pages * kv.kv_heads * kv.page_size;
       const int n_box = 128 / box_rows * S::kChunks;
       auto load = [&](const CUtensorMap* map, int t) {
@@ -237,8 +264,10 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         bad |= in && !ok;
         // a row behind the tensor's end reads zeros
         const int y = ok ? (page * kv.kv_heads + u.h) * kv.page_size + pos - pi * kv.page_size : rows_total;
-        wait(&sh.empty[at], round ^ 1);
-        if (gone()) return;
+        if (quit || !wait_warp(&sh.empty[at], round ^ 1)) {
+          quit = true;
+          return;
+        }
         if (lane == 0) mbar_expect_tx(&sh.full[at], S::kTileBytes);
         __syncwarp();
         if (lane < n_box)
@@ -248,7 +277,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       };
       if (NQ == 2) {
         load(&k_map, ta);
-        for (bool go = true; go;) {
+        for (bool go = true; go && !quit;) {
           for (int t = ta; t < tb; ++t) {
             load(&v_map, t);
             if (t + 1 < tb) load(&k_map, t + 1);
@@ -260,7 +289,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           }
         }
       } else {
-        for (bool go = true; go;) {
+        for (bool go = true; go && !quit;) {
           load(&k_map, ta);
           if (ta + 1 < tb) load(&k_map, ta + 1);
           for (int t = ta; t < tb; ++t) {
@@ -274,7 +303,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       if (bad) *err = 1;
       // whatever happened, no copy is in flight when the CTA leaves: a slot's
       // last fill is complete once its barrier has left that phase
-      if (gone()) {
+      if (quit) {
         for (int i = 0; i < S::kSlots; ++i) {
           mbar_wait(&sh.full[i], 0);
           mbar_wait(&sh.full[i], 1);
@@ -286,10 +315,13 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       // next sequence that it may hold fill rows that nothing is written from
       uint32_t n = 0;
       const uint32_t bytes = static_cast<uint32_t>(tq * a.group) * 128 * S::kChunks;
-      for (bool go = true; go && !gone(); ++n) {
-        for (int i = 0; i < NQ; ++i) {
-          wait(&sh.q_empty[i], n ^ 1);
-          if (gone()) break;
+      bool quit = false;
+      for (bool go = true; go && !quit; ++n) {
+        for (int i = 0; i < NQ && !quit; ++i) {
+          if (!wait_warp(&sh.q_empty[i], n ^ 1)) {
+            quit = true;
+            break;
+          }
           if (lane == 0) {
             mbar_expect_tx(&sh.q_full[i], bytes);
 #pragma unroll
@@ -302,8 +334,33 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         go = more();
         if (go) next();
       }
-      if (gone())
+      if (quit)
         for (int i = 0; i < NQ; ++i) mbar_wait(&sh.q_full[i], 0), mbar_wait(&sh.q_full[i], 1);
+    } else if (warp == 11) {
+      // ---- V rows behind a sequence's end ----------------------------------------
+      // when the thread that issues the products finds such a tile loaded
+      uint32_t n = 0;
+      for (bool go = true, quit = false; go && !quit;) {
+        if (v_to_fix(u, tb - 1)) {
+          if (!wait_warp(&sh.v_fix, n++)) {
+            quit = true;
+          } else {
+            const int r0 = u.n_kv - (u.t0 + tb - 1) * S::kTile;
+            const int r1 = (r0 + box_rows - 1) / box_rows * box_rows;   // box_rows divides the tile
+            char* v = smem + (NQ + sh.v_slot) * S::kTileBytes;
+            for (int i = lane; i < (r1 - r0) * 8; i += kWarp)
+#pragma unroll
+              for (int c = 0; c < S::kChunks; ++c)
+                *reinterpret_cast<uint4*>(v + c * (128 * 128) + (r0 + i / 8) * 128 + (i % 8) * 16) =
+                    make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.v_fixed);
+          }
+        }
+        go = more();
+        if (go) next();
+      }
     } else {
       // ---- products ------------------------------------------------------------
       const uint32_t id_s = tc_idesc<T>(128, false), id_o = tc_idesc<T>(HD, true);
@@ -313,77 +370,62 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       auto step_ring = [&] {
         if (++at == S::kSlots) at = 0, round ^= 1;
       };
+      bool quit = false;
+      uint32_t n_fix = 0;
+      auto ready = [&](uint64_t* bar, uint32_t parity) {
+        if (!quit && !wait_warp(bar, parity)) quit = true;
+        tc_fence_after();
+      };
       // S of stream i from the K tile in the current slot
       auto qk = [&](int i) {
-        if (lane == 0) {
-          const uint32_t qa = smem0 + (NQ == 2 ? i : 0) * S::kTileBytes, ka = ring0 + at * S::kTileBytes;
+        if (quit || !elect_one()) return;
+        const uint32_t qa = smem0 + (NQ == 2 ? i : 0) * S::kTileBytes, ka = ring0 + at * S::kTileBytes;
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {
-            const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
-            tc_mma_ss(tmem + S::kColS + i * 128, sdesc128(qa + off, 16, 1024), sdesc128(ka + off, 16, 1024), id_s,
-                      k > 0);
-          }
-          tc_commit(&sh.s_full[i]);
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
+          tc_mma_ss(tmem + S::kColS + i * 128, sdesc128(qa + off, 16, 1024), sdesc128(ka + off, 16, 1024), id_s, k > 0);
         }
-        __syncwarp();
+        tc_commit(&sh.s_full[i]);
       };
       // O of stream i += P . V tile in the current slot, in two halves of 64
       // positions: the first product runs while the second half's weights are made
       auto pv = [&](int i, bool acc) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          wait(&sh.p_full[i][h], n_p[i]);
-          tc_fence_after();
-          if (lane == 0) {
+          ready(&sh.p_full[i][h], n_p[i]);
+          if (quit) return;
+          if (elect_one()) {
             const uint32_t va = ring0 + at * S::kTileBytes;
 #pragma unroll
             for (int k = 4 * h; k < 4 * h + 4; ++k)   // 16 positions: two groups of 8 rows of 128 bytes
               tc_mma_ts(tmem + S::kColO + i * HD, tmem + S::kColS + i * 128 + 8 * k,
                         sdesc128(va + k * 2048, 128 * 128, 1024), id_o, acc || k > 0);
+            if (h == 1) tc_commit(&sh.pv_done[i]);
           }
-          __syncwarp();
         }
         ++n_p[i];
-        if (lane == 0) tc_commit(&sh.pv_done[i]);
-        __syncwarp();
+      };
+      auto release = [&] {
+        if (!quit && elect_one()) tc_commit(&sh.empty[at]);
+        step_ring();
       };
       // nothing reads Q block i any more
       auto q_done = [&](int i) {
-        if (lane == 0) tc_commit(&sh.q_empty[i]);
-        __syncwarp();
+        if (!quit && elect_one()) tc_commit(&sh.q_empty[i]);
       };
-      auto release = [&] {
-        if (lane == 0) tc_commit(&sh.empty[at]);
-        __syncwarp();
-        step_ring();
-      };
-      // The V tile t: rows behind the sequence's end that came with its last
-      // page hold anything, and a zero weight times NaN is NaN: clear them.
       auto v_ready = [&](int t) {
-        wait(&sh.full[at], round);
-        const int base = (u.t0 + t) * S::kTile;
-        if (base + S::kTile > u.n_kv && !gone()) {
-          const int r0 = max(u.n_kv - base, 0);
-          const int r1 = min(S::kTile, (r0 + box_rows - 1) / box_rows * box_rows);
-          char* v = smem + (NQ + at) * S::kTileBytes;
-          for (int i = lane; i < (r1 - r0) * 8; i += kWarp)
-#pragma unroll
-            for (int c = 0; c < S::kChunks; ++c)
-              *reinterpret_cast<uint4*>(v + c * (128 * 128) + (r0 + i / 8) * 128 + (i % 8) * 16) =
-                  make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
+        ready(&sh.full[at], round);
+        if (t + 1 == tb && !quit && v_to_fix(u, t)) {
+          if (lane == 0) {
+            sh.v_slot = at;
+            mbar_arrive(&sh.v_fix);   // (releases the slot number, and the tile it has seen)
+          }
           __syncwarp();
+          ready(&sh.v_fixed, n_fix++);
         }
-        tc_fence_after();
       };
-      auto k_ready = [&] {
-        wait(&sh.full[at], round);
-        tc_fence_after();
-      };
-      auto q_ready = [&](int i) {
-        wait(&sh.q_full[i], n_q[i]++);
-        tc_fence_after();
-      };
+      auto k_ready = [&] { ready(&sh.full[at], round); };
+      auto q_ready = [&](int i) { ready(&sh.q_full[i], n_q[i]++); };
       if (NQ == 2) {
         q_ready(0);
         k_ready();
@@ -394,7 +436,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         if (ta + 1 == tb) q_done(1);
         release();
         bool first = true;   // tile t is the unit's first here
-        for (int t = ta; !gone();) {
+        for (int t = ta; !quit;) {
           const int v_at = at;
           const uint32_t v_round = round;
           const bool cross = t + 1 == tb, another = !cross || more();
@@ -423,7 +465,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           first = cross;
         }
       } else {
-        for (bool go = true; go && !gone();) {
+        for (bool go = true; go && !quit;) {
           q_ready(0);
           k_ready();
           qk(0);
@@ -434,7 +476,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
             release();
           }
           if (tb - ta <= 2) q_done(0);
-          for (int t = ta; t < tb && !gone(); ++t) {
+          for (int t = ta; t < tb && !quit; ++t) {
             const int i = (t - ta) & 1;
             v_ready(t);
             pv(i, t - ta >= 2);
@@ -481,7 +523,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         float m = kNegInf, l = 0.f;
         int n_mine = 0;
         for (int t = ca + (NQ == 1 ? st : 0); t < cb; t += NQ == 1 ? 2 : 1) {
-          wait(&sh.s_full[st], n_s);
+          wait_warp(&sh.s_full[st], n_s);
           tc_fence_after();
           if (any_live) {
             uint32_t sr[4][32];
@@ -516,7 +558,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
                 const float f = grow ? ex2((m - base) * a.scale_log2) : 1.f;
                 m = base;
                 l *= f;
-                wait(&sh.pv_done[st], n_s - 1);
+                wait_warp(&sh.pv_done[st], n_s - 1);
                 tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
@@ -569,7 +611,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
 
         // ---- the unit's end ------------------------------------------------------
         if (n_mine > 0) {
-          wait(&sh.pv_done[st], n_s - 1);
+          wait_warp(&sh.pv_done[st], n_s - 1);
           tc_fence_after();
         }
         const bool whole = ca == 0 && cb == cu.n_tile;
