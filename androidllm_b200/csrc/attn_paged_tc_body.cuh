@@ -13,10 +13,12 @@
 // tiles, with kNQ = 1 (at most 128 rows in a sequence) the even and the odd
 // tiles of one block, joined at the unit's end.
 //
-// Warps 0-3 and 4-7: softmax of stream 0 and 1, one row a thread.  Warp 8:
-// issues the products.  Warp 9: loads K and V tiles with TMA, one box per page
-// piece and 64 columns, into a ring of tiles in the order they are used.  Warp
-// 10: loads Q.  Warp 11: clears V rows behind a sequence's end.
+// Warps 0-3 and 4-7: softmax of stream 0 and 1, one row a thread.  Warps 8 and
+// 11: issue the products of stream 0 and 1 (a thread's issue of the 16 products
+// of a tile and its waits take about as long as the tensor core does, so one
+// for both streams held them up: 336 us against 290 us at 4 x 2047 rows).  Warp 9:
+// loads K and V tiles with TMA, one box per page piece and 64 columns, into a
+// ring of tiles.  Warp 10: loads Q.
 //
 // The reference maximum m follows the row's maximum only when that has grown
 // by more than kSlack (in powers of two): weights stay below 2^kSlack, and the
@@ -49,6 +51,10 @@ struct TcShape {
   static constexpr int kChunks = HD / 64;                  // 128-byte column groups
   static constexpr int kTileBytes = 128 * HD * 2;          // Q block, K or V tile
   static constexpr int kSlots = HD == 128 ? (NQ == 2 ? 5 : 6) : 10;
+  // slots of one ring: both streams follow every fill of a shared ring; where
+  // each has tiles of its own it has a ring of its own (a barrier's parity
+  // tells one phase from the next, not from the one after)
+  static constexpr int kRing = NQ == 2 ? kSlots : kSlots / 2;
   static constexpr size_t kSmem = static_cast<size_t>(NQ + kSlots) * kTileBytes + 1024;
   static constexpr int kColS = 0, kColO = 256, kTmemCols = 512;
 };
@@ -56,8 +62,7 @@ struct TcShape {
 struct TcShared {
   SchedShared sched;
   uint64_t full[10], empty[10];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], pv_done[2], v_fix, v_fixed;
-  int v_slot;    // slot of the V tile to clear
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], pv_done[2];
   uint32_t tmem;
   int dead;      // a wait ran out: everybody leaves
 };
@@ -168,15 +173,14 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
   grid_dep_launch();
   if (warp == 8) {
     if (lane == 0) {
-      for (int i = 0; i < S::kSlots; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
+      for (int i = 0; i < S::kSlots; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], NQ);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sh.q_full[i], 1);
-        mbar_init(&sh.q_empty[i], 1);
+        mbar_init(&sh.q_empty[i], 3 - NQ);
         mbar_init(&sh.s_full[i], 1);
         mbar_init(&sh.p_full[i][0], 128), mbar_init(&sh.p_full[i][1], 128);
         mbar_init(&sh.pv_done[i], 1);
       }
-      mbar_init(&sh.v_fix, 1), mbar_init(&sh.v_fixed, 1);
       sh.dead = 0;
       fence_mbar_init();
     }
@@ -209,13 +213,6 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     const bool ok = wait(bar, parity);
     return __all_sync(0xffffffffu, ok) != 0;
   };
-  // The V tile that holds the sequence's end, when its last page piece goes on
-  // behind it: those rows hold anything, and a zero weight times NaN is NaN,
-  // so warp 11 clears them.
-  auto v_to_fix = [&](const Unit& u, int t) {
-    return (u.t0 + t + 1) * S::kTile > u.n_kv && u.n_kv % box_rows != 0 && u.n_kv > (u.t0 + t) * S::kTile;
-  };
-
   // Each role walks this CTA's part of the line by itself.
   struct Walk {
     Unit u;
@@ -248,12 +245,13 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     auto more = [&] { return w.more(); };
     if (warp == 9) {
       // ---- loads ---------------------------------------------------------------
-      int at = 0;
-      uint32_t round = 0;
+      uint32_t fills[2] = {0, 0};   // of each ring
       bool bad = false, quit = false;
       const int rows_total = kv.n_pages * kv.kv_heads * kv.page_size;
       const int n_box = 128 / box_rows * S::kChunks;
-      auto load = [&](const CUtensorMap* map, int t) {
+      auto load = [&](const CUtensorMap* map, int t, int ring) {
+        const uint32_t fill = ring == 0 ? fills[0]++ : fills[1]++;
+        const int at = ring * S::kRing + fill % S::kRing;
         // one box a lane: at most 128 / 8 pieces of at most 2 column groups
         const int box = lane / S::kChunks, c = lane % S::kChunks;
         const int pos = (u.t0 + t) * S::kTile + box * box_rows;
@@ -264,7 +262,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         bad |= in && !ok;
         // a row behind the tensor's end reads zeros
         const int y = ok ? (page * kv.kv_heads + u.h) * kv.page_size + pos - pi * kv.page_size : rows_total;
-        if (quit || !wait_warp(&sh.empty[at], round ^ 1)) {
+        if (quit || !wait_warp(&sh.empty[at], fill / S::kRing + 1)) {
           quit = true;
           return;
         }
@@ -273,32 +271,14 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         if (lane < n_box)
           tma_2d(ring0 + at * S::kTileBytes + c * (128 * 128) + box * box_rows * 128, map, c * 64, y, &sh.full[at]);
         __syncwarp();
-        if (++at == S::kSlots) at = 0, round ^= 1;
       };
-      if (NQ == 2) {
-        load(&k_map, ta);
-        for (bool go = true; go && !quit;) {
-          for (int t = ta; t < tb; ++t) {
-            load(&v_map, t);
-            if (t + 1 < tb) load(&k_map, t + 1);
-          }
-          go = more();
-          if (go) {
-            next();
-            load(&k_map, ta);
-          }
+      for (bool go = true; go && !quit;) {
+        for (int t = ta; t < tb; ++t) {
+          load(&k_map, t, NQ == 2 ? 0 : (t - ta) & 1);
+          load(&v_map, t, NQ == 2 ? 0 : (t - ta) & 1);
         }
-      } else {
-        for (bool go = true; go && !quit;) {
-          load(&k_map, ta);
-          if (ta + 1 < tb) load(&k_map, ta + 1);
-          for (int t = ta; t < tb; ++t) {
-            load(&v_map, t);
-            if (t + 2 < tb) load(&k_map, t + 2);
-          }
-          go = more();
-          if (go) next();
-        }
+        go = more();
+        if (go) next();
       }
       if (bad) *err = 1;
       // whatever happened, no copy is in flight when the CTA leaves: a slot's
@@ -336,161 +316,99 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       }
       if (quit)
         for (int i = 0; i < NQ; ++i) mbar_wait(&sh.q_full[i], 0), mbar_wait(&sh.q_full[i], 1);
-    } else if (warp == 11) {
-      // ---- V rows behind a sequence's end ----------------------------------------
-      // when the thread that issues the products finds such a tile loaded
-      uint32_t n = 0;
-      for (bool go = true, quit = false; go && !quit;) {
-        if (v_to_fix(u, tb - 1)) {
-          if (!wait_warp(&sh.v_fix, n++)) {
-            quit = true;
-          } else {
-            const int r0 = u.n_kv - (u.t0 + tb - 1) * S::kTile;
-            const int r1 = (r0 + box_rows - 1) / box_rows * box_rows;   // box_rows divides the tile
-            char* v = smem + (NQ + sh.v_slot) * S::kTileBytes;
-            for (int i = lane; i < (r1 - r0) * 8; i += kWarp)
-#pragma unroll
-              for (int c = 0; c < S::kChunks; ++c)
-                *reinterpret_cast<uint4*>(v + c * (128 * 128) + (r0 + i / 8) * 128 + (i % 8) * 16) =
-                    make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.v_fixed);
-          }
-        }
-        go = more();
-        if (go) next();
-      }
     } else {
-      // ---- products ------------------------------------------------------------
+      // ---- products of stream i (the whole warp walks, one lane issues) ----------
+      const int i = warp == 8 ? 0 : 1;
+      constexpr int kStep = NQ == 2 ? 1 : 2;           // the stream's tiles of a unit: every, or every second
+      const int q_blk = NQ == 2 ? i : 0;
       const uint32_t id_s = tc_idesc<T>(128, false), id_o = tc_idesc<T>(HD, true);
-      int at = 0;
-      uint32_t round = 0;
-      uint32_t n_p[2] = {0, 0}, n_q[2] = {0, 0};
-      auto step_ring = [&] {
-        if (++at == S::kSlots) at = 0, round ^= 1;
-      };
+      const uint32_t qa = smem0 + q_blk * S::kTileBytes;
+      const uint32_t d_s = tmem + S::kColS + i * 128, d_o = tmem + S::kColO + i * HD;
+      uint32_t n_p = 0, n_u = 0;                       // tiles and units of the stream so far
+      // K and V of the stream's n-th tile are fills 2 n and 2 n + 1 of its ring
+      const uint32_t ring = NQ == 2 ? 0 : i * S::kRing;
+      int t = ta, t_first = ta;
       bool quit = false;
-      uint32_t n_fix = 0;
       auto ready = [&](uint64_t* bar, uint32_t parity) {
         if (!quit && !wait_warp(bar, parity)) quit = true;
         tc_fence_after();
       };
-      // S of stream i from the K tile in the current slot
-      auto qk = [&](int i) {
+      // S = Q . K^T of tile t; then its K may go, and after the unit's last so may Q
+      auto qk = [&] {
+        const uint32_t fill = 2 * n_p, at = ring + fill % S::kRing;
+        ready(&sh.full[at], fill / S::kRing);
         if (quit || !elect_one()) return;
-        const uint32_t qa = smem0 + (NQ == 2 ? i : 0) * S::kTileBytes, ka = ring0 + at * S::kTileBytes;
+        const uint32_t ka = ring0 + at * S::kTileBytes;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
-          tc_mma_ss(tmem + S::kColS + i * 128, sdesc128(qa + off, 16, 1024), sdesc128(ka + off, 16, 1024), id_s, k > 0);
+          tc_mma_ss(d_s, sdesc128(qa + off, 16, 1024), sdesc128(ka + off, 16, 1024), id_s, k > 0);
         }
         tc_commit(&sh.s_full[i]);
+        tc_commit(&sh.empty[at]);
+        if (t + kStep >= tb) tc_commit(&sh.q_empty[q_blk]);
       };
-      // O of stream i += P . V tile in the current slot, in two halves of 64
-      // positions: the first product runs while the second half's weights are made
-      auto pv = [&](int i, bool acc) {
+      // O += P . V of tile t in two halves of 64 positions: the first product
+      // runs while the second half's weights are made
+      auto pv = [&] {
+        const uint32_t fill = 2 * n_p + 1, at = ring + fill % S::kRing;
+        ready(&sh.full[at], fill / S::kRing);
+        const int base = (u.t0 + t) * S::kTile, r0 = u.n_kv - base;
+        if (r0 < S::kTile && r0 > 0 && !quit) {
+          // The sequence ends in this tile, and its last page piece goes on
+          // behind it: those rows hold anything, and a zero weight times NaN
+          // is NaN.  (Both streams of a shared tile write the same zeros.)
+          const int r1 = (r0 + box_rows - 1) / box_rows * box_rows;   // box_rows divides the tile
+          char* v = smem + (NQ + at) * S::kTileBytes;
+          for (int j = lane; j < (r1 - r0) * 8; j += kWarp)
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+              *reinterpret_cast<uint4*>(v + c * (128 * 128) + (r0 + j / 8) * 128 + (j % 8) * 16) =
+                  make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          ready(&sh.p_full[i][h], n_p[i]);
+          ready(&sh.p_full[i][h], n_p);
           if (quit) return;
           if (elect_one()) {
             const uint32_t va = ring0 + at * S::kTileBytes;
 #pragma unroll
             for (int k = 4 * h; k < 4 * h + 4; ++k)   // 16 positions: two groups of 8 rows of 128 bytes
-              tc_mma_ts(tmem + S::kColO + i * HD, tmem + S::kColS + i * 128 + 8 * k,
-                        sdesc128(va + k * 2048, 128 * 128, 1024), id_o, acc || k > 0);
-            if (h == 1) tc_commit(&sh.pv_done[i]);
-          }
-        }
-        ++n_p[i];
-      };
-      auto release = [&] {
-        if (!quit && elect_one()) tc_commit(&sh.empty[at]);
-        step_ring();
-      };
-      // nothing reads Q block i any more
-      auto q_done = [&](int i) {
-        if (!quit && elect_one()) tc_commit(&sh.q_empty[i]);
-      };
-      auto v_ready = [&](int t) {
-        ready(&sh.full[at], round);
-        if (t + 1 == tb && !quit && v_to_fix(u, t)) {
-          if (lane == 0) {
-            sh.v_slot = at;
-            mbar_arrive(&sh.v_fix);   // (releases the slot number, and the tile it has seen)
-          }
-          __syncwarp();
-          ready(&sh.v_fixed, n_fix++);
-        }
-      };
-      auto k_ready = [&] { ready(&sh.full[at], round); };
-      auto q_ready = [&](int i) { ready(&sh.q_full[i], n_q[i]++); };
-      if (NQ == 2) {
-        q_ready(0);
-        k_ready();
-        qk(0);
-        if (ta + 1 == tb) q_done(0);
-        q_ready(1);
-        qk(1);
-        if (ta + 1 == tb) q_done(1);
-        release();
-        bool first = true;   // tile t is the unit's first here
-        for (int t = ta; !quit;) {
-          const int v_at = at;
-          const uint32_t v_round = round;
-          const bool cross = t + 1 == tb, another = !cross || more();
-          v_ready(t);
-          pv(0, !first);
-          step_ring();
-          if (cross && another) next();
-          t = cross ? ta : t + 1;
-          if (another) {
-            if (cross) q_ready(0);
-            k_ready();
-            qk(0);
-            if (t + 1 == tb) q_done(0);
-          }
-          const int k_at = at;
-          const uint32_t k_round = round;
-          at = v_at, round = v_round;
-          pv(1, !first);
-          release();
-          at = k_at, round = k_round;
-          if (!another) break;
-          if (cross) q_ready(1);
-          qk(1);
-          if (t + 1 == tb) q_done(1);
-          release();
-          first = cross;
-        }
-      } else {
-        for (bool go = true; go && !quit;) {
-          q_ready(0);
-          k_ready();
-          qk(0);
-          release();
-          if (ta + 1 < tb) {
-            k_ready();
-            qk(1);
-            release();
-          }
-          if (tb - ta <= 2) q_done(0);
-          for (int t = ta; t < tb && !quit; ++t) {
-            const int i = (t - ta) & 1;
-            v_ready(t);
-            pv(i, t - ta >= 2);
-            release();
-            if (t + 2 < tb) {
-              k_ready();
-              qk(i);
-              release();
-              if (t + 3 == tb) q_done(0);
+              tc_mma_ts(d_o, d_s + 8 * k, sdesc128(va + k * 2048, 128 * 128, 1024), id_o, t > t_first || k > 0);
+            if (h == 1) {
+              tc_commit(&sh.pv_done[i]);
+              tc_commit(&sh.empty[at]);
             }
           }
-          go = more();
-          if (go) next();
         }
+        ++n_p;
+      };
+      // the stream's first tile of this unit or a later one; false: there is none
+      auto enter = [&] {
+        for (;;) {
+          t = t_first = NQ == 2 ? ta : ta + i;
+          ready(&sh.q_full[q_blk], n_u++);
+          if (quit) return false;
+          if (t < tb) return true;
+          if (lane == 0) mbar_arrive(&sh.q_empty[q_blk]);   // reads nothing of this Q
+          if (!more()) return false;
+          next();
+        }
+      };
+      bool go = enter();
+      if (go) qk();
+      while (go && !quit) {
+        pv();
+        if (t + kStep < tb) {
+          t += kStep;
+        } else {
+          if (!more()) break;
+          next();
+          go = enter();
+        }
+        if (go) qk();
       }
     }
     }

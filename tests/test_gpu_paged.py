@@ -225,10 +225,26 @@ def test_attend_4096_sequences(ctx):
     check_attend(ctx, b, b.randn(b.n_rows, 1, 32))
 
 
-@pytest.mark.parametrize("rows", [1, 7, 60])
-def test_attend_long_context_joined_from_many_parts(ctx, rows):
-    b = Batch([rows], [40000], 64, 2, 128, torch.float16, seed=6)
-    check_attend(ctx, b, b.randn(b.n_rows, 8, 128))
+@pytest.mark.parametrize("rows", [1, 7, 20, 31, 60])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_long_context_joined_from_many_parts(ctx, rows, dim):
+    b = Batch([rows], [60000], 64, 2, dim, torch.float16, seed=6)
+    q = b.randn(b.n_rows, 8, dim)
+    first = check_attend(ctx, b, q)
+    for _ in range(10):
+        out, _ = attend(ctx, b, q)
+        assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("most", [10, 32, 200])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_many_units_a_cta(ctx, most, dim):
+    """Hundreds of sequences of every small number of tiles: each CTA runs through dozens of units."""
+    n = 900
+    rows = [1 + (i * 13) % most for i in range(n)]
+    lens = [r + (i * 101) % 900 for i, r in enumerate(rows)]
+    b = Batch(rows, lens, 16, 1, dim, torch.bfloat16, seed=5)
+    check_attend(ctx, b, b.randn(b.n_rows, 4, dim))
 
 
 def test_attend_slots_strides_and_scale(ctx):
