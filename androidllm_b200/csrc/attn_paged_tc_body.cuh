@@ -130,6 +130,7 @@ ALM_DEV bool elect_one() {
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
   return p != 0;
 }
+ALM_DEV void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 ALM_DEV void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 // Instruction descriptor: fp32 accumulator, A and B of type T, N wide; bmn: B
@@ -333,12 +334,14 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         if (!quit && !wait_warp(bar, parity)) quit = true;
         tc_fence_after();
       };
-      // S = Q . K^T of tile t; then its K may go, and after the unit's last so may Q
-      auto qk = [&] {
-        const uint32_t fill = 2 * n_p, at = ring + fill % S::kRing;
-        ready(&sh.full[at], fill / S::kRing);
+      // K tile of the stream's n-th tile
+      auto k_ready = [&](uint32_t n) { ready(&sh.full[ring + 2 * n % S::kRing], 2 * n / S::kRing); };
+      // S = Q . K^T of tile t, whose K is there.  One commit tells that all
+      // products so far are done, the last P . V among them; then its K (and a V
+      // that is done with) may go, and after the unit's last so may Q.
+      auto qk = [&](int v_slot) {
         if (quit || !elect_one()) return;
-        const uint32_t ka = ring0 + at * S::kTileBytes;
+        const uint32_t at = ring + 2 * n_p % S::kRing, ka = ring0 + at * S::kTileBytes;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
@@ -346,11 +349,12 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         }
         tc_commit(&sh.s_full[i]);
         tc_commit(&sh.empty[at]);
+        if (v_slot >= 0) tc_commit(&sh.empty[v_slot]);
         if (t + kStep >= tb) tc_commit(&sh.q_empty[q_blk]);
       };
       // O += P . V of tile t in two halves of 64 positions: the first product
-      // runs while the second half's weights are made
-      auto pv = [&] {
+      // runs while the second half's weights are made.  Returns V's slot.
+      auto pv = [&](bool last) {
         const uint32_t fill = 2 * n_p + 1, at = ring + fill % S::kRing;
         ready(&sh.full[at], fill / S::kRing);
         const int base = (u.t0 + t) * S::kTile, r0 = u.n_kv - base;
@@ -368,22 +372,26 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           fence_proxy_async_smem();
           __syncwarp();
         }
+        // the next tile's K before the weights: it is there long since, and
+        // then nothing stands between this product and the next
+        if (!last) k_ready(n_p + 1);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           ready(&sh.p_full[i][h], n_p);
-          if (quit) return;
+          if (quit) return -1;
           if (elect_one()) {
             const uint32_t va = ring0 + at * S::kTileBytes;
 #pragma unroll
             for (int k = 4 * h; k < 4 * h + 4; ++k)   // 16 positions: two groups of 8 rows of 128 bytes
               tc_mma_ts(d_o, d_s + 8 * k, sdesc128(va + k * 2048, 128 * 128, 1024), id_o, t > t_first || k > 0);
-            if (h == 1) {
+            if (last && h == 1) {
               tc_commit(&sh.pv_done[i]);
               tc_commit(&sh.empty[at]);
             }
           }
         }
         ++n_p;
+        return static_cast<int>(at);
       };
       // the stream's first tile of this unit or a later one; false: there is none
       auto enter = [&] {
@@ -398,17 +406,25 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         }
       };
       bool go = enter();
-      if (go) qk();
+      if (go) {
+        k_ready(0);
+        qk(-1);
+      }
       while (go && !quit) {
-        pv();
         if (t + kStep < tb) {
+          const int v_slot = pv(false);
           t += kStep;
+          qk(v_slot);
         } else {
+          pv(true);
           if (!more()) break;
           next();
           go = enter();
+          if (go) {
+            k_ready(n_p);
+            qk(-1);
+          }
         }
-        if (go) qk();
       }
     }
     }
@@ -427,8 +443,9 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       const uint32_t t_o = tc_addr(tmem + S::kColO + st * HD, (warp % 4) * 32, 0);
       const int blk = NQ == 2 ? st : 0;                // 128-row block of the unit
       uint32_t n_s = 0;                                // tiles of this stream so far
+      if (NQ == 2 && st == 1) bar_arrive(2, 256);      // stream 0 has the first turn
 
-      uint32_t n_u = 0;                                // units so far
+      uint32_t n_u = 0, n_done = 0;                    // units so far, and those with a tile
       for (bool go = true; go;) {
         const Unit cu = u;
         const int ca = ta, cb = tb;
@@ -443,7 +460,12 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         for (int t = ca + (NQ == 1 ? st : 0); t < cb; t += NQ == 1 ? 2 : 1) {
           wait_warp(&sh.s_full[st], n_s);
           tc_fence_after();
-          if (any_live) {
+          if (!any_live) {
+            if (NQ == 2) bar_sync(2 + st, 256);
+            mbar_arrive(&sh.p_full[st][0]);
+            mbar_arrive(&sh.p_full[st][1]);
+            if (NQ == 2) bar_arrive(3 - st, 256);
+          } else {
             uint32_t sr[4][32];
 #pragma unroll
             for (int i = 0; i < 4; ++i) tc_ld32(t_s + 32 * i, sr[i]);
@@ -476,8 +498,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
                 const float f = grow ? ex2((m - base) * a.scale_log2) : 1.f;
                 m = base;
                 l *= f;
-                wait_warp(&sh.pv_done[st], n_s - 1);
-                tc_fence_after();
+                // (the scores' commit covers the product before them, so O is at rest)
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
                   uint32_t ov[32];
@@ -491,6 +512,9 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
               }
             }
             const float mc = m == kNegInf ? 0.f : m * a.scale_log2;
+            // The streams take turns at the exponentials: together they would
+            // share that unit first and the tensor core afterwards.
+            if (NQ == 2) bar_sync(2 + st, 256);
             const uint64_t c2 = pair(a.scale_log2, a.scale_log2), m2 = pair(-mc, -mc);
             uint64_t sum[2] = {0, 0};   // (+0, +0)
 #pragma unroll
@@ -512,13 +536,11 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
               tc_fence_before();
               mbar_arrive(&sh.p_full[st][h]);
             }
+            if (NQ == 2) bar_arrive(3 - st, 256);
             float s0, s1, s2, s3;
             unpair(sum[0], s0, s1);
             unpair(sum[1], s2, s3);
             l += (s0 + s1) + (s2 + s3);
-          } else {
-            mbar_arrive(&sh.p_full[st][0]);
-            mbar_arrive(&sh.p_full[st][1]);
           }
           ++n_s;
           ++n_mine;
@@ -529,7 +551,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
 
         // ---- the unit's end ------------------------------------------------------
         if (n_mine > 0) {
-          wait_warp(&sh.pv_done[st], n_s - 1);
+          wait_warp(&sh.pv_done[st], n_done++);
           tc_fence_after();
         }
         const bool whole = ca == 0 && cb == cu.n_tile;
