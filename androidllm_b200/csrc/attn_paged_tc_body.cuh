@@ -44,6 +44,10 @@ constexpr int kTcPagedThreads = 384;
 constexpr int kSoftRegs = 216, kRestRegs = 72;
 static_assert(256 * kSoftRegs + 128 * kRestRegs == kTcPagedThreads * 168, "the shares add up to the launch's registers");
 constexpr float kSlack = 8.f;
+#ifndef KTURNS
+#define KTURNS true
+#endif
+constexpr bool kTurns = KTURNS;
 
 template <int HD, int NQ>
 struct TcShape {
@@ -87,6 +91,23 @@ ALM_DEV void tc_ld32(uint32_t taddr, uint32_t (&d)[32]) {
         "=r"(d[25]), "=r"(d[26]), "=r"(d[27]), "=r"(d[28]), "=r"(d[29]), "=r"(d[30]), "=r"(d[31])
       : "r"(taddr));
 }
+// After tc_ld32: the values have arrived (named, so that nothing that uses
+// them is moved before the wait).
+ALM_DEV void tc_landed(uint32_t (&d)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]), "+r"(d[4]), "+r"(d[5]), "+r"(d[6]), "+r"(d[7]),
+                 "+r"(d[8]), "+r"(d[9]), "+r"(d[10]), "+r"(d[11]), "+r"(d[12]), "+r"(d[13]), "+r"(d[14]), "+r"(d[15]),
+                 "+r"(d[16]), "+r"(d[17]), "+r"(d[18]), "+r"(d[19]), "+r"(d[20]), "+r"(d[21]), "+r"(d[22]),
+                 "+r"(d[23]), "+r"(d[24]), "+r"(d[25]), "+r"(d[26]), "+r"(d[27]), "+r"(d[28]), "+r"(d[29]),
+                 "+r"(d[30]), "+r"(d[31])::"memory");
+}
+ALM_DEV void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 ALM_DEV void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -122,6 +143,18 @@ ALM_DEV float fmax3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+ALM_DEV float max64(const uint32_t (&a)[32], const uint32_t (&b)[32]) {
+  float t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t* v = i < 2 ? a + 16 * i : b + 16 * (i - 2);
+    t[i] = fmax3(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
+#pragma unroll
+    for (int j = 3; j < 15; j += 2) t[i] = fmax3(t[i], __uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+    t[i] = fmaxf(t[i], __uint_as_float(v[15]));
+  }
+  return fmaxf(fmax3(t[0], t[1], t[2]), t[3]);
 }
 // One lane of a converged warp.  (With this instruction, unlike a test of the
 // lane number, the compiler knows that one thread runs what follows.)
@@ -443,7 +476,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       const uint32_t t_o = tc_addr(tmem + S::kColO + st * HD, (warp % 4) * 32, 0);
       const int blk = NQ == 2 ? st : 0;                // 128-row block of the unit
       uint32_t n_s = 0;                                // tiles of this stream so far
-      if (NQ == 2 && st == 1) bar_arrive(2, 256);      // stream 0 has the first turn
+      if (kTurns && NQ == 2 && st == 1) bar_arrive(2, 256);      // stream 0 has the first turn
 
       uint32_t n_u = 0, n_done = 0;                    // units so far, and those with a tile
       for (bool go = true; go;) {
@@ -461,65 +494,39 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           wait_warp(&sh.s_full[st], n_s);
           tc_fence_after();
           if (!any_live) {
-            if (NQ == 2) bar_sync(2 + st, 256);
+            if (kTurns && NQ == 2) bar_sync(2 + st, 256);
             mbar_arrive(&sh.p_full[st][0]);
             mbar_arrive(&sh.p_full[st][1]);
-            if (NQ == 2) bar_arrive(3 - st, 256);
+            if (kTurns && NQ == 2) bar_arrive(3 - st, 256);
           } else {
             uint32_t sr[4][32];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) tc_ld32(t_s + 32 * i, sr[i]);
-            tc_wait_ld();
+            tc_ld32(t_s, sr[0]);
+            tc_ld32(t_s + 32, sr[1]);
             const int p0 = (cu.t0 + t) * S::kTile;
-            if (p0 + S::kTile - 1 > pos_a || (a.window > 0 && p0 <= pos_b - a.window)) {
-              const int lo = a.window > 0 ? hi - a.window + 1 : 0;
+            const bool mask = p0 + S::kTile - 1 > pos_a || (a.window > 0 && p0 <= pos_b - a.window);
+            const int lo = a.window > 0 ? hi - a.window + 1 : 0;
+            auto hide = [&](int h) {
 #pragma unroll
-              for (int i = 0; i < 128; ++i) {
+              for (int i = 64 * h; i < 64 * h + 64; ++i) {
                 const int p = p0 + i;
                 if (p > hi || p < lo) sr[i / 32][i % 32] = 0xff800000u;
               }
-            }
-            float top[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              top[i] = fmax3(__uint_as_float(sr[i][0]), __uint_as_float(sr[i][1]), __uint_as_float(sr[i][2]));
-#pragma unroll
-              for (int j = 3; j < 31; j += 2)
-                top[i] = fmax3(top[i], __uint_as_float(sr[i][j]), __uint_as_float(sr[i][j + 1]));
-              top[i] = fmaxf(top[i], __uint_as_float(sr[i][31]));
-            }
-            const float row_top = fmaxf(fmax3(top[0], top[1], top[2]), top[3]);
-            if (n_mine == 0) {
-              m = row_top;
-            } else {
-              const bool grow = row_top > m && !((row_top - m) * a.scale_log2 <= kSlack);
-              if (__any_sync(0xffffffffu, grow)) {
-                const float base = grow ? row_top : m;
-                const float f = grow ? ex2((m - base) * a.scale_log2) : 1.f;
-                m = base;
-                l *= f;
-                // (the scores' commit covers the product before them, so O is at rest)
-#pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                  uint32_t ov[32];
-                  tc_ld32(t_o + 32 * c, ov);
-                  tc_wait_ld();
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * f);
-                  tc_st32(t_o + 32 * c, ov);
-                }
-                tc_wait_st();
-              }
-            }
-            const float mc = m == kNegInf ? 0.f : m * a.scale_log2;
+            };
+            tc_landed(sr[0]);
+            tc_landed(sr[1]);
+            tc_ld32(t_s + 64, sr[2]);
+            tc_ld32(t_s + 96, sr[3]);
+            if (mask) hide(0);
             // The streams take turns at the exponentials: together they would
             // share that unit first and the tensor core afterwards.
-            if (NQ == 2) bar_sync(2 + st, 256);
-            const uint64_t c2 = pair(a.scale_log2, a.scale_log2), m2 = pair(-mc, -mc);
-            uint64_t sum[2] = {0, 0};   // (+0, +0)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t pr[32];
+            if (kTurns && NQ == 2) bar_sync(2 + st, 256);
+            // The first half's weights by the reference so far: the maximum of
+            // the tile is taken beside them, not before, and only where it has
+            // grown too far are they made again.
+            const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
+            uint64_t sum[2], m2;
+            uint32_t pr[32];
+            auto weights = [&](int h) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 const int e = 64 * h + 2 * j;
@@ -531,12 +538,45 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
                 sum[j & 1] = add2(sum[j & 1], pair(p, q));
                 pr[j] = Elem<T>::pack(p, q);
               }
+            };
+#pragma unroll 1
+            for (bool again = false;; again = true) {
+              const float mc = m == kNegInf ? 0.f : m * a.scale_log2;
+              m2 = pair(-mc, -mc);
+              sum[0] = sum[1] = 0;   // (+0, +0)
+              weights(0);
+              if (again) break;
+              tc_landed(sr[2]);
+              tc_landed(sr[3]);
+              if (mask) hide(1);
+              const float row_top = fmaxf(max64(sr[0], sr[1]), max64(sr[2], sr[3]));
+              const bool grow = row_top > m && !((row_top - m) * a.scale_log2 <= kSlack);
+              if (!__any_sync(0xffffffffu, grow)) break;
+              const float f = grow ? ex2((m - row_top) * a.scale_log2) : 1.f;
+              if (grow) m = row_top;
+              l *= f;
+              if (n_mine > 0) {
+                // (the scores' commit covers the product before them, so O is at rest)
+#pragma unroll 1
+                for (int c = 0; c < HD / 16; ++c) {
+                  uint32_t ov[16];
+                  tc_ld16(t_o + 16 * c, ov);
+                  tc_wait_ld();
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * f);
+                  tc_st16(t_o + 16 * c, ov);
+                }
+              }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h == 1) weights(1);
               tc_st32(t_s + 32 * h, pr);
               tc_wait_st();
               tc_fence_before();
               mbar_arrive(&sh.p_full[st][h]);
             }
-            if (NQ == 2) bar_arrive(3 - st, 256);
+            if (kTurns && NQ == 2) bar_arrive(3 - st, 256);
             float s0, s1, s2, s3;
             unpair(sum[0], s0, s1);
             unpair(sum[1], s2, s3);
@@ -566,7 +606,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
             for (int c = 0; c < HD / 32; ++c) {
               uint32_t ov[32];
               tc_ld32(t_o + 32 * c, ov);
-              tc_wait_ld();
+              tc_landed(ov);
 #pragma unroll
               for (int j = 0; j < 32; j += 4)
                 *reinterpret_cast<uint4*>(half_sum + r * HD + 32 * c + j) =
@@ -602,7 +642,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           for (int c = 0; c < HD / 32; ++c) {
             uint32_t ov[32];
             tc_ld32(t_o + 32 * c, ov);
-            tc_wait_ld();
+            tc_landed(ov);
             float o[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(ov[j]) * w0;
