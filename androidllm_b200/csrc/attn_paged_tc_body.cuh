@@ -44,10 +44,6 @@ constexpr int kTcPagedThreads = 384;
 constexpr int kSoftRegs = 216, kRestRegs = 72;
 static_assert(256 * kSoftRegs + 128 * kRestRegs == kTcPagedThreads * 168, "the shares add up to the launch's registers");
 constexpr float kSlack = 8.f;
-#ifndef KTURNS
-#define KTURNS true
-#endif
-constexpr bool kTurns = KTURNS;
 
 template <int HD, int NQ>
 struct TcShape {
@@ -100,6 +96,18 @@ ALM_DEV void tc_landed(uint32_t (&d)[32]) {
                  "+r"(d[16]), "+r"(d[17]), "+r"(d[18]), "+r"(d[19]), "+r"(d[20]), "+r"(d[21]), "+r"(d[22]),
                  "+r"(d[23]), "+r"(d[24]), "+r"(d[25]), "+r"(d[26]), "+r"(d[27]), "+r"(d[28]), "+r"(d[29]),
                  "+r"(d[30]), "+r"(d[31])::"memory");
+}
+// 32 columns of 16 lanes (tensor-memory lanes of the address and the 15 behind
+// it): register 4 q + 2 k + e of lane l is row l / 4 + 8 k, column 8 q + 2 (l
+// mod 4) + e.  Waits for the values.
+ALM_DEV void tc_ld_rows(uint32_t taddr, uint32_t (&d)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]), "=r"(d[8]),
+        "=r"(d[9]), "=r"(d[10]), "=r"(d[11]), "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15])
+      : "r"(taddr)
+      : "memory");
 }
 ALM_DEV void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -476,12 +484,14 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       const uint32_t t_o = tc_addr(tmem + S::kColO + st * HD, (warp % 4) * 32, 0);
       const int blk = NQ == 2 ? st : 0;                // 128-row block of the unit
       uint32_t n_s = 0;                                // tiles of this stream so far
-      if (kTurns && NQ == 2 && st == 1) bar_arrive(2, 256);      // stream 0 has the first turn
+      if (NQ == 2 && st == 1) bar_arrive(2, 256);      // stream 0 has the first turn
 
       uint32_t n_u = 0, n_done = 0;                    // units so far, and those with a tile
       for (bool go = true; go;) {
         const Unit cu = u;
         const int ca = ta, cb = tb;
+        go = more();
+        if (go) next();                                  // early: its lengths are loads
         const int tk = r / a.group, tok = blk * tq + tk, head = cu.h * a.group + r - tk * a.group;
         const bool live = tk < tq && tok < cu.n_tok;
         const int hi = live ? cu.pos0 + tok : -1;       // last position the row sees
@@ -494,22 +504,25 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           wait_warp(&sh.s_full[st], n_s);
           tc_fence_after();
           if (!any_live) {
-            if (kTurns && NQ == 2) bar_sync(2 + st, 256);
+            if (NQ == 2) bar_sync(2 + st, 256);
             mbar_arrive(&sh.p_full[st][0]);
             mbar_arrive(&sh.p_full[st][1]);
-            if (kTurns && NQ == 2) bar_arrive(3 - st, 256);
+            if (NQ == 2) bar_arrive(3 - st, 256);
           } else {
             uint32_t sr[4][32];
             tc_ld32(t_s, sr[0]);
             tc_ld32(t_s + 32, sr[1]);
             const int p0 = (cu.t0 + t) * S::kTile;
             const bool mask = p0 + S::kTile - 1 > pos_a || (a.window > 0 && p0 <= pos_b - a.window);
-            const int lo = a.window > 0 ? hi - a.window + 1 : 0;
+            const int n_hi = hi - p0, n_lo = hi - a.window - p0;   // columns > n_hi, and with a window <= n_lo, are hidden
             auto hide = [&](int h) {
 #pragma unroll
-              for (int i = 64 * h; i < 64 * h + 64; ++i) {
-                const int p = p0 + i;
-                if (p > hi || p < lo) sr[i / 32][i % 32] = 0xff800000u;
+              for (int i = 64 * h; i < 64 * h + 64; ++i)
+                sr[i / 32][i % 32] = i > n_hi ? 0xff800000u : sr[i / 32][i % 32];
+              if (a.window > 0) {
+#pragma unroll
+                for (int i = 64 * h; i < 64 * h + 64; ++i)
+                  sr[i / 32][i % 32] = i <= n_lo ? 0xff800000u : sr[i / 32][i % 32];
               }
             };
             tc_landed(sr[0]);
@@ -517,45 +530,19 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
             tc_ld32(t_s + 64, sr[2]);
             tc_ld32(t_s + 96, sr[3]);
             if (mask) hide(0);
-            // The streams take turns at the exponentials: together they would
-            // share that unit first and the tensor core afterwards.
-            if (kTurns && NQ == 2) bar_sync(2 + st, 256);
-            // The first half's weights by the reference so far: the maximum of
-            // the tile is taken beside them, not before, and only where it has
-            // grown too far are they made again.
-            const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
-            uint64_t sum[2], m2;
-            uint32_t pr[32];
-            auto weights = [&](int h) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int e = 64 * h + 2 * j;
-                float p, q;
-                unpair(fma2(pair(__uint_as_float(sr[e / 32][e % 32]), __uint_as_float(sr[e / 32][e % 32 + 1])), c2, m2),
-                       p, q);
-                p = ex2(p);
-                q = ex2(q);
-                sum[j & 1] = add2(sum[j & 1], pair(p, q));
-                pr[j] = Elem<T>::pack(p, q);
-              }
-            };
-#pragma unroll 1
-            for (bool again = false;; again = true) {
-              const float mc = m == kNegInf ? 0.f : m * a.scale_log2;
-              m2 = pair(-mc, -mc);
-              sum[0] = sum[1] = 0;   // (+0, +0)
-              weights(0);
-              if (again) break;
-              tc_landed(sr[2]);
-              tc_landed(sr[3]);
-              if (mask) hide(1);
-              const float row_top = fmaxf(max64(sr[0], sr[1]), max64(sr[2], sr[3]));
+            float row_top = max64(sr[0], sr[1]);
+            tc_landed(sr[2]);
+            tc_landed(sr[3]);
+            if (mask) hide(1);
+            row_top = fmaxf(row_top, max64(sr[2], sr[3]));
+            if (n_mine == 0) {
+              m = row_top;
+            } else {
               const bool grow = row_top > m && !((row_top - m) * a.scale_log2 <= kSlack);
-              if (!__any_sync(0xffffffffu, grow)) break;
-              const float f = grow ? ex2((m - row_top) * a.scale_log2) : 1.f;
-              if (grow) m = row_top;
-              l *= f;
-              if (n_mine > 0) {
+              if (__any_sync(0xffffffffu, grow)) {
+                const float f = grow ? ex2((m - row_top) * a.scale_log2) : 1.f;
+                if (grow) m = row_top;
+                l *= f;
                 // (the scores' commit covers the product before them, so O is at rest)
 #pragma unroll 1
                 for (int c = 0; c < HD / 16; ++c) {
@@ -568,15 +555,40 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
                 }
               }
             }
+            const float mc = m == kNegInf ? 0.f : m * a.scale_log2;
+            const uint64_t c2 = pair(a.scale_log2, a.scale_log2), m2 = pair(-mc, -mc);
+            uint64_t sum[2] = {0, 0};   // (+0, +0)
+            uint32_t pr[2][32];
+            auto weights = [&](int h, int j0, int j1) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (h == 1) weights(1);
-              tc_st32(t_s + 32 * h, pr);
-              tc_wait_st();
-              tc_fence_before();
-              mbar_arrive(&sh.p_full[st][h]);
-            }
-            if (kTurns && NQ == 2) bar_arrive(3 - st, 256);
+              for (int j = j0; j < j1; ++j) {
+                const int e = 64 * h + 2 * j;
+                float p, q;
+                unpair(fma2(pair(__uint_as_float(sr[e / 32][e % 32]), __uint_as_float(sr[e / 32][e % 32 + 1])), c2, m2),
+                       p, q);
+                p = ex2(p);
+                q = ex2(q);
+                sum[j & 1] = add2(sum[j & 1], pair(p, q));
+                pr[h][j] = Elem<T>::pack(p, q);
+              }
+            };
+            // The streams take turns at the exponentials: together they would
+            // share that unit first and the tensor core afterwards.  A turn is
+            // filled with them: the first half's weights leave while the
+            // second's are made.
+            if (NQ == 2) bar_sync(2 + st, 256);
+            weights(0, 0, 32);
+            tc_st32(t_s, pr[0]);
+            weights(1, 0, 12);
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sh.p_full[st][0]);
+            weights(1, 12, 32);
+            if (NQ == 2) bar_arrive(3 - st, 256);
+            tc_st32(t_s + 32, pr[1]);
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sh.p_full[st][1]);
             float s0, s1, s2, s3;
             unpair(sum[0], s0, s1);
             unpair(sum[1], s2, s3);
@@ -585,9 +597,6 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           ++n_s;
           ++n_mine;
         }
-
-        go = more();
-        if (go) next();
 
         // ---- the unit's end ------------------------------------------------------
         if (n_mine > 0) {
@@ -603,15 +612,14 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         if (NQ == 1 && st == 1) {
           if (two) {
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-              uint32_t ov[32];
-              tc_ld32(t_o + 32 * c, ov);
-              tc_landed(ov);
+            for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-              for (int j = 0; j < 32; j += 4)
-                *reinterpret_cast<uint4*>(half_sum + r * HD + 32 * c + j) =
-                    make_uint4(ov[j], ov[j + 1], ov[j + 2], ov[j + 3]);
-            }
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t ov[16];
+                tc_ld_rows(t_o + (16u << 16) * hh + 32 * c, ov);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) half_sum[((hh * (HD / 32) + c) * 16 + j) * 128 + r] = __uint_as_float(ov[j]);
+              }
             half_sum[128 * HD + r] = m;
             half_sum[128 * HD + 128 + r] = l;
           }
@@ -636,43 +644,71 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         const float w0 = f0 * inv, w1 = f1 * inv;
         char* dst = a.out + (cu.row0 + tok) * a.out_row + head * a.out_head;
         const int prow = blk * 128 + r;
-        bool odd = false;
+        // Rows leave through the load that spreads a row over four lanes (two
+        // columns of every eight each), so that a store covers whole 32-byte
+        // sectors of 8 rows instead of half ones of 32.
+        unsigned spoilt[2][2] = {};
         if (any_live) {
+          const unsigned live_rows = __ballot_sync(0xffffffffu, live);
+          const int g = lane / 4, t4 = lane % 4;
 #pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t ov[32];
-            tc_ld32(t_o + 32 * c, ov);
-            tc_landed(ov);
-            float o[32];
+          for (int hh = 0; hh < 2; ++hh) {
+            char* d[2];        // of rows 16 hh + g and 16 hh + g + 8
+            float s0[2], s1[2], zero[2] = {0.f, 0.f};
+            bool on[2];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(ov[j]) * w0;
-            if (two && live) {
+            for (int k = 0; k < 2; ++k) {
+              const int src = 16 * hh + g + 8 * k;
+              d[k] = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), src));
+              s0[k] = __shfl_sync(0xffffffffu, w0, src);
+              s1[k] = NQ == 1 ? __shfl_sync(0xffffffffu, w1, src) : 0.f;
+              on[k] = (live_rows >> src) & 1;
+              if (!whole) d[k] = reinterpret_cast<char*>(part + (prow - lane + src) * HD);
+            }
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 y = *reinterpret_cast<const float4*>(half_sum + r * HD + 32 * c + j);
-                o[j] = fmaf(y.x, w1, o[j]), o[j + 1] = fmaf(y.y, w1, o[j + 1]);
-                o[j + 2] = fmaf(y.z, w1, o[j + 2]), o[j + 3] = fmaf(y.w, w1, o[j + 3]);
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t ov[16];
+              tc_ld_rows(t_o + (16u << 16) * hh + 32 * c, ov);
+              float o[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                o[j] = __uint_as_float(ov[j]) * s0[(j >> 1) & 1];
+                if (two) o[j] = fmaf(half_sum[((hh * (HD / 32) + c) * 16 + j) * 128 + r], s1[(j >> 1) & 1], o[j]);
+                zero[(j >> 1) & 1] = fmaf(0.f, o[j], zero[(j >> 1) & 1]);   // NaN if any is NaN or infinite
+              }
+              if (whole) {
+#pragma unroll
+                for (int q = 0; q < 4; q += 2)     // columns 32 c + 8 q .. + 15 of both rows
+#pragma unroll
+                  for (int k = 0; k < 2; ++k) {
+                    const uint32_t x0 = Elem<T>::pack(o[4 * q + 2 * k], o[4 * q + 2 * k + 1]);
+                    const uint32_t x1 = Elem<T>::pack(o[4 * q + 4 + 2 * k], o[4 * q + 5 + 2 * k]);
+                    // four neighbouring columns a lane: lanes 0, 1 the first eight, 2, 3 the others
+                    const uint32_t y = __shfl_xor_sync(0xffffffffu, (t4 & 2) ? x0 : x1, 2);
+                    const uint32_t lo = (t4 & 2) ? y : x0, hi2 = (t4 & 2) ? x1 : y;
+                    const uint32_t z = __shfl_xor_sync(0xffffffffu, (t4 & 1) ? lo : hi2, 1);
+                    if (on[k])
+                      *reinterpret_cast<uint2*>(d[k] + (32 * c + 8 * q + 4 * t4) * 2) =
+                          (t4 & 1) ? make_uint2(z, hi2) : make_uint2(lo, z);
+                  }
+              } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                  for (int k = 0; k < 2; ++k)
+                    if (on[k])
+                      *reinterpret_cast<float2*>(d[k] + (32 * c + 8 * q + 2 * t4) * 4) =
+                          make_float2(o[4 * q + 2 * k], o[4 * q + 2 * k + 1]);
               }
             }
-            float zero = 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) zero = fmaf(0.f, o[j], zero);   // NaN if any is NaN or infinite
-            odd |= zero != 0.f;
-            if (!live) continue;
-            if (whole) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 8)
-                *reinterpret_cast<uint4*>(dst + (32 * c + j) * 2) =
-                    make_uint4(Elem<T>::pack(o[j], o[j + 1]), Elem<T>::pack(o[j + 2], o[j + 3]),
-                               Elem<T>::pack(o[j + 4], o[j + 5]), Elem<T>::pack(o[j + 6], o[j + 7]));
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; j += 4)
-                *reinterpret_cast<float4*>(part + prow * HD + 32 * c + j) =
-                    make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-            }
+            for (int k = 0; k < 2; ++k) spoilt[hh][k] = __ballot_sync(0xffffffffu, zero[k] != 0.f);
           }
         }
+        // four lanes speak for a row
+        const unsigned mine4 = (lane & 16) ? ((lane & 8) ? spoilt[1][1] : spoilt[1][0])
+                                           : ((lane & 8) ? spoilt[0][1] : spoilt[0][0]);
+        const bool odd = ((mine4 >> (4 * (lane & 7))) & 15u) != 0;
         tc_fence_before();
         if (live) {
           if (!whole) {

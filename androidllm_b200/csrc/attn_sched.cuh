@@ -16,7 +16,10 @@
 namespace alm {
 
 constexpr int kSchedThreads = 256;   // threads that run sched_init (warps 0 .. 7)
-constexpr int kUnitCost = 2;         // in tiles
+#ifndef UNITCOST
+#define UNITCOST 2
+#endif
+constexpr int kUnitCost = UNITCOST;         // in tiles
 
 struct Unit {
   int s, mb, h;       // sequence, token block, K/V head
