@@ -16,10 +16,7 @@
 namespace alm {
 
 constexpr int kSchedThreads = 256;   // threads that run sched_init (warps 0 .. 7)
-#ifndef UNITCOST
-#define UNITCOST 2
-#endif
-constexpr int kUnitCost = UNITCOST;         // in tiles
+constexpr int kUnitCost = 2;         // in tiles: measured 1 / 2 / 3 at 4 x 2047 prefill rows: 367 / 285 / 283 us
 
 struct Unit {
   int s, mb, h;       // sequence, token block, K/V head
