@@ -18,11 +18,14 @@
 // on the wk-th slice of each tile, with its own running statistics;
 // the WK slices are merged at a unit's end through the stage just consumed.
 #pragma once
+#include <algorithm>
+
 #include "attn_sched.cuh"
 
 namespace alm {
 
 constexpr int kPagedThreads = 256;
+constexpr int kJoinThreads = 128;
 constexpr int kPagedWarps = kPagedThreads / kWarp;
 
 template <typename T>
@@ -105,6 +108,15 @@ ALM_DEV float* partial_at(char* work, int rows, int cta, int which) {
   return reinterpret_cast<float*>(work) + (static_cast<size_t>(cta) * 2 + which) * rows * (HD + 2);
 }
 
+// What a CTA leaves for the join: the unit that it began and did not finish as
+// (number of partials, first packed row, tokens, K/V head); 0 partials: none.
+ALM_DEV int4* join_record(const AttnPaged& a, int cta) { return reinterpret_cast<int4*>(a.records) + cta; }
+ALM_DEV int4 record_of(const Unit& u, int cta, int n_cta, long long total) {
+  // the CTA of the unit's last place p: the largest i with total i / n <= p
+  const int last = static_cast<int>(((u.start + u.n_tile) * n_cta - 1) / total);
+  return make_int4(last - cta + 1, u.row0, u.n_tok, u.h);
+}
+
 // One row by one warp straight from the formula, skipping every position the
 // row does not see: for rows whose sums are not finite, since a hidden
 // position's infinity or NaN times a zero weight spoils a matrix product.
@@ -171,6 +183,7 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
       [] { __syncthreads(); });
   const long long total = sched.total;
   const int n_cta = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
+  if (tid == 0) *join_record(a, cta) = make_int4(0, 0, 0, 0);
   if (cta >= n_cta) return;
   const long long x0 = share(total, cta, n_cta), x1 = share(total, cta + 1, n_cta);
 
@@ -371,6 +384,7 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
     float* buf = reinterpret_cast<float*>(smem + stage * S::kStageBytes);
     const bool whole = t_first == 0 && tb == u.n_tile;
     float* part = partial_at<HD>(a.work, kRows, cta, t_first == 0 ? 1 : 0);
+    if (tid == 0 && !whole && t_first == 0) *join_record(a, cta) = record_of(u, cta, n_cta, total);
     constexpr int kCols = HD / S::kPasses;
     bool any_bad = false;
 #pragma unroll
@@ -454,76 +468,80 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
   if (bad_page) *err = 1;
 }
 
-// Joins the partial results of the unit that CTA blockIdx.x began and did not
-// finish: rows 8 blockIdx.y + warp.  Partials are added in CTA order.  A unit's
-// ROWS rows are blocks of BLK rows, whole tokens each.
-template <typename T, int HD, int TILE, int ROWS, int BLK>
-__global__ void __launch_bounds__(kPagedThreads)
-attn_paged_join_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ SeqBatch b,
-                       const __grid_constant__ PagedKV kv) {
-  __shared__ SchedShared sched;
-  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-  const int tq = BLK / a.group, tpu = ROWS / BLK * tq, cta = blockIdx.x;
-  long long x0 = 0, x1 = 0;
-  sched_init<TILE>(
-      b, kv, tpu, a.window, sched,
-      [&](long long total) {
-        const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
-        if (cta >= n) return -1ll;
-        x0 = share(total, cta, n);
-        x1 = share(total, cta + 1, n);
-        return x1 - 1;
-      },
-      [] { __syncthreads(); });
-  const long long total = sched.total;
-  const int n_cta = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
-  Unit u;
-  bool mine = cta < n_cta && x1 < total;
-  if (mine) {
-    u = unit_at<TILE>(b, kv, tpu, a.window, sched.found_seq, sched.found_at, x1 - 1);
-    mine = u.start >= x0 && u.start < x1 && u.start + u.n_tile > x1;
+// V consecutive fp32 values behind L1 (another SM wrote them).
+template <int V>
+ALM_DEV void load_row(const float* p, float (&v)[V]) {
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(p + i));
+      v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+    }
+  } else if constexpr (V == 2) {
+    const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
+    v[0] = x.x, v[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = __ldcg(p + i);
   }
-  grid_dep_wait();
-  if (!mine) return;
-  int last = cta + 1;   // the CTA that holds the unit's last tile
-  while (share(total, last + 1, n_cta) < u.start + u.n_tile) ++last;
-  const int row = blockIdx.y * kPagedWarps + warp;
-  const int tk = row % BLK / a.group, tok = row / BLK * tq + tk, head = u.h * a.group + row % BLK - tk * a.group;
-  if (tk >= tq || tok >= u.n_tok) return;
-  const int n = last - cta + 1;
+}
 
+// Joins the partial results of the unit that CTA blockIdx.x began and did not
+// finish, as its record says: a warp a row, partials added in CTA order.  A
+// unit's ROWS rows are blocks of BLK rows, whole tokens each.
+template <typename T, int HD, int ROWS, int BLK>
+__global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const __grid_constant__ AttnPaged a) {
+  constexpr int V = HD / 32, kWarps = kJoinThreads / kWarp;
+  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp, cta = blockIdx.x;
+  const int tq = BLK / a.group;
+  grid_dep_wait();
+  const int4 rec = __ldcg(join_record(a, cta));
+  const int n = rec.x, row0 = rec.y, n_tok = rec.z, kv_head = rec.w;
+  if (n == 0) return;
   auto part = [&](int i) { return partial_at<HD>(a.work, ROWS, cta + i, i == 0 ? 1 : 0); };
-  float m = kNegInf;
-  for (int i = lane; i < n; i += kWarp) m = fmaxf(m, __ldcg(part(i) + ROWS * HD + row));
-  m = warp_max(m);
-  const float base = m == kNegInf ? 0.f : m;
-  float l = 0.f, o[HD / 32];
+  for (int row = blockIdx.y * kWarps + warp; row < ROWS; row += gridDim.y * kWarps) {
+    const int tk = row % BLK / a.group, tok = row / BLK * tq + tk;
+    const int head = kv_head * a.group + row % BLK - tk * a.group;
+    if (tk >= tq || tok >= n_tok) continue;
+    float m = kNegInf;
+    for (int i = lane; i < n; i += kWarp) m = fmaxf(m, __ldcg(part(i) + ROWS * HD + row));
+    m = warp_max(m);
+    const float base = m == kNegInf ? 0.f : m;
+    float l = 0.f, o[V];
 #pragma unroll
-  for (int j = 0; j < HD / 32; ++j) o[j] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += kWarp) {
-    float w = 0.f, li = 0.f;
-    if (i0 + lane < n) {
-      const float* p = part(i0 + lane) + ROWS * HD;
-      w = ex2((__ldcg(p + row) - base) * a.scale_log2);
-      li = __ldcg(p + ROWS + row);
-    }
-    const int k = min(kWarp, n - i0);
+    for (int j = 0; j < V; ++j) o[j] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += kWarp) {
+      float w = 0.f, li = 0.f;
+      if (i0 + lane < n) {
+        const float* p = part(i0 + lane) + ROWS * HD;
+        w = ex2((__ldcg(p + row) - base) * a.scale_log2);
+        li = __ldcg(p + ROWS + row);
+      }
+      const int k = min(kWarp, n - i0);
 #pragma unroll 8
-    for (int i = 0; i < k; ++i) {
-      const float f = __shfl_sync(0xffffffffu, w, i);
-      l = fmaf(__shfl_sync(0xffffffffu, li, i), f, l);
-      const float* p = part(i0 + i) + row * HD;
+      for (int i = 0; i < k; ++i) {
+        const float f = __shfl_sync(0xffffffffu, w, i);
+        l = fmaf(__shfl_sync(0xffffffffu, li, i), f, l);
+        float v[V];
+        load_row<V>(part(i0 + i) + row * HD + lane * V, v);
 #pragma unroll
-      for (int j = 0; j < HD / 32; ++j) o[j] = fmaf(__ldcg(p + lane + 32 * j), f, o[j]);
+        for (int j = 0; j < V; ++j) o[j] = fmaf(v[j], f, o[j]);
+      }
     }
-  }
-  const float inv = m == kNegInf && l == 0.f ? 0.f : 1.f / l;
-  T* dst = reinterpret_cast<T*>(a.out + (u.row0 + tok) * a.out_row + head * a.out_head);
+    const float inv = m == kNegInf && l == 0.f ? 0.f : 1.f / l;
+    T* dst = reinterpret_cast<T*>(a.out + (row0 + tok) * a.out_row + head * a.out_head) + lane * V;
+    if constexpr (V % 2 == 0) {
 #pragma unroll
-  for (int j = 0; j < HD / 32; ++j) dst[lane + 32 * j] = Elem<T>::down(o[j] * inv);
-  if (a.lse && lane == 0)
-    a.lse[(u.row0 + tok) * a.lse_row + head] =
-        m == kNegInf ? kNegInf : (m * a.scale_log2 + log2f(l)) * 0.693147180559945309f;
+      for (int j = 0; j < V; j += 2)
+        reinterpret_cast<uint32_t*>(dst)[j / 2] = Elem<T>::pack(o[j] * inv, o[j + 1] * inv);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) dst[j] = Elem<T>::down(o[j] * inv);
+    }
+    if (a.lse && lane == 0)
+      a.lse[(row0 + tok) * a.lse_row + head] =
+          m == kNegInf ? kNegInf : (m * a.scale_log2 + log2f(l)) * 0.693147180559945309f;
+  }
 }
 
 template <typename T, int HD, int WM>
@@ -551,18 +569,19 @@ cudaError_t paged_attr_all() {
   return e;
 }
 
-template <typename T, int HD, int TILE, int ROWS, int BLK>
-cudaError_t launch_join(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, cudaStream_t st) {
+template <typename T, int HD, int ROWS, int BLK>
+cudaError_t launch_join(const AttnPaged& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.n_cta, ROWS / kPagedWarps, 1);
-  cfg.blockDim = dim3(kPagedThreads, 1, 1);
+  // 16 blocks an owner at most: all of them are resident at once
+  cfg.gridDim = dim3(a.n_cta, std::min(ROWS / (kJoinThreads / kWarp), 16), 1);
+  cfg.blockDim = dim3(kJoinThreads, 1, 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<T, HD, TILE, ROWS, BLK>, a, b, kv);
+  return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<T, HD, ROWS, BLK>, a);
 }
 
 template <typename T, int HD, int WM>
@@ -570,7 +589,7 @@ cudaError_t launch_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& k
   using S = PagedShape<HD, WM>;
   attn_paged_kernel<T, HD, WM><<<a.n_cta, kPagedThreads, S::kSmem, st>>>(a, b, kv, err);
   const cudaError_t e = cudaGetLastError();
-  return e != cudaSuccess ? e : launch_join<T, HD, S::kTile, S::kRows, S::kRows>(a, b, kv, st);
+  return e != cudaSuccess ? e : launch_join<T, HD, S::kRows, S::kRows>(a, st);
 }
 
 // The smallest row block that holds the longest sequence's rows: K and V are

@@ -246,6 +246,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
   const long long x0 = cta < n_cta ? share(total, cta, n_cta) : 0;
   const long long x1 = cta < n_cta ? share(total, cta + 1, n_cta) : 0;
 
+  if (tid == 0) *join_record(a, cta) = make_int4(0, 0, 0, 0);
   volatile int* dead = &sh.dead;
   // Waits are bounded: one that runs out marks the CTA dead, and every role leaves.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -605,6 +606,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         }
         const bool whole = ca == 0 && cb == cu.n_tile;
         float* part = partial_at<HD>(a.work, NQ * 128, cta, ca == 0 ? 1 : 0);
+        if (tid == 0 && !whole && ca == 0) *join_record(a, cta) = record_of(cu, cta, n_cta, total);
         // stream 1 of a single block leaves its sums in global memory for
         // stream 0, in two places in turn: one is read while the next is written
         float* half_sum = NQ == 1 ? partial_at<HD>(a.work, 128, a.n_cta + cta, n_u++ & 1) : nullptr;
@@ -825,7 +827,7 @@ cudaError_t launch_tc(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, 
     return cudaErrorInvalidValue;
   attn_paged_tc_kernel<T, HD, NQ><<<a.n_cta, kTcPagedThreads, S::kSmem, st>>>(km, vm, qm, a, b, kv, box, err);
   const cudaError_t e = cudaGetLastError();
-  return e != cudaSuccess ? e : launch_join<T, HD, S::kTile, NQ * 128, 128>(a, b, kv, st);
+  return e != cudaSuccess ? e : launch_join<T, HD, NQ * 128, 128>(a, st);
 }
 
 template <typename T>

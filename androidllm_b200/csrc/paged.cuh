@@ -79,7 +79,8 @@ struct AttnPaged {
   int64_t lse_row;             // elements
   int heads, group, window;
   float scale_log2;            // scale * log2(e)
-  char* work;
+  char* work;                  // partial results
+  void* records;               // 16 bytes a CTA
   int n_cta;                   // CTAs that share the tiles
 };
 
@@ -104,6 +105,7 @@ struct Verify {
 cudaError_t launch_rope_append(const RopeAppend& a, const SeqBatch& b, const PagedKV& kv, int dtype, int rope_dtype,
                                bool interleaved, int* err, cudaStream_t st);
 cudaError_t launch_verify(const Verify& a, int dtype, cudaStream_t st);
+size_t attn_paged_part_bytes(int n_sms, int head_dim);
 size_t attn_paged_work_bytes(int n_sms, int head_dim);
 cudaError_t paged_init_attrs();
 

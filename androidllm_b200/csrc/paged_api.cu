@@ -40,9 +40,12 @@ cudaError_t paged_init_attrs() {
 // head) take the tcgen05 kernel.
 constexpr long long kTcMinRows = 32;
 
-// Two partial results a CTA, of the largest row block.
-size_t attn_paged_work_bytes(int n_sms, int head_dim) {
+// Two partial results a CTA, of the largest row block; a record a CTA.
+size_t attn_paged_part_bytes(int n_sms, int head_dim) {
   return static_cast<size_t>(n_sms) * 2 * 256 * (head_dim + 2) * sizeof(float);
+}
+size_t attn_paged_work_bytes(int n_sms, int head_dim) {
+  return attn_paged_part_bytes(n_sms, head_dim) + static_cast<size_t>(n_sms) * 16;
 }
 }  // namespace alm
 
@@ -219,6 +222,7 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   a.window = v->window;
   a.scale_log2 = v->scale * 1.4426950408889634f;
   a.work = static_cast<char*>(v->work_dev);
+  a.records = a.work + attn_paged_part_bytes(n_sms, kv.head_dim);
   a.n_cta = n_sms;
   OnDevice on(device);
   const long long rows = static_cast<long long>(b.max_rows) * a.group;
