@@ -169,6 +169,7 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
   __shared__ float row_m[kRows], row_l[kRows];
   __shared__ int row_bad[kRows];
 
+  grid_dep_wait();
   grid_dep_launch();
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
   const int wm = warp % WM, wk = warp / WM, g = lane / 4, t4 = lane % 4;
@@ -571,24 +572,16 @@ cudaError_t paged_attr_all() {
 
 template <typename T, int HD, int ROWS, int BLK>
 cudaError_t launch_join(const AttnPaged& a, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
   // 16 blocks an owner at most: all of them are resident at once
-  cfg.gridDim = dim3(a.n_cta, std::min(ROWS / (kJoinThreads / kWarp), 16), 1);
-  cfg.blockDim = dim3(kJoinThreads, 1, 1);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<T, HD, ROWS, BLK>, a);
+  OpLaunch l(dim3(a.n_cta, std::min(ROWS / (kJoinThreads / kWarp), 16), 1), kJoinThreads, 0, st);
+  return cudaLaunchKernelEx(&l.cfg, attn_paged_join_kernel<T, HD, ROWS, BLK>, a);
 }
 
 template <typename T, int HD, int WM>
 cudaError_t launch_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st) {
   using S = PagedShape<HD, WM>;
-  attn_paged_kernel<T, HD, WM><<<a.n_cta, kPagedThreads, S::kSmem, st>>>(a, b, kv, err);
-  const cudaError_t e = cudaGetLastError();
+  OpLaunch l(dim3(a.n_cta, 1, 1), kPagedThreads, S::kSmem, st);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, attn_paged_kernel<T, HD, WM>, a, b, kv, err);
   return e != cudaSuccess ? e : launch_join<T, HD, S::kRows, S::kRows>(a, st);
 }
 

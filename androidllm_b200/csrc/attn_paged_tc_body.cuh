@@ -212,7 +212,6 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
   const int tq = 128 / a.group;      // tokens a 128-row block
   const int tpu = NQ * tq;
 
-  grid_dep_launch();
   if (warp == 8) {
     if (lane == 0) {
       for (int i = 0; i < S::kSlots; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], NQ);
@@ -228,7 +227,10 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     }
     __syncwarp();
     tc_alloc(&sh.tmem, S::kTmemCols);
-  } else if (warp < 8) {
+  }
+  grid_dep_wait();
+  grid_dep_launch();
+  if (warp < 8) {
     sched_init<S::kTile>(
         b, kv, tpu, a.window, sh.sched,
         [&](long long total) {
@@ -825,8 +827,8 @@ cudaError_t launch_tc(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, 
   if (!encode_pages<T>(&km, kv.k, kv, box) || !encode_pages<T>(&vm, kv.v, kv, box) ||
       !encode_q<T>(&qm, a, b, HD))
     return cudaErrorInvalidValue;
-  attn_paged_tc_kernel<T, HD, NQ><<<a.n_cta, kTcPagedThreads, S::kSmem, st>>>(km, vm, qm, a, b, kv, box, err);
-  const cudaError_t e = cudaGetLastError();
+  OpLaunch l(dim3(a.n_cta, 1, 1), kTcPagedThreads, S::kSmem, st);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, attn_paged_tc_kernel<T, HD, NQ>, km, vm, qm, a, b, kv, box, err);
   return e != cudaSuccess ? e : launch_join<T, HD, NQ * 128, 128>(a, st);
 }
 

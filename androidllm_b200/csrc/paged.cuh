@@ -58,6 +58,31 @@ ALM_DEV size_t kv_offset(const PagedKV& kv, int page, int head, int in_page) {
   return ((static_cast<size_t>(page) * kv.kv_heads + head) * kv.page_size + in_page) * kv.head_dim;
 }
 
+// Launch of an operator: its grid may be set up while the stream's last kernel
+// ends (programmatic dependent launch); every kernel here calls
+// grid_dep_wait() before it reads anything.
+struct OpLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  OpLaunch(dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster = 0) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cluster > 0) {
+      attr[1].id = cudaLaunchAttributeClusterDimension;
+      attr[1].val.clusterDim.x = cluster;
+      attr[1].val.clusterDim.y = 1;
+      attr[1].val.clusterDim.z = 1;
+      cfg.numAttrs = 2;
+    }
+  }
+};
+
 struct RopeAppend {
   const char *q, *k, *v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // bytes

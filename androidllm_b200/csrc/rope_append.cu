@@ -87,6 +87,8 @@ ALM_DEV int seq_of_row(const SeqBatch& b, int r) {
 // One block a row.  HL: lanes that share a head (a power of two >= head_dim / 16).
 template <typename T, typename R, bool INTER, int HL>
 __global__ void __launch_bounds__(1024) rope_append_kernel(const RopeAppend a, const SeqBatch b, const PagedKV kv, int* err) {
+  grid_dep_wait();
+  grid_dep_launch();
   const int r = blockIdx.x;
   const int d = kv.head_dim, per_head = d / 16;
   const int n_heads = a.heads + 2 * kv.kv_heads;
@@ -200,13 +202,13 @@ cudaError_t launch_hl(const RopeAppend& a, const SeqBatch& b, const PagedKV& kv,
   const int hl = lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
   const int items = ((a.heads + 2 * kv.kv_heads) * hl + kWarp - 1) / kWarp * kWarp;
   const int threads = items < 1024 ? items : 1024;
+  OpLaunch l(dim3(b.n_rows, 1, 1), threads, 0, st);
   switch (hl) {
-    case 2: rope_append_kernel<T, R, INTER, 2><<<b.n_rows, threads, 0, st>>>(a, b, kv, err); break;
-    case 4: rope_append_kernel<T, R, INTER, 4><<<b.n_rows, threads, 0, st>>>(a, b, kv, err); break;
-    case 8: rope_append_kernel<T, R, INTER, 8><<<b.n_rows, threads, 0, st>>>(a, b, kv, err); break;
-    default: rope_append_kernel<T, R, INTER, 16><<<b.n_rows, threads, 0, st>>>(a, b, kv, err); break;
+    case 2: return cudaLaunchKernelEx(&l.cfg, rope_append_kernel<T, R, INTER, 2>, a, b, kv, err);
+    case 4: return cudaLaunchKernelEx(&l.cfg, rope_append_kernel<T, R, INTER, 4>, a, b, kv, err);
+    case 8: return cudaLaunchKernelEx(&l.cfg, rope_append_kernel<T, R, INTER, 8>, a, b, kv, err);
+    default: return cudaLaunchKernelEx(&l.cfg, rope_append_kernel<T, R, INTER, 16>, a, b, kv, err);
   }
-  return cudaGetLastError();
 }
 
 template <typename T>

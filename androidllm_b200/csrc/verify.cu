@@ -139,6 +139,8 @@ template <typename T>
 __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) {
   cg::cluster_group cl = cg::this_cluster();
   __shared__ VerShared sh;
+  grid_dep_wait();
+  grid_dep_launch();
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
   const int n_cta = static_cast<int>(cl.num_blocks()), cta = static_cast<int>(cl.block_rank());
   const int s = blockIdx.x / n_cta;
@@ -485,18 +487,8 @@ cudaError_t launch_t(const Verify& a, cudaStream_t st) {
   // few sequences: 16 CTAs each, so that a row's slices stay short; many: 8
   // (the portable size, which more GPCs can place)
   const int ctas = a.n_seq <= 8 ? 16 : 8;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.n_seq * ctas, 1, 1);
-  cfg.blockDim = dim3(kVerThreads, 1, 1);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, verify_kernel<T>, a);
+  OpLaunch l(dim3(a.n_seq * ctas, 1, 1), kVerThreads, 0, st, ctas);
+  return cudaLaunchKernelEx(&l.cfg, verify_kernel<T>, a);
 }
 
 }  // namespace

@@ -13,10 +13,11 @@ is replayed.  What the device finds out of range is reported by the next
 ``Context.sync()``.
 """
 import ctypes
+import struct
 
 import numpy as np
 
-from ._lib import AttnPagedArgs, PagedKVView, RopeAppendArgs, SeqBatchView, VerifyArgs, check, lib
+from ._lib import PagedKVView, SeqBatchView, check, lib
 from .ops import DeviceBuffer
 
 F16, BF16, F32 = 0, 1, 2          # ALM_F16, ALM_BF16, ALM_F32
@@ -119,16 +120,50 @@ def _contiguous(a, what, codes, ndim, device=None):
     return p, code, shape
 
 
-def _rows(a, what, code, n_rows, heads, dim, device):
+def _flat(a, what, code, shape, device):
+    """Pointer of a contiguous array of this type and shape.  (The first lines
+    are the common case, a tensor that is all of that: these calls are made
+    for every layer, and a launch takes a few microseconds.)"""
+    try:
+        if a.shape == shape and _CODES.get(a.dtype) == code and a.get_device() == device and a.is_contiguous():
+            return a.data_ptr()
+    except AttributeError:
+        pass
+    p, _, got, stride = _array(a, what, (code,), len(shape), device)
+    if tuple(got) != shape:
+        raise ValueError(f"{what} must be {shape}, not {tuple(got)}")
+    if not _dense(shape, stride):
+        raise ValueError(f"{what} must be contiguous")
+    return p
+
+
+def _rows(a, what, code, shape, device):
     """(pointer, row stride, head stride) of a (rows, heads, dim) array."""
-    p, _, shape, stride = _array(a, what, (code,), 3, device)
-    if shape[0] != n_rows or shape[2] != dim or (heads is not None and shape[1] != heads):
-        want = f"({n_rows}, {'heads' if heads is None else heads}, {dim})"
-        raise ValueError(f"{what} must be {want}, not {tuple(shape)}")
-    if stride[2] != 1 and dim > 1:
+    try:
+        if a.shape == shape and _CODES.get(a.dtype) == code and a.get_device() == device:
+            stride = a.stride()
+            if stride[2] == 1 and shape[0] > 1 and shape[1] > 1:
+                return a.data_ptr(), stride[0], stride[1]
+    except AttributeError:
+        pass
+    p, _, got, stride = _array(a, what, (code,), 3, device)
+    if tuple(got) != shape:
+        raise ValueError(f"{what} must be {shape}, not {tuple(got)}")
+    if stride[2] != 1 and shape[2] > 1:
         raise ValueError(f"{what} must be contiguous in its last dimension")
     # a stride nothing is stepped with may be any number
-    return p, stride[0] if n_rows > 1 else 0, stride[1] if shape[1] > 1 else 0
+    return p, stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
+
+
+def _on(ctx, *views):
+    for v in views:
+        if v.device is not None and v.device != ctx.device:
+            raise ValueError(f"the {type(v).__name__} is on device {v.device}, the context on device {ctx.device}")
+
+
+def _device_of(a):
+    dev = getattr(a, "device", None)
+    return getattr(dev, "index", None)
 
 
 class PagedKV:
@@ -144,6 +179,7 @@ class PagedKV:
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = (int(n) for n in shape)
         self.c = PagedKVView(kp, vp, code, self.n_pages, self.page_size, self.kv_heads, self.head_dim)
         self.ref = ctypes.addressof(self.c)
+        self.device = _device_of(k) if device is None else device
         self._keep = (k, v)
 
     @classmethod
@@ -154,6 +190,7 @@ class PagedKV:
         self.page_size, self.head_dim = view.page_size, view.head_dim
         self.c, self._keep = view, keep
         self.ref = ctypes.addressof(view)
+        self.device = keep.model.ctx.device
         return self
 
 
@@ -205,6 +242,7 @@ class SeqBatch:
         most = self.n_rows if max_rows is None else int(max_rows)
         self.c = SeqBatchView(n_seq, self.n_rows, most, rows, pages, step, rp, lp, tp, sp)
         self.ref = ctypes.addressof(self.c)
+        self.device = _device_of(row_start) if device is None else device
         self._keep = (row_start, kv_len, page_table, slots)
 
 
@@ -217,7 +255,23 @@ class AttnWorkspace:
         n = ctypes.c_size_t()
         check(lib.alm_attn_paged_work(ctx.h, int(heads), int(kv_heads), int(head_dim), ctypes.byref(n)))
         self.buf = DeviceBuffer(ctx, n.value)
-        self.pointer, self.nbytes = self.buf.h.value, n.value
+        self.pointer, self.nbytes, self.device = self.buf.h.value, n.value, ctx.device
+
+
+# The argument structs of the header, packed at once (native alignment).
+_ROPE_ARGS = struct.Struct("@PPPqqqqqqPqqiPPfPiiii").pack
+_ATTN_ARGS = struct.Struct("@PqqPqqPqiifPN").pack
+_VERIFY_ARGS = struct.Struct("@iiiiPPiqPPqqPPPPPP").pack
+
+
+def _heads_of(q, what, n_rows, dim):
+    """(n_rows, heads, dim) with q's own number of heads."""
+    shape = getattr(q, "shape", None)
+    if shape is None:
+        shape = _array(q, what, (F16, BF16), 3)[2]
+    if len(shape) != 3:
+        raise ValueError(f"{what} must have 3 dimensions")
+    return n_rows, int(shape[1]), dim
 
 
 def rope_append(ctx, kv, seqs, q, k, v, rope, q_out, q_norm=None, k_norm=None, eps=1e-6, interleaved=False):
@@ -227,22 +281,21 @@ def rope_append(ctx, kv, seqs, q, k, v, rope, q_out, q_norm=None, k_norm=None, e
     strides that are multiples of 8; q_out may be q.  rope (positions,
     rot_dim): [cos | sin], fp16, bf16 or fp32; interleaved rotates neighbours
     (2i, 2i + 1) instead of halves (i, i + rot_dim / 2)."""
-    dev, n, d, code = ctx.device, seqs.n_rows, kv.head_dim, kv.code
-    qp, qr, qh = _rows(q, "q", code, n, None, d, dev)
-    kp, kr, kh = _rows(k, "k", code, n, kv.kv_heads, d, dev)
-    vp, vr, vh = _rows(v, "v", code, n, kv.kv_heads, d, dev)
-    heads = int(q.shape[1])
-    op, o_r, oh = _rows(q_out, "q_out", code, n, heads, d, dev)
+    dev, n, d, code, hk = ctx.device, seqs.n_rows, kv.head_dim, kv.code, kv.kv_heads
+    if kv.device != dev or seqs.device != dev:
+        _on(ctx, kv, seqs)
+    shape = _heads_of(q, "q", n, d)
+    qp, qr, qh = _rows(q, "q", code, shape, dev)
+    op, o_r, oh = _rows(q_out, "q_out", code, shape, dev)
+    heads, shape = shape[1], (n, hk, d)
+    kp, kr, kh = _rows(k, "k", code, shape, dev)
+    vp, vr, vh = _rows(v, "v", code, shape, dev)
     rp, rcode, rs = _contiguous(rope, "rope", (F16, BF16, F32), 2, dev)
-    np_ = [None, None]
-    for i, (w, what) in enumerate(((q_norm, "q_norm"), (k_norm, "k_norm"))):
-        if w is not None:
-            np_[i], _, ws = _contiguous(w, what, (code,), 1, dev)
-            if ws[0] != d:
-                raise ValueError(f"{what} must have head_dim entries")
-    a = RopeAppendArgs(qp, kp, vp, qr, qh, kr, kh, vr, vh, op, o_r, oh, heads, np_[0], np_[1], eps, rp, rcode,
-                       rs[0], rs[1], 1 if interleaved else 0)
-    check(lib.alm_rope_append(ctx.h, kv.ref, seqs.ref, ctypes.addressof(a)))
+    qw = _flat(q_norm, "q_norm", code, (d,), dev) if q_norm is not None else 0
+    kw = _flat(k_norm, "k_norm", code, (d,), dev) if k_norm is not None else 0
+    check(lib.alm_rope_append(ctx.h, kv.ref, seqs.ref, _ROPE_ARGS(
+        qp, kp, vp, qr, qh, kr, kh, vr, vh, op, o_r, oh, heads, qw, kw, eps, rp, rcode, rs[0], rs[1],
+        1 if interleaved else 0)))
 
 
 def attn_paged(ctx, kv, seqs, q, out, work, scale=None, window=0, lse=None):
@@ -252,18 +305,20 @@ def attn_paged(ctx, kv, seqs, q, out, work, scale=None, window=0, lse=None):
     to head_dim ** -0.5; lse (n_rows, heads) fp32 receives the log of the sum
     of exponentials.  Rows that see nothing get zeros and -inf."""
     dev, n, d, code = ctx.device, seqs.n_rows, kv.head_dim, kv.code
-    qp, qr, qh = _rows(q, "q", code, n, None, d, dev)
-    heads = int(q.shape[1])
-    op, o_r, oh = _rows(out, "out", code, n, heads, d, dev)
-    lp, ls = None, 0
+    if kv.device != dev or seqs.device != dev or work.device != dev:
+        _on(ctx, kv, seqs, work)
+    shape = _heads_of(q, "q", n, d)
+    qp, qr, qh = _rows(q, "q", code, shape, dev)
+    op, o_r, oh = _rows(out, "out", code, shape, dev)
+    lp, ls = 0, 0
     if lse is not None:
-        lp, _, shape, stride = _array(lse, "lse", (F32,), 2, dev)
-        if shape[0] != n or shape[1] != heads or (heads > 1 and stride[1] != 1):
+        lp, _, got, stride = _array(lse, "lse", (F32,), 2, dev)
+        if tuple(got) != shape[:2] or (shape[1] > 1 and stride[1] != 1):
             raise ValueError("lse must be (n_rows, heads), contiguous in its last dimension")
         ls = stride[0]
-    a = AttnPagedArgs(qp, qr, qh, op, o_r, oh, lp, ls, heads, window, d ** -0.5 if scale is None else scale,
-                      work.pointer, work.nbytes)
-    check(lib.alm_attn_paged(ctx.h, kv.ref, seqs.ref, ctypes.addressof(a)))
+    check(lib.alm_attn_paged(ctx.h, kv.ref, seqs.ref, _ATTN_ARGS(
+        qp, qr, qh, op, o_r, oh, lp, ls, shape[1], window, d ** -0.5 if scale is None else scale, work.pointer,
+        work.nbytes)))
 
 
 def verify(ctx, row_start, logits, draft_tokens, draft_probs, uniforms, temperature, tokens, n_accepted,
@@ -284,32 +339,19 @@ def verify(ctx, row_start, logits, draft_tokens, draft_probs, uniforms, temperat
         raise ValueError("logits must be contiguous in the last dimension")
     dp, _, ds = _contiguous(draft_tokens, "draft_tokens", (I32,), 2, dev)
     n_seq, k = ds
-    rp, _, rs = _contiguous(row_start, "row_start", (I32,), 1, dev)
-    if rs[0] != n_seq + 1:
-        raise ValueError("row_start must have n_seq + 1 entries")
-    qp, q_seq, q_step = None, 0, 0
+    rp = _flat(row_start, "row_start", I32, (n_seq + 1,), dev)
+    qp, q_seq, q_step = 0, 0, 0
     if draft_probs is not None:
         qp, _, qs, qst = _array(draft_probs, "draft_probs", (F32,), 3, dev)
         if tuple(qs) != (n_seq, k, vocab) or (vocab > 1 and qst[2] != 1):
             raise ValueError("draft_probs must be (n_seq, k_max, vocab), contiguous in its last dimension")
         q_seq, q_step = qst[0], qst[1]
-    up, _, us = _contiguous(uniforms, "uniforms", (F64,), 2, dev)
-    op, _, os_ = _contiguous(tokens, "tokens", (I32,), 2, dev)
-    if tuple(us) != (n_seq, k + 1) or tuple(os_) != (n_seq, k + 1):
-        raise ValueError("uniforms and tokens must be (n_seq, k_max + 1)")
-    tp, _, ts = _contiguous(temperature, "temperature", (F32,), 1, dev)
-    ap, _, as_ = _contiguous(n_accepted, "n_accepted", (I32,), 1, dev)
-    mp = pp = None
-    if min_p is not None:
-        mp, _, ms = _contiguous(min_p, "min_p", (F32,), 1, dev)
-        if ms[0] != n_seq:
-            raise ValueError("min_p must have n_seq entries")
-    if ts[0] != n_seq or as_[0] != n_seq:
-        raise ValueError("temperature and n_accepted must have n_seq entries")
-    if p_draft is not None:
-        pp, _, ps = _contiguous(p_draft, "p_draft", (F32,), 2, dev)
-        if tuple(ps) != (n_seq, k):
-            raise ValueError("p_draft must be (n_seq, k_max)")
-    a = VerifyArgs(n_seq, n_rows, k, vocab, rp, lp, lcode, lstride[0] if n_rows > 1 else vocab, dp, qp, q_seq, q_step,
-                   up, tp, mp, op, ap, pp)
-    check(lib.alm_verify(ctx.h, ctypes.addressof(a)))
+    up = _flat(uniforms, "uniforms", F64, (n_seq, k + 1), dev)
+    op = _flat(tokens, "tokens", I32, (n_seq, k + 1), dev)
+    tp = _flat(temperature, "temperature", F32, (n_seq,), dev)
+    ap = _flat(n_accepted, "n_accepted", I32, (n_seq,), dev)
+    mp = _flat(min_p, "min_p", F32, (n_seq,), dev) if min_p is not None else 0
+    pp = _flat(p_draft, "p_draft", F32, (n_seq, k), dev) if p_draft is not None else 0
+    check(lib.alm_verify(ctx.h, _VERIFY_ARGS(
+        n_seq, n_rows, k, vocab, rp, lp, lcode, lstride[0] if n_rows > 1 else vocab, dp, qp, q_seq, q_step, up, tp, mp,
+        op, ap, pp)))

@@ -201,7 +201,7 @@ def test_python_append_refuses(kw, err):
     (dict(lse=Fake((5, 4))), TypeError), (dict(out=Fake((5, 4, 64), "float32")), TypeError)])
 def test_python_attention_refuses(kw, err):
     class Work:
-        pointer, nbytes = P, 1 << 30
+        pointer, nbytes, device = P, 1 << 30, None
     a = dict(q=Fake((5, 4, 64)), out=Fake((5, 4, 64)), work=Work)
     a.update(kw)
     with pytest.raises(err):
