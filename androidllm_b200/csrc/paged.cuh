@@ -58,6 +58,29 @@ ALM_DEV size_t kv_offset(const PagedKV& kv, int page, int head, int in_page) {
   return ((static_cast<size_t>(page) * kv.kv_heads + head) * kv.page_size + in_page) * kv.head_dim;
 }
 
+// Pairs of fp32 in one 64-bit register: one instruction for both.
+ALM_DEV uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+ALM_DEV void unpair(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r)); }
+ALM_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+ALM_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+ALM_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Launch of an operator: its grid may be set up while the stream's last kernel
 // ends (programmatic dependent launch); every kernel here calls
 // grid_dep_wait() before it reads anything.
@@ -128,7 +151,7 @@ struct Verify {
 
 // dtype: ALM_F16 / ALM_BF16 / ALM_F32
 cudaError_t launch_rope_append(const RopeAppend& a, const SeqBatch& b, const PagedKV& kv, int dtype, int rope_dtype,
-                               bool interleaved, int* err, cudaStream_t st);
+                               bool interleaved, int n_sms, int* err, cudaStream_t st);
 cudaError_t launch_verify(const Verify& a, int dtype, cudaStream_t st);
 size_t attn_paged_part_bytes(int n_sms, int head_dim);
 size_t attn_paged_work_bytes(int n_sms, int head_dim);

@@ -174,7 +174,7 @@ ALM_API int alm_rope_append(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq
   a.rope_rows = v->rope_rows;
   a.rot = v->rot_dim;
   OnDevice on(device);
-  return cuda_status(launch_rope_append(a, b, kv, kv_->dtype, v->rope_dtype, v->interleaved != 0, err, st),
+  return cuda_status(launch_rope_append(a, b, kv, kv_->dtype, v->rope_dtype, v->interleaved != 0, n_sms, err, st),
                      "rope_append");
 }
 
