@@ -20,6 +20,8 @@
 // a draw is found by one scan over the warps' sums and one over a warp's lanes.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "../../include/androidllm_b200.h"
 #include "paged.cuh"
 
@@ -34,21 +36,6 @@ constexpr int kVerRows = 32;        // k_max + 1 at most
 constexpr int kVerBlock = 8 * kWarp;   // entries a warp takes at a time
 constexpr double kNear = 1e-4;
 
-template <typename T>
-struct Logit;
-template <>
-struct Logit<half> {
-  ALM_DEV static float up(half v) { return __half2float(v); }
-};
-template <>
-struct Logit<__nv_bfloat16> {
-  ALM_DEV static float up(__nv_bfloat16 v) { return __bfloat162float(v); }
-};
-template <>
-struct Logit<float> {
-  ALM_DEV static float up(float v) { return v; }
-};
-
 struct VerShared {
   double table[64];     // 2^(i / 64)
   float wm[kVerRows][kVerWarps];
@@ -62,10 +49,8 @@ struct VerShared {
   float row_m[kVerRows];
   double row_z[kVerRows];
   int row_i[kVerRows];
-  int near_min;         // an entry next to the min-p border
   double dsum[kVerWarps];
   double cta_d[2];      // two slots in turn: one is read while the next is written
-  int cta_near[2];
   double cta_r[2][kVerWarps];   // the residual's sums by warp, in index order (by attempt)
   int cta_last[2];              // last index with a positive residual, or -1
 };
@@ -83,12 +68,10 @@ ALM_DEV float ex2f_(float x) {
 // (Tang's table-driven method).  12 instructions of the 64-bit pipe, about a
 // third of the library function's.  NaN counts as -inf, +inf logits (l == top)
 // share the mass; below 2^-1000 the result is 0.
-ALM_DEV double weight64(float l, float top, double c, const double* table) {
+ALM_DEV double exp64(double t, const double* table) {   // 2^(t / 64)
   constexpr double kMagic = 6755399441055744.0;   // 1.5 * 2^52: adding it rounds to a whole number
   constexpr double a1 = 0.693147180559945309417 / 64, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3, a4 = a3 * a1 / 4,
                    a5 = a4 * a1 / 5;
-  if (l == top) return l > kNegInf ? 1.0 : 0.0;
-  const double t = (static_cast<double>(l) - static_cast<double>(top)) * c;
   if (!(t > -64000.0)) return 0.0;
   const double r = t + kMagic;
   const int n = __double2loint(r);
@@ -101,26 +84,105 @@ ALM_DEV double weight64(float l, float top, double c, const double* table) {
   const double e = p * table[n & 63];
   return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
 }
+ALM_DEV double weight64(float l, float top, double c, const double* table) {
+  if (l == top) return l > kNegInf ? 1.0 : 0.0;
+  return exp64((static_cast<double>(l) - static_cast<double>(top)) * c, table);
+}
 
-// Entries j .. j + 7 of a row; -inf behind the slice's end.
+// 16-bit logits have few leading parts: l = h + r with h the value without its
+// low bits and r what they add, so exp((l - top) / T) = exp((h - top) / T)
+// exp(r / T), two table entries and one product in 64 bits instead of the 25
+// instructions above.  h has one entry per sign, exponent and leading
+// mantissa bits, r one per sign, exponent and low bits.
 template <typename T>
-ALM_DEV void load8(const T* l, int j, int end, bool vec, float (&v)[8]) {
+struct Split {   // fp32: no tables
+  static constexpr int kHi = 0, kLo = 0;
+  ALM_DEV static int hi(uint32_t) { return 0; }
+  ALM_DEV static int lo(uint32_t) { return 0; }
+  ALM_DEV static void parts(int, float&, bool&) {}
+  ALM_DEV static double rest(int) { return 0.0; }
+};
+template <>
+struct Split<half> {   // 5 + 5 bits of the mantissa
+  static constexpr int kHi = 2048, kLo = 2048;
+  ALM_DEV static int hi(uint32_t b) { return b >> 5; }
+  ALM_DEV static int lo(uint32_t b) { return (b >> 10) << 5 | (b & 31); }
+  ALM_DEV static float value(uint32_t b) { return __half2float(__ushort_as_half(static_cast<unsigned short>(b))); }
+  ALM_DEV static void parts(int i, float& v, bool& finite) {
+    v = value(i << 5);
+    finite = (i >> 5 & 31) != 31;
+  }
+  ALM_DEV static double rest(int i) {
+    const uint32_t se = i >> 5;
+    if ((se & 31) == 31) return 0.0;
+    return static_cast<double>(value(se << 10 | (i & 31))) - static_cast<double>(value(se << 10));
+  }
+};
+template <>
+struct Split<__nv_bfloat16> {   // 3 + 4 bits of the mantissa; r for exponents 2^-63 .. 2^32
+  static constexpr int kHi = 4096, kLo = 2 * 96 * 16;
+  ALM_DEV static int hi(uint32_t b) { return b >> 4; }
+  ALM_DEV static int lo(uint32_t b) {
+    const int e = min(max(static_cast<int>(b >> 7 & 255) - 64, 0), 95);
+    return ((b >> 15) * 96 + e) << 4 | (b & 15);
+  }
+  ALM_DEV static float value(uint32_t b) { return __uint_as_float(b << 16); }
+  ALM_DEV static void parts(int i, float& v, bool& finite) {
+    v = value(i << 4);
+    finite = (i >> 3 & 255) != 255;
+  }
+  ALM_DEV static double rest(int i) {
+    const int se = i >> 4, sign = se / 96;
+    const uint32_t base = static_cast<uint32_t>(sign << 15 | (se % 96 + 64) << 7);
+    return static_cast<double>(value(base | (i & 15))) - static_cast<double>(value(base));
+  }
+};
+// Where the tables hold: both factors far from overflow, and no low bits
+// that matter outside the exponents above.  (Weights below e^-630 of the
+// largest may count as zero.)
+ALM_DEV bool tables_hold(float top, float temp) {
+  return fabsf(top) <= 2000.f * temp && temp >= 2.5e-4f && temp <= 1e4f;
+}
+
+// The bits of entries j .. j + 7 of a row; those of -inf behind the slice's end.
+template <typename T>
+ALM_DEV void load8(const T* l, int j, int end, bool vec, uint32_t (&v)[8]) {
+  constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, half>::value ? 0xfc00u : 0xff80u;
   if (vec && j + 8 <= end) {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(l + j));
     if constexpr (sizeof(T) == 4) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(l + j)), y = __ldg(reinterpret_cast<const float4*>(l + j) + 1);
+      const uint4 y = __ldg(reinterpret_cast<const uint4*>(l + j) + 1);
       v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
     } else {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(l + j));
-      const T* e = reinterpret_cast<const T*>(&x);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = Logit<T>::up(e[i]);
+      for (int i = 0; i < 4; ++i) v[2 * i] = w[i] & 0xffffu, v[2 * i + 1] = w[i] >> 16;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = j + i < end ? Logit<T>::up(l[j + i]) : kNegInf;
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 4) v[i] = j + i < end ? __ldg(reinterpret_cast<const unsigned*>(l) + j + i) : kNone;
+      else v[i] = j + i < end ? __ldg(reinterpret_cast<const unsigned short*>(l) + j + i) : kNone;
+    }
   }
 }
+template <typename T>
+ALM_DEV float value_of(uint32_t b) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(b);
+  else return Split<T>::value(b);
+}
+ALM_DEV void load8f(const float* l, int j, int end, bool vec, float (&v)[8]) {
+  uint32_t b[8];
+  load8(l, j, end, vec, b);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(b[i]);
+}
 
+ALM_DEV double warp_sum64(double z) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+  return z;
+}
 // (maximum, sum of 2^((v - maximum) k)) of two parts
 ALM_DEV void join(float& m, double& z, float om, double oz, float k) {
   const float nm = fmaxf(m, om);
@@ -169,193 +231,275 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
 
   auto row_ptr = [&](int i) { return reinterpret_cast<const T*>(a.logits + (row0 + i) * a.logits_row); };
 
-  // maximum and 32-bit sum (greedy: first place of the maximum) of every row's slice
-  for (int i = 0; i < n_row; ++i) {
-    const T* l = row_ptr(i);
-    float m = kNegInf;
-    if (greedy) {
+  // Maximum and 32-bit sum (greedy: first place of the maximum) of every row's
+  // slice.  The rows' blocks of 256 entries form one line that the warps share.
+  for (int i = tid; i < n_row * kVerWarps; i += kVerThreads) {
+    sh.wm[i / kVerWarps][i % kVerWarps] = kNegInf;
+    sh.ws[i / kVerWarps][i % kVerWarps] = 0.0;
+    sh.wi[i / kVerWarps][i % kVerWarps] = 0x7fffffff;
+  }
+  __syncthreads();
+  {
+    const int n_blk = (v1 - v0 + kVerBlock - 1) / kVerBlock;
+    const int b1 = n_row * n_blk * (warp + 1) / kVerWarps;
+    constexpr int kDeep = sizeof(T) == 4 ? 2 : 4;   // blocks in flight
+    for (int blk = n_row * n_blk * warp / kVerWarps; blk < b1;) {
+      const int i = blk / n_blk;
+      const int row_end = min(b1, (i + 1) * n_blk);
+      const T* l = row_ptr(i);
+      float m = kNegInf, z = 0.f;
       int at = 0x7fffffff;
-#pragma unroll 2
-      for (int j = v0 + tid * 8; j < v1; j += kVerThreads * 8) {
-        float v[8];
-        load8(l, j, v1, vec, v);
+      while (blk < row_end) {
+        uint32_t v[kDeep][8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (v[q] > m) m = v[q], at = j + q;
-      }
+        for (int d = 0; d < kDeep; ++d)
+          load8(l, v0 + (blk + d - i * n_blk) * kVerBlock + lane * 8, blk + d < row_end ? v1 : 0, vec, v[d]);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        join_first(m, at, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, at, o));
-      if (lane == 0) sh.wm[i][warp] = m, sh.wi[i][warp] = at;
-    } else {
-      float z = 0.f;
-#pragma unroll 4
-      for (int j = v0 + tid * 8; j < v1; j += kVerThreads * 8) {
-        float v[8];
-        load8(l, j, v1, vec, v);
-        float top = v[0];
+        for (int d = 0; d < kDeep; ++d) {
+          float f[8];
 #pragma unroll
-        for (int q = 1; q < 8; ++q) top = fmaxf(top, v[q]);   // a NaN is passed over
-        if (top > m) {
-          z *= ex2f_((m - top) * k_log2);
-          m = top;
+          for (int q = 0; q < 8; ++q) f[q] = value_of<T>(v[d][q]);
+          float top = f[0];
+#pragma unroll
+          for (int q = 1; q < 8; ++q) top = fmaxf(top, f[q]);   // a NaN is passed over
+          if (greedy) {
+            if (top > m) {
+              m = top;
+#pragma unroll
+              for (int q = 7; q >= 0; --q)
+                if (f[q] == top) at = v0 + (blk + d - i * n_blk) * kVerBlock + lane * 8 + q;
+            }
+            continue;
+          }
+          if (top > m) {
+            z *= ex2f_((m - top) * k_log2);
+            m = top;
+          }
+          // the difference first: it is small where the weight is not
+          const uint64_t m2 = pair(-m, -m), k2 = pair(k_log2, k_log2);
+          float sum = 0.f;
+#pragma unroll
+          for (int q = 0; q < 8; q += 2) {
+            float x, y;
+            unpair(mul2(add2(pair(f[q], f[q + 1]), m2), k2), x, y);
+            sum += ex2f_(x) + ex2f_(y);
+          }
+          if (!(sum < 16.f)) {   // NaN: a NaN logit, or infinities less infinities
+            sum = 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              sum += !(f[q] > kNegInf) ? 0.f : f[q] == m ? 1.f : ex2f_((f[q] - m) * k_log2);
+          }
+          z += sum;
         }
-        // the difference first: it is small where the weight is not
-        float sum = 0.f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) sum += ex2f_((v[q] - m) * k_log2);
-        if (!(sum < 16.f)) {   // NaN: a NaN logit, or infinities less infinities
-          sum = 0.f;
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            sum += !(v[q] > kNegInf) ? 0.f : v[q] == m ? 1.f : ex2f_((v[q] - m) * k_log2);
-        }
-        z += sum;
+        blk += kDeep;
       }
+      blk = row_end;
       double zd = z;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        join(m, zd, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, zd, o), k_log2);
-      if (lane == 0) sh.wm[i][warp] = m, sh.ws[i][warp] = zd;
+      for (int o = 16; o > 0; o >>= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, m, o);
+        if (greedy) join_first(m, at, om, __shfl_xor_sync(0xffffffffu, at, o));
+        else join(m, zd, om, __shfl_xor_sync(0xffffffffu, zd, o), k_log2);
+      }
+      if (lane == 0) sh.wm[i][warp] = m, sh.ws[i][warp] = zd, sh.wi[i][warp] = at;
     }
   }
   __syncthreads();
-  if (tid < n_row) {
-    float m = sh.wm[tid][0];
-    if (greedy) {
-      int at = sh.wi[tid][0];
-      for (int w = 1; w < kVerWarps; ++w) join_first(m, at, sh.wm[tid][w], sh.wi[tid][w]);
-      sh.cta_i[tid] = at;
-    } else {
-      double z = sh.ws[tid][0];
-      for (int w = 1; w < kVerWarps; ++w) join(m, z, sh.wm[tid][w], sh.ws[tid][w], k_log2);
-      sh.cta_s[tid] = z;
+  // a warp a row: the CTA's warps, then the cluster's CTAs, a lane each
+  auto join_lanes = [&](float& m, double& z, int& at) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, m, o);
+      if (greedy) join_first(m, at, om, __shfl_xor_sync(0xffffffffu, at, o));
+      else join(m, z, om, __shfl_xor_sync(0xffffffffu, z, o), k_log2);
     }
-    sh.cta_m[tid] = m;
+  };
+  for (int i = warp; i < n_row; i += kVerWarps) {
+    float m = sh.wm[i][lane % kVerWarps];
+    double z = lane < kVerWarps ? sh.ws[i][lane] : 0.0;
+    int at = sh.wi[i][lane % kVerWarps];
+    join_lanes(m, z, at);
+    if (lane == 0) sh.cta_m[i] = m, sh.cta_s[i] = z, sh.cta_i[i] = at;
   }
   cl.sync();
-  if (tid < n_row) {
-    const VerShared* r = cl.map_shared_rank(&sh, 0);
-    float m = r->cta_m[tid];
-    if (greedy) {
-      int at = r->cta_i[tid];
-      for (int c = 1; c < n_cta; ++c) {
-        const VerShared* q = cl.map_shared_rank(&sh, c);
-        join_first(m, at, q->cta_m[tid], q->cta_i[tid]);
-      }
-      sh.row_i[tid] = at;
-    } else {
-      double z = r->cta_s[tid];
-      for (int c = 1; c < n_cta; ++c) {
-        const VerShared* q = cl.map_shared_rank(&sh, c);
-        join(m, z, q->cta_m[tid], q->cta_s[tid], k_log2);
-      }
-      sh.row_z[tid] = z;
-    }
-    sh.row_m[tid] = m;
+  for (int i = warp; i < n_row; i += kVerWarps) {
+    const VerShared* o = cl.map_shared_rank(&sh, min(lane % 16, n_cta - 1));
+    const bool on = lane < n_cta;
+    float m = on ? o->cta_m[i] : kNegInf;
+    double z = on ? o->cta_s[i] : 0.0;
+    int at = on ? o->cta_i[i] : 0x7fffffff;
+    join_lanes(m, z, at);
+    if (lane == 0) sh.row_m[i] = m, sh.row_z[i] = z, sh.row_i[i] = at;
   }
   __syncthreads();
 
+  // 64-bit weights of row i: through the tables where they hold
+  extern __shared__ __align__(16) double tables[];
+  double *const t_hi = tables, *const t_lo = tables + Split<T>::kHi;
+  int tab_row = -1;          // the row the tables are made for
+  bool tab = false;          // ... and whether they are used
+  auto make_tables = [&](int i) {   // by the whole CTA
+    tab_row = i;
+    const float top = sh.row_m[i];
+    tab = Split<T>::kHi > 0 && tables_hold(top, temp);
+    if (!tab) return;
+    __syncthreads();         // the last row's are no longer read
+    for (int j = tid; j < Split<T>::kHi; j += kVerThreads) {
+      float v = 0.f;
+      bool finite = false;
+      Split<T>::parts(j, v, finite);
+      // (entries above the maximum are not read)
+      t_hi[j] = finite && v <= top + fabsf(top) ? exp64((static_cast<double>(v) - static_cast<double>(top)) * c64, sh.table) : 0.0;
+    }
+    for (int j = tid; j < Split<T>::kLo; j += kVerThreads) t_lo[j] = exp64(Split<T>::rest(j) * c64, sh.table);
+    __syncthreads();
+  };
+  auto wt = [&](uint32_t bits, float top) {   // of row tab_row
+    double e;
+    if (tab) e = t_hi[Split<T>::hi(bits)] * t_lo[Split<T>::lo(bits)];
+    else e = weight64(value_of<T>(bits), top, c64, sh.table);
+    return e < min_p ? 0.0 : e;
+  };
+  auto bits_at = [&](int i, int j) -> uint32_t {
+    if constexpr (sizeof(T) == 4) return __ldg(reinterpret_cast<const unsigned*>(row_ptr(i)) + j);
+    else return __ldg(reinterpret_cast<const unsigned short*>(row_ptr(i)) + j);
+  };
+
   // Sum of f over the vocabulary, 8 entries a lane; every CTA of the cluster
-  // calls it together.  near: whether any CTA's f raised sh.near_min.
+  // calls it together and gets the same value (the same additions).
   int turn = 0;
-  auto cluster_sum = [&](auto&& f, const T* l, bool& near) {
+  auto cluster_sum = [&](auto&& f, const T* l) {
     double z = 0.0;
     for (int j = v0 + tid * 8; j < v1; j += kVerThreads * 8) {
-      float v[8];
+      uint32_t v[8];
       load8(l, j, v1, vec, v);
 #pragma unroll
       for (int q = 0; q < 8; ++q) z += f(v[q]);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    z = warp_sum64(z);
     if (lane == 0) sh.dsum[warp] = z;
     __syncthreads();
-    if (tid == 0) {
-      double t = 0.0;
-      for (int w = 0; w < kVerWarps; ++w) t += sh.dsum[w];
-      sh.cta_d[turn] = t;
-      sh.cta_near[turn] = sh.near_min;
+    if (warp == 0) {
+      const double t = warp_sum64(lane < kVerWarps ? sh.dsum[lane] : 0.0);
+      if (lane == 0) sh.cta_d[turn] = t;
     }
     cl.sync();
-    double t = 0.0;
-    near = false;
-    for (int c = 0; c < n_cta; ++c) {
-      t += cl.map_shared_rank(&sh, c)->cta_d[turn];
-      near |= cl.map_shared_rank(&sh, c)->cta_near[turn] != 0;
-    }
+    // a lane a CTA: the remote reads are in flight together
+    const double part = lane < n_cta ? cl.map_shared_rank(&sh, lane)->cta_d[turn] : 0.0;
     turn ^= 1;
-    return t;
+    return warp_sum64(part);
   };
   auto exact_sum = [&](int i) {
     const float top = sh.row_m[i];
-    bool near;
-    return cluster_sum(
-        [&](float v) {
-          const double e = weight64(v, top, c64, sh.table);
-          return e < min_p ? 0.0 : e;
-        },
-        row_ptr(i), near);
+    if (tab_row != i) make_tables(i);
+    return cluster_sum([&](uint32_t v) { return wt(v, top); }, row_ptr(i));
   };
-  // The 32-bit sum without the entries below min-p; the 64-bit one where an
-  // entry is too near the border to tell.
-  auto min_p_sum = [&](int i, bool& exact) {
-    const float top = sh.row_m[i];
+  // Min-p: the 32-bit sums again without the entries below it, now that the
+  // maxima are known.  row_i tells whether an entry lies too near the border.
+  if (min_p > 0.0) {
     const float cut = static_cast<float>(min_p), lo = cut * (1.f - 1e-4f), hi = cut * (1.f + 1e-4f);
-    if (tid == 0) sh.near_min = 0;
+    const int n_blk = (v1 - v0 + kVerBlock - 1) / kVerBlock;
+    const int b1 = n_row * n_blk * (warp + 1) / kVerWarps;
+    for (int i = tid; i < n_row * kVerWarps; i += kVerThreads) {
+      sh.ws[i / kVerWarps][i % kVerWarps] = 0.0;
+      sh.wi[i / kVerWarps][i % kVerWarps] = 0;
+    }
     __syncthreads();
-    const double z = cluster_sum(
-        [&](float v) {
-          const float e = !(v > kNegInf) ? 0.f : v == top ? 1.f : ex2f_((v - top) * k_log2);
-          if (e >= lo && e <= hi) sh.near_min = 1;
-          return static_cast<double>(e < cut ? 0.f : e);
-        },
-        row_ptr(i), exact);
-    return exact ? exact_sum(i) : z;
-  };
+    for (int blk = n_row * n_blk * warp / kVerWarps; blk < b1;) {
+      const int i = blk / n_blk, row_end = min(b1, (i + 1) * n_blk);
+      const T* l = row_ptr(i);
+      const float top = sh.row_m[i];
+      float z = 0.f;
+      bool near = false;
+#pragma unroll 4
+      for (; blk < row_end; ++blk) {
+        uint32_t v[8];
+        load8(l, v0 + (blk - i * n_blk) * kVerBlock + lane * 8, v1, vec, v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float f = value_of<T>(v[q]);
+          const float e = !(f > kNegInf) ? 0.f : f == top ? 1.f : ex2f_((f - top) * k_log2);
+          near |= e >= lo && e <= hi;
+          z += e < cut ? 0.f : e;
+        }
+      }
+      const double zd = warp_sum64(z);
+      near = __any_sync(0xffffffffu, near);
+      if (lane == 0) sh.ws[i][warp] = zd, sh.wi[i][warp] = near;
+    }
+    cl.sync();       // (the CTA's barrier too; the first sums have been read)
+    for (int i = warp; i < n_row; i += kVerWarps) {
+      const double z = warp_sum64(lane < kVerWarps ? sh.ws[i][lane] : 0.0);
+      const int near = __any_sync(0xffffffffu, sh.wi[i][lane % kVerWarps] != 0);
+      if (lane == 0) sh.cta_s[i] = z, sh.cta_i[i] = near;
+    }
+    cl.sync();
+    for (int i = warp; i < n_row; i += kVerWarps) {
+      const VerShared* o = cl.map_shared_rank(&sh, min(lane, n_cta - 1));
+      const double z = warp_sum64(lane < n_cta ? o->cta_s[i] : 0.0);
+      const int near = __any_sync(0xffffffffu, o->cta_i[i] != 0);
+      if (lane == 0) sh.row_z[i] = z, sh.row_i[i] = near;
+    }
+    __syncthreads();
+  }
 
+  // Acceptance: lane i weighs token i (every warp alike), then the tokens are
+  // gone through in order; what the 32-bit sums leave open is summed in 64 bits.
   const int* x = a.draft + static_cast<size_t>(s) * a.k_max;
   int acc = 0;
   double z_stop = 0.0;
-  bool have_z = false, open = true;
-  for (int i = 0; i < k; ++i) {
-    const int xi = __ldg(x + i);
-    const bool in = xi >= 0 && xi < a.vocab;
-    const float top = sh.row_m[i];
-    double p = 0.0;
-    if (greedy) {
-      const bool same = in && top > kNegInf && xi == sh.row_i[i];
-      p = same ? 1.0 : 0.0;
-      if (open) {
-        if (same) ++acc;
-        else open = false;
-      }
-    } else {
-      double e = in ? weight64(Logit<T>::up(row_ptr(i)[xi]), top, c64, sh.table) : 0.0;
-      if (e < min_p) e = 0.0;
-      bool exact = false;
-      double z = sh.row_z[i];
-      if (min_p > 0.0 && top > kNegInf) z = min_p_sum(i, exact);
-      p = e > 0.0 ? e / z : 0.0;
-      if (open) {
+  bool have_z = false;
+  {
+    double p = 0.0, uq = 0.0, z = 0.0;
+    int xi = -1;
+    bool in = false, open = false;   // open: not decided by the 32-bit sum
+    if (lane < k) {
+      xi = __ldg(x + lane);
+      in = xi >= 0 && xi < a.vocab;
+      const float top = sh.row_m[lane];
+      if (greedy) {
+        p = in && top > kNegInf && xi == sh.row_i[lane] ? 1.0 : 0.0;
+      } else {
+        double e = in ? weight64(value_of<T>(bits_at(lane, xi)), top, c64, sh.table) : 0.0;
+        if (e < min_p) e = 0.0;
         const double q =
-            !a.q ? 1.0 : in ? static_cast<double>(__ldg(a.q + s * a.q_seq + i * a.q_step + xi)) : 0.0;
-        const double uq = __ldg(a.u + static_cast<size_t>(s) * (a.k_max + 1) + i) * q;
-        if (!exact && fabs(uq - p) <= kNear * p) {
-          z = exact_sum(i);
-          exact = true;
-          p = e > 0.0 ? e / z : 0.0;
-        }
-        if (uq < p) {
-          ++acc;
-        } else {
-          open = false;
-          z_stop = z;
-          have_z = exact;
-        }
+            !a.q ? 1.0 : in ? static_cast<double>(__ldg(a.q + s * a.q_seq + lane * a.q_step + xi)) : 0.0;
+        uq = __ldg(a.u + static_cast<size_t>(s) * (a.k_max + 1) + lane) * q;
+        z = sh.row_z[lane];
+        p = e > 0.0 ? e / z : 0.0;
+        open = fabs(uq - p) <= kNear * p || (min_p > 0.0 && sh.row_i[lane] != 0);
       }
     }
-    if (cta == 0 && tid == 0 && a.p_draft) a.p_draft[static_cast<size_t>(s) * a.k_max + i] = static_cast<float>(p);
+    unsigned yes = __ballot_sync(0xffffffffu, lane < k && uq < p);
+    unsigned unsure = __ballot_sync(0xffffffffu, open);
+    for (acc = 0; acc < k; ++acc) {
+      if (unsure >> acc & 1) {
+        const double zx = exact_sum(acc);
+        bool ok = false;
+        if (lane == acc) {
+          const double e = in ? wt(bits_at(acc, xi), sh.row_m[acc]) : 0.0;   // by the sum's own weights
+          z = zx;
+          p = e > 0.0 ? e / zx : 0.0;
+          ok = uq < p;
+        }
+        yes = (yes & ~(1u << acc)) | __ballot_sync(0xffffffffu, ok);
+        if (!(yes >> acc & 1)) z_stop = zx, have_z = true;
+      }
+      if (!(yes >> acc & 1)) break;
+    }
+    // (behind the first refusal p is reported from the 32-bit sums, but for
+    // entries at the min-p border, which only the 64-bit weights tell apart)
+    for (int i = acc + 1; i < k; ++i)
+      if (min_p > 0.0 && sh.row_i[i] != 0 && !greedy) {
+        const double zx = exact_sum(i);
+        if (lane == i) {
+          const double e = in ? wt(bits_at(i, xi), sh.row_m[i]) : 0.0;
+          p = e > 0.0 ? e / zx : 0.0;
+        }
+      }
+    if (cta == 0 && warp == 0 && a.p_draft && lane < k)
+      a.p_draft[static_cast<size_t>(s) * a.k_max + lane] = static_cast<float>(p);
   }
   if (cta == 0) {
     if (a.p_draft)
@@ -370,6 +514,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
     if (cta == 0 && tid == 0) tokens[acc] = top > kNegInf ? sh.row_i[acc] : -1;
   } else {
     const double z = have_z ? z_stop : exact_sum(acc);
+    if (tab_row != acc) make_tables(acc);
     const double inv_z = 1.0 / z;
     const T* l = row_ptr(acc);
     const float* q = a.q && acc < k ? a.q + s * a.q_seq + acc * a.q_step : nullptr;
@@ -382,13 +527,13 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
     for (int use_q = 1; use_q >= 0; --use_q) {
       // what a lane's 8 entries leave after the draft's share
       auto rest8 = [&](int j, double (&r)[8]) {
-        float v[8], w[8];
+        uint32_t v[8];
+        float w[8];
         load8(l, j, j1, vec, v);
-        if (use_q && q) load8(q, j, j1, q_vec, w);
+        if (use_q && q) load8f(q, j, j1, q_vec, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          double e = weight64(v[i], top, c64, sh.table);
-          e = e < min_p ? 0.0 : e * inv_z;
+          double e = wt(v[i], top) * inv_z;
           if (use_q && q) {
             // (a NaN or infinite share leaves nothing)
             e = fmax(e - static_cast<double>(w[i]), 0.0);
@@ -483,22 +628,32 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
 }
 
 template <typename T>
+constexpr int table_bytes() {
+  return (Split<T>::kHi + Split<T>::kLo) * static_cast<int>(sizeof(double));
+}
+
+template <typename T>
 cudaError_t launch_t(const Verify& a, cudaStream_t st) {
   // few sequences: 16 CTAs each, so that a row's slices stay short; many: 8
   // (the portable size, which more GPCs can place)
   const int ctas = a.n_seq <= 8 ? 16 : 8;
-  OpLaunch l(dim3(a.n_seq * ctas, 1, 1), kVerThreads, 0, st, ctas);
+  OpLaunch l(dim3(a.n_seq * ctas, 1, 1), kVerThreads, table_bytes<T>(), st, ctas);
   return cudaLaunchKernelEx(&l.cfg, verify_kernel<T>, a);
 }
 
 }  // namespace
 
+template <typename T>
+static cudaError_t verify_attrs_t() {
+  cudaError_t e = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, table_bytes<T>());
+  return e;
+}
 cudaError_t verify_init_attrs() {
-  cudaError_t e = cudaFuncSetAttribute(verify_kernel<half>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(verify_kernel<__nv_bfloat16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(verify_kernel<float>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaError_t e = verify_attrs_t<half>();
+  if (e == cudaSuccess) e = verify_attrs_t<__nv_bfloat16>();
+  if (e == cudaSuccess) e = verify_attrs_t<float>();
   return e;
 }
 
