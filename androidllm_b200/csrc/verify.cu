@@ -72,21 +72,24 @@ ALM_DEV double exp64(double t, const double* table) {   // 2^(t / 64)
   constexpr double kMagic = 6755399441055744.0;   // 1.5 * 2^52: adding it rounds to a whole number
   constexpr double a1 = 0.693147180559945309417 / 64, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3, a4 = a3 * a1 / 4,
                    a5 = a4 * a1 / 5;
-  if (!(t > -64000.0)) return 0.0;
-  const double r = t + kMagic;
+  // no branch: eight of these run side by side, and the 64-bit pipe's latency is long
+  const bool some = t > -64000.0;
+  const double tt = some ? t : 0.0;
+  const double r = tt + kMagic;
   const int n = __double2loint(r);
-  const double g = t - (r - kMagic);
+  const double g = tt - (r - kMagic);
   double p = fma(g, a5, a4);
   p = fma(g, p, a3);
   p = fma(g, p, a2);
   p = fma(g, p, a1);
   p = fma(g, p, 1.0);
   const double e = p * table[n & 63];
-  return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+  const double w = __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+  return some ? w : 0.0;
 }
 ALM_DEV double weight64(float l, float top, double c, const double* table) {
-  if (l == top) return l > kNegInf ? 1.0 : 0.0;
-  return exp64((static_cast<double>(l) - static_cast<double>(top)) * c, table);
+  const double e = exp64((static_cast<double>(l) - static_cast<double>(top)) * c, table);
+  return l == top && l > kNegInf ? 1.0 : e;
 }
 
 // 16-bit logits have few leading parts: l = h + r with h the value without its
@@ -183,14 +186,8 @@ ALM_DEV double warp_sum64(double z) {
   for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
   return z;
 }
-// (maximum, sum of 2^((v - maximum) k)) of two parts
-ALM_DEV void join(float& m, double& z, float om, double oz, float k) {
-  const float nm = fmaxf(m, om);
-  const double fa = m == nm ? 1.0 : static_cast<double>(ex2f_((m - nm) * k));
-  const double fb = om == nm ? 1.0 : static_cast<double>(ex2f_((om - nm) * k));
-  z = z * fa + oz * fb;
-  m = nm;
-}
+// A sum of 2^((v - m) k) for the maximum `top` instead of m.
+ALM_DEV float scaled(float z, float m, float top, float k) { return m == top ? z : z * ex2f_((m - top) * k); }
 // first place of the maximum
 ALM_DEV void join_first(float& m, int& at, float om, int oi) {
   at = m > om ? at : om > m ? oi : min(at, oi);
@@ -295,25 +292,29 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
         blk += kDeep;
       }
       blk = row_end;
-      double zd = z;
+      if (greedy) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o);
-        if (greedy) join_first(m, at, om, __shfl_xor_sync(0xffffffffu, at, o));
-        else join(m, zd, om, __shfl_xor_sync(0xffffffffu, zd, o), k_log2);
+        for (int o = 16; o > 0; o >>= 1)
+          join_first(m, at, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, at, o));
       }
+      const float top = warp_max(m);
+      const double zd = warp_sum(scaled(z, m, top, k_log2));
+      m = top;
       if (lane == 0) sh.wm[i][warp] = m, sh.ws[i][warp] = zd, sh.wi[i][warp] = at;
     }
   }
   __syncthreads();
   // a warp a row: the CTA's warps, then the cluster's CTAs, a lane each
   auto join_lanes = [&](float& m, double& z, int& at) {
+    if (greedy) {
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      const float om = __shfl_xor_sync(0xffffffffu, m, o);
-      if (greedy) join_first(m, at, om, __shfl_xor_sync(0xffffffffu, at, o));
-      else join(m, z, om, __shfl_xor_sync(0xffffffffu, z, o), k_log2);
+      for (int o = 8; o > 0; o >>= 1)
+        join_first(m, at, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, at, o));
+      return;
     }
+    const float top = warp_max(m);
+    z = warp_sum64(z * static_cast<double>(scaled(1.f, m, top, k_log2)));
+    m = top;
   };
   for (int i = warp; i < n_row; i += kVerWarps) {
     float m = sh.wm[i][lane % kVerWarps];
