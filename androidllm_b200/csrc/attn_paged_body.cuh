@@ -10,7 +10,7 @@
 // maximum grows).  A decode or verify pass reads far more K/V bytes than
 // it computes on, so HBM bounds it: the CTAs share all tiles evenly
 // (attn_sched.cuh), each streams its run of tiles through a ring of
-// shared-memory stages filled with cp.async across unit borders, and the rows
+// shared-memory stages filled across unit borders, and the rows
 // of the query heads that share a K/V head are one matrix operand, so K and V
 // are read once for all of them.
 //
@@ -20,6 +20,7 @@
 #pragma once
 #include <algorithm>
 
+#include "attn_paged_tma.cuh"
 #include "attn_sched.cuh"
 
 namespace alm {
@@ -81,8 +82,12 @@ ALM_DEV void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <int HD, int WM>
+// TMA: stages filled by a producer warp, each 128-byte column group of a tile
+// swizzled as TMA does; else (other head dimensions, pages that are not whole
+// 8-row pieces) by cp.async from all threads, with padded rows.
+template <int HD, int WM, bool TMA>
 struct PagedShape {
+  static constexpr int kThreads = kPagedThreads + (TMA ? kWarp : 0);
   static constexpr int kTile = HD > 128 ? 64 : 128;        // positions a tile
   static constexpr int kWK = kPagedWarps / WM;
   static constexpr int kNP = kTile / kWK;                  // positions a warp and tile
@@ -90,13 +95,22 @@ struct PagedShape {
   static constexpr int kRows = 16 * WM;
   // rows padded by 16 bytes: an odd number of 16-byte units, so that the 8
   // rows of an ldmatrix matrix lie in 8 different bank groups
-  static constexpr int kPitch = HD * 2 + 16;
-  static constexpr int kStageBytes = 2 * kTile * kPitch;
+  static constexpr int kPitch = TMA ? HD * 2 : HD * 2 + 16;
+  static constexpr int kTileBytes = kTile * kPitch;
+  static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kStages = HD <= 64 ? 6 : HD <= 96 ? 4 : 3;
-  // merge of the WK slices: 128 fp32 rows of HD / kPasses + 8 columns in one stage
+  // merge of the WK slices in one stage: 128 fp32 rows of HD / kPasses columns,
+  // padded by 8, or groups of 8 columns exchanged by the row's number
   static constexpr int kPasses = HD > 128 ? 4 : 1;
-  static constexpr int kMergePitch = HD / kPasses + 8;
-  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes;
+  static constexpr int kMergePitch = TMA ? HD : HD / kPasses + 8;
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + (TMA ? 1024 : 0);
+  // byte offset of 16-byte unit c of row r in a tile
+  ALM_DEV static uint32_t unit(int r, int c) {
+    if constexpr (TMA) return (c / 8) * (kTile * 128) + r * 128 + ((c ^ r) & 7) * 16;
+    else return r * kPitch + c * 16;
+  }
+  // element offset of column c of row r in the merge
+  ALM_DEV static int merge(int r, int c) { return r * kMergePitch + (TMA ? c ^ (r & 7) * 8 : c); }
   static_assert(128 * kMergePitch * 4 <= kStageBytes, "merge fits a stage");
   static_assert(kNP >= 16, "a warp's slice holds a k16 step");
 };
@@ -157,14 +171,18 @@ __device__ __noinline__ void row_by_formula(const AttnPaged& a, const PagedKV& k
   }
 }
 
-template <typename T, int HD, int WM>
-__global__ void __launch_bounds__(kPagedThreads, 1)
-attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ SeqBatch b,
-                  const __grid_constant__ PagedKV kv, int* err) {
-  using S = PagedShape<HD, WM>;
+template <typename T, int HD, int WM, bool TMA>
+__global__ void __launch_bounds__(PagedShape<HD, WM, TMA>::kThreads, 1)
+attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                  const __grid_constant__ AttnPaged a, const __grid_constant__ SeqBatch b,
+                  const __grid_constant__ PagedKV kv, int box_rows, int* err) {
+  using S = PagedShape<HD, WM, TMA>;
   constexpr int kTile = S::kTile, kWK = S::kWK, kNP = S::kNP, kChunk = S::kChunk, kRows = S::kRows;
-  extern __shared__ __align__(128) char smem[];
+  extern __shared__ __align__(128) char smem_raw[];
+  char* const smem = TMA ? smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023) : smem_raw;
   __shared__ SchedShared sched;
+  __shared__ uint64_t full[S::kStages], empty[S::kStages];
+  __shared__ int dead_flag;   // a wait ran out: everybody leaves
   __shared__ float st_m[kWK][kRows], st_l[kWK][kRows];
   __shared__ float row_m[kRows], row_l[kRows];
   __shared__ int row_bad[kRows];
@@ -175,13 +193,25 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
   const int wm = warp % WM, wk = warp / WM, g = lane / 4, t4 = lane % 4;
   const int tpu = kRows / a.group;
   const int cta = blockIdx.x;
-  sched_init<kTile>(
-      b, kv, tpu, a.window, sched,
-      [&](long long total) {
-        const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
-        return cta < n ? share(total, cta, n) : -1ll;
-      },
-      [] { __syncthreads(); });
+  // barrier of the eight computing warps
+  auto sync = [] {
+    if constexpr (TMA) bar_sync(1, kPagedThreads);
+    else __syncthreads();
+  };
+  if (TMA && tid == kPagedThreads) {
+    for (int i = 0; i < S::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], kPagedWarps);
+    dead_flag = 0;
+    fence_mbar_init();
+  }
+  if (!TMA || warp < kPagedWarps)
+    sched_init<kTile>(
+        b, kv, tpu, a.window, sched,
+        [&](long long total) {
+          const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
+          return cta < n ? share(total, cta, n) : -1ll;
+        },
+        sync);
+  if (TMA) __syncthreads();
   const long long total = sched.total;
   const int n_cta = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
   if (tid == 0) *join_record(a, cta) = make_int4(0, 0, 0, 0);
@@ -195,6 +225,42 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
   Unit lu = u;
   int lt = t, ltb = tb;
   const uint32_t smem0 = smem_addr(smem);
+  volatile int* dead = &dead_flag;
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) {   // the same answer for the whole warp
+    const bool ok = mbar_try_wait(bar, parity & 1) || slow_wait(bar, parity & 1, dead, err);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
+  if (TMA && warp == kPagedWarps) {
+    // the producer: a page piece of K and of V a lane (128 / 8 pieces of 2 column groups at most)
+    const int n_box = kTile / box_rows * (HD / 64), box = lane / (HD / 64), c = lane % (HD / 64);
+    bool bad = false, quit = false;
+    for (uint32_t n = 0; !quit; ++n) {
+      const int y = piece_row(kv, lu.pages, lu.h, lu.n_kv, (lu.t0 + lt) * kTile + box * box_rows, lane < n_box, bad);
+      const uint32_t st = n % S::kStages;
+      if (!wait_warp(&empty[st], n / S::kStages + 1)) {
+        quit = true;
+        break;
+      }
+      if (lane == 0) mbar_expect_tx(&full[st], S::kStageBytes);
+      __syncwarp();
+      if (lane < n_box) {
+        const uint32_t dst = smem0 + st * S::kStageBytes + c * (kTile * 128) + box * box_rows * 128;
+        tma_2d(dst, &k_map, c * 64, y, &full[st]);
+        tma_2d(dst + S::kTileBytes, &v_map, c * 64, y, &full[st]);
+      }
+      __syncwarp();
+      if (++lt == ltb) {
+        if (!lu.more(x1)) break;
+        next_unit<kTile>(b, kv, tpu, a.window, lu);
+        lt = 0;
+        ltb = lu.upto(x1);
+      }
+    }
+    if (bad) *err = 1;
+    if (quit)   // no copy is in flight when the CTA leaves
+      for (int i = 0; i < S::kStages; ++i) mbar_wait(&full[i], 0), mbar_wait(&full[i], 1);
+    return;
+  }
   constexpr int kUnits16 = HD / 8;   // 16-byte units of a K or V row
   bool bad_page = false;
 
@@ -219,8 +285,8 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
         bad_page |= !ok && pos < lu.n_kv;
         const size_t off =
             (ok ? kv_offset(kv, page[i], lu.h, pos - page_of(kv, pos) * kv.page_size) + c * 8 : 0) * sizeof(T);
-        cp_async16(dst + r * S::kPitch + c * 16, kv.k + off, ok ? 16 : 0);
-        cp_async16(dst + (kTile + r) * S::kPitch + c * 16, kv.v + off, ok ? 16 : 0);
+        cp_async16(dst + S::unit(r, c), kv.k + off, ok ? 16 : 0);
+        cp_async16(dst + S::kTileBytes + S::unit(r, c), kv.v + off, ok ? 16 : 0);
       }
       if (++lt == ltb && lu.more(x1)) {
         next_unit<kTile>(b, kv, tpu, a.window, lu);
@@ -230,8 +296,10 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
     }
     cp_async_commit();
   };
+  if (!TMA) {
 #pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) load_tile(i);
+    for (int i = 0; i < S::kStages - 1; ++i) load_tile(i);
+  }
 
   int t_first = t;   // first tile of the unit computed here
   uint32_t qf[HD / 16][4];
@@ -262,11 +330,33 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
   begin_unit();
 
   int stage = 0;
+  uint32_t round = 0;
+  auto next_stage = [&] {
+    if (++stage == S::kStages) stage = 0, round ^= 1;
+  };
   for (;;) {
-    cp_async_wait<S::kStages - 2>();
-    __syncthreads();
-    load_tile(stage == 0 ? S::kStages - 1 : stage - 1);
-    const uint32_t kb = smem0 + stage * S::kStageBytes, vb = kb + kTile * S::kPitch;
+    if constexpr (TMA) {
+      wait_warp(&full[stage], round);
+    } else {
+      cp_async_wait<S::kStages - 2>();
+      __syncthreads();
+      load_tile(stage == 0 ? S::kStages - 1 : stage - 1);
+    }
+    const uint32_t kb = smem0 + stage * S::kStageBytes, vb = kb + S::kTileBytes;
+    if constexpr (TMA) {
+      // The sequence ends in this tile, and its last page piece goes on behind
+      // it: those rows hold anything, and a zero weight times NaN is NaN.  Each
+      // warp clears what it reads.
+      const int end = u.n_kv - (u.t0 + t) * kTile;   // rows of the tile that exist
+      if (end < (wk + 1) * kNP) {
+        const int z0 = max(end, wk * kNP);
+        for (int i = lane; i < ((wk + 1) * kNP - z0) * kUnits16; i += kWarp)
+          *reinterpret_cast<uint4*>(smem + stage * S::kStageBytes + S::kTileBytes +
+                                    S::unit(z0 + i / kUnits16, i % kUnits16)) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();   // before the stage is filled again
+        __syncwarp();
+      }
+    }
 #pragma unroll 1
     for (int c0 = 0; c0 < kNP; c0 += kChunk) {
       const int r0 = wk * kNP + c0;                    // first row of the chunk in the stage
@@ -282,8 +372,7 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
         for (int n = 0; n < kChunk / 8; n += 2) {
           uint32_t b0, b1, b2, b3;
           ldmatrix_x4_at(b0, b1, b2, b3,
-                         kb + (r0 + n * 8 + (lane & 7) + ((lane >> 4) & 1) * 8) * S::kPitch +
-                             (2 * k + ((lane >> 3) & 1)) * 16);
+                         kb + S::unit(r0 + n * 8 + (lane & 7) + ((lane >> 4) & 1) * 8, 2 * k + ((lane >> 3) & 1)));
           Elem<T>::mma(s[n], qf[k], b0, b1);
           Elem<T>::mma(s[n + 1], qf[k], b2, b3);
         }
@@ -335,8 +424,7 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
         for (int n = 0; n < HD / 8; n += 2) {
           uint32_t b0, b1, b2, b3;
           ldmatrix_x4_trans(b0, b1, b2, b3,
-                            vb + (r0 + k * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * S::kPitch +
-                                (n + (lane >> 4)) * 16);
+                            vb + S::unit(r0 + k * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, n + (lane >> 4)));
           Elem<T>::mma(o[n], p, b0, b1);
           Elem<T>::mma(o[n + 1], p, b2, b3);
         }
@@ -344,7 +432,11 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
     }
     if (t + 1 < tb) {
       ++t;
-      if (++stage == S::kStages) stage = 0;
+      if constexpr (TMA) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+      }
+      next_stage();
       continue;
     }
 
@@ -359,7 +451,7 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
       }
     }
     if (tid < kRows) row_bad[tid] = 0;
-    __syncthreads();
+    sync();
     if (tid < kRows) {
       float mm = kNegInf, ll = 0.f;
 #pragma unroll
@@ -394,9 +486,9 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
       for (int n = 0; n < kCols / 8; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          *reinterpret_cast<float2*>(buf + (wk * kRows + wm * 16 + g + 8 * j) * S::kMergePitch + n * 8 + 2 * t4) =
+          *reinterpret_cast<float2*>(buf + S::merge(wk * kRows + wm * 16 + g + 8 * j, n * 8 + 2 * t4)) =
               make_float2(o[ps * (kCols / 8) + n][2 * j], o[ps * (kCols / 8) + n][2 * j + 1]);
-      __syncthreads();
+      sync();
       for (int i = tid; i < kRows * (kCols / 4); i += kPagedThreads) {
         const int row = i / (kCols / 4), c = (i % (kCols / 4)) * 4;
         const int tok = row / a.group, hh = row - tok * a.group;
@@ -404,7 +496,7 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWK; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(buf + (w * kRows + row) * S::kMergePitch + c);
+          const float4 y = *reinterpret_cast<const float4*>(buf + S::merge(w * kRows + row, c));
           v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
         }
         const bool bad = !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < __int_as_float(0x7f800000)) ;
@@ -431,9 +523,18 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
           }
         }
       }
-      if (ps + 1 < S::kPasses) __syncthreads();
+      if (ps + 1 < S::kPasses) sync();
     }
-    if (__syncthreads_or(any_bad)) {
+    bool some_bad;
+    if constexpr (TMA) some_bad = bar_or(1, kPagedThreads, any_bad);
+    else some_bad = __syncthreads_or(any_bad) != 0;
+    if constexpr (TMA) {
+      // the merge wrote the stage: its next fill comes after that
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+    }
+    if (some_bad) {
       for (int row = warp; row < kRows; row += kPagedWarps) {
         if (!row_bad[row]) continue;
         const int tok = row / a.group, hh = row - tok * a.group, head = u.h * a.group + hh;
@@ -463,9 +564,9 @@ attn_paged_kernel(const __grid_constant__ AttnPaged a, const __grid_constant__ S
     t = t_first = 0;
     tb = u.upto(x1);
     begin_unit();
-    if (++stage == S::kStages) stage = 0;
+    next_stage();
   }
-  cp_async_wait<0>();
+  if (!TMA) cp_async_wait<0>();
   if (bad_page) *err = 1;
 }
 
@@ -545,16 +646,20 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const __g
   }
 }
 
-template <typename T, int HD, int WM>
+template <typename T, int HD, int WM, bool TMA = false>
 cudaError_t paged_attr() {
-  return cudaFuncSetAttribute(attn_paged_kernel<T, HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(PagedShape<HD, WM>::kSmem));
+  return cudaFuncSetAttribute(attn_paged_kernel<T, HD, WM, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              static_cast<int>(PagedShape<HD, WM, TMA>::kSmem));
 }
 template <typename T, int HD>
 cudaError_t paged_attr_hd() {
   cudaError_t e = paged_attr<T, HD, 2>();
   if constexpr (HD <= 128) {
     if (e == cudaSuccess) e = paged_attr<T, HD, 1>();
+  }
+  if constexpr (HD == 64 || HD == 128) {
+    if (e == cudaSuccess) e = paged_attr<T, HD, 1, true>();
+    if (e == cudaSuccess) e = paged_attr<T, HD, 2, true>();
   }
   if (e == cudaSuccess) e = paged_attr<T, HD, 4>();
   if (e == cudaSuccess) e = paged_attr<T, HD, 8>();
@@ -577,11 +682,14 @@ cudaError_t launch_join(const AttnPaged& a, cudaStream_t st) {
   return cudaLaunchKernelEx(&l.cfg, attn_paged_join_kernel<T, HD, ROWS, BLK>, a);
 }
 
-template <typename T, int HD, int WM>
+template <typename T, int HD, int WM, bool TMA = false>
 cudaError_t launch_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st) {
-  using S = PagedShape<HD, WM>;
-  OpLaunch l(dim3(a.n_cta, 1, 1), kPagedThreads, S::kSmem, st);
-  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, attn_paged_kernel<T, HD, WM>, a, b, kv, err);
+  using S = PagedShape<HD, WM, TMA>;
+  CUtensorMap km = {}, vm = {};
+  const int box = TMA ? page_box_rows(kv) : 0;
+  if (TMA && (!encode_pages<T>(&km, kv.k, kv, box) || !encode_pages<T>(&vm, kv.v, kv, box))) return cudaErrorInvalidValue;
+  OpLaunch l(dim3(a.n_cta, 1, 1), S::kThreads, S::kSmem, st);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, attn_paged_kernel<T, HD, WM, TMA>, km, vm, a, b, kv, box, err);
   return e != cudaSuccess ? e : launch_join<T, HD, S::kRows, S::kRows>(a, st);
 }
 
@@ -590,6 +698,10 @@ cudaError_t launch_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& k
 template <typename T, int HD>
 cudaError_t launch_paged_hd(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int* err, cudaStream_t st) {
   const long long rows = static_cast<long long>(b.max_rows) * a.group;
+  if constexpr (HD == 64 || HD == 128) {
+    if (rows <= 32 && tma_pages(kv))
+      return rows <= 16 ? launch_paged<T, HD, 1, true>(a, b, kv, err, st) : launch_paged<T, HD, 2, true>(a, b, kv, err, st);
+  }
   if constexpr (HD <= 128) {
     if (rows <= 16) return launch_paged<T, HD, 1>(a, b, kv, err, st);
   }

@@ -26,11 +26,6 @@
 // and exponential units bound long chunks (at 128 x 128 x 128 both take
 // about 512 cycles of an SM), HBM short ones.
 #pragma once
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include <algorithm>
-#include <type_traits>
 
 #include "attn_paged_body.cuh"
 #include "tc.cuh"
@@ -116,20 +111,6 @@ ALM_DEV void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-ALM_DEV void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          dst),
-      "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
-      : "memory");
-}
-ALM_DEV void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
-      : "memory");
-}
 ALM_DEV float fmax3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -147,35 +128,12 @@ ALM_DEV float max64(const uint32_t (&a)[32], const uint32_t (&b)[32]) {
   }
   return fmaxf(fmax3(t[0], t[1], t[2]), t[3]);
 }
-// One lane of a converged warp.  (With this instruction, unlike a test of the
-// lane number, the compiler knows that one thread runs what follows.)
-ALM_DEV bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
-  return p != 0;
-}
-ALM_DEV void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-ALM_DEV void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-
 // Instruction descriptor: fp32 accumulator, A and B of type T, N wide; bmn: B
 // is stored with N contiguous (V: positions by head dimensions).
 template <typename T>
 constexpr uint32_t tc_idesc(int n, bool bmn) {
   const uint32_t f = sizeof(T) == 2 && !std::is_same<T, half>::value ? 1u : 0u;
   return (1u << 4) | (f << 7) | (f << 10) | ((bmn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
-}
-
-// The rest of a wait whose first look failed: true when the phase completed.
-ALM_DEV bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
-  const unsigned long long t0 = global_ns();
-  for (unsigned i = 0; i < kSpinLimit; ++i) {
-    if (mbar_try_wait_suspend(bar, parity)) return true;
-    if (*dead) return false;
-    if (global_ns() - t0 > kWaitLimitNs) break;
-  }
-  *dead = 1;
-  *err = 2;
-  return false;
 }
 
 template <typename T, int HD, int NQ>
@@ -275,21 +233,13 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       // ---- loads ---------------------------------------------------------------
       uint32_t fills[2] = {0, 0};   // of each ring
       bool bad = false, quit = false;
-      const int rows_total = kv.n_pages * kv.kv_heads * kv.page_size;
       const int n_box = 128 / box_rows * S::kChunks;
       auto load = [&](const CUtensorMap* map, int t, int ring) {
         const uint32_t fill = ring == 0 ? fills[0]++ : fills[1]++;
         const int at = ring * S::kRing + fill % S::kRing;
         // one box a lane: at most 128 / 8 pieces of at most 2 column groups
         const int box = lane / S::kChunks, c = lane % S::kChunks;
-        const int pos = (u.t0 + t) * S::kTile + box * box_rows;
-        const bool in = lane < n_box && pos < u.n_kv;
-        const int pi = page_of(kv, pos);
-        const int page = in && u.pages ? __ldg(u.pages + pi) : -1;
-        const bool ok = page >= 0 && page < kv.n_pages;
-        bad |= in && !ok;
-        // a row behind the tensor's end reads zeros
-        const int y = ok ? (page * kv.kv_heads + u.h) * kv.page_size + pos - pi * kv.page_size : rows_total;
+        const int y = piece_row(kv, u.pages, u.h, u.n_kv, (u.t0 + t) * S::kTile + box * box_rows, lane < n_box, bad);
         if (quit || !wait_warp(&sh.empty[at], fill / S::kRing + 1)) {
           quit = true;
           return;
@@ -752,35 +702,11 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
 }
 
 // ---- host --------------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 cu_tensor_map_encoder();
-
-// K or V as rows of head_dim elements, read as boxes of box_rows rows x 64 columns.
-template <typename T>
-bool encode_pages(CUtensorMap* map, const char* p, const PagedKV& kv, int box_rows) {
-  const PFN_cuTensorMapEncodeTiled_v12000 enc = cu_tensor_map_encoder();
-  if (enc == nullptr) return false;
-  cuuint64_t dims[2] = {static_cast<cuuint64_t>(kv.head_dim),
-                        static_cast<cuuint64_t>(kv.n_pages) * kv.kv_heads * kv.page_size};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(kv.head_dim) * sizeof(T)};
-  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
-  cuuint32_t estr[2] = {1, 1};
-  return enc(map, std::is_same<T, half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-             const_cast<char*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// Rows of a TMA box: the largest power of two that divides the page, at most a tile.
-inline int page_box_rows(const PagedKV& kv) { return std::min(kv.page_size & -kv.page_size, 128); }
-
-// What the tensor-core kernels take: pages of whole 8-row pieces (the swizzle's
-// period), head dimensions of 64 or 128, and a row index that fits a TMA coordinate.
-// Q strides are positive and below 2^40 bytes, as a tensor map's have to be.
+// What the tensor-core kernels take: pages that TMA reads, and Q strides that
+// are positive and below 2^40 bytes, as a tensor map's have to be.
 inline bool tc_paged_fits(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv) {
   auto stride = [](int64_t bytes, int n) { return n <= 1 || (bytes > 0 && bytes < (1ll << 40)); };
-  return (kv.head_dim == 64 || kv.head_dim == 128) && kv.page_size % 8 == 0 && stride(a.q_head, a.heads) &&
-         stride(a.q_row, b.n_rows) &&
-         static_cast<long long>(kv.n_pages) * kv.kv_heads * kv.page_size < (1ll << 31) - 256;
+  return tma_pages(kv) && stride(a.q_head, a.heads) && stride(a.q_row, b.n_rows);
 }
 
 // Q as (columns, heads, rows): boxes of 64 columns x the heads of one K/V head
