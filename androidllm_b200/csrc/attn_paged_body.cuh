@@ -132,8 +132,9 @@ ALM_DEV int4 record_of(const Unit& u, int cta, int n_cta, long long total) {
 }
 
 // One row by one warp straight from the formula, skipping every position the
-// row does not see: for rows whose sums are not finite, since a hidden
-// position's infinity or NaN times a zero weight spoils a matrix product.
+// row does not see: for rows whose sums are not finite though their weights
+// are, since a hidden position's infinity or NaN times a zero weight spoils a
+// matrix product.
 template <typename T, int HD>
 __device__ __noinline__ void row_by_formula(const AttnPaged& a, const PagedKV& kv, const int* pages, int kv_head, int row,
                                             int head, int p_lo, int p_hi, float (&o)[HD / 32], float& m, float& l) {
@@ -232,7 +233,8 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   };
   if (TMA && warp == kPagedWarps) {
     // the producer: a page piece of K and of V a lane (128 / 8 pieces of 2 column groups at most)
-    const int n_box = kTile / box_rows * (HD / 64), box = lane / (HD / 64), c = lane % (HD / 64);
+    constexpr int kGroups = HD < 64 ? 1 : HD / 64;   // 128-byte column groups
+    const int n_box = kTile / box_rows * kGroups, box = lane / kGroups, c = lane % kGroups;
     bool bad = false, quit = false;
     for (uint32_t n = 0; !quit; ++n) {
       const int y = piece_row(kv, lu.pages, lu.h, lu.n_kv, (lu.t0 + lt) * kTile + box * box_rows, lane < n_box, bad);
@@ -536,7 +538,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     }
     if (some_bad) {
       for (int row = warp; row < kRows; row += kPagedWarps) {
-        if (!row_bad[row]) continue;
+        if (!row_bad[row] || row_l[row] != row_l[row]) continue;   // a NaN score that it sees spoils the whole row
         const int tok = row / a.group, hh = row - tok * a.group, head = u.h * a.group + hh;
         const int last = u.pos0 + tok;
         const int p_lo = max((u.t0 + t_first) * kTile, a.window > 0 ? last - a.window + 1 : 0);

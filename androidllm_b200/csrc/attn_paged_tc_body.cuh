@@ -657,7 +657,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           }
         }
         // rows whose sums are not finite, by the formula
-        unsigned todo = __ballot_sync(0xffffffffu, odd && live);
+        unsigned todo = __ballot_sync(0xffffffffu, odd && live && l == l);   // (a NaN score spoils its whole row)
         while (todo) {
           const int src = __ffs(todo) - 1;
           todo &= todo - 1;

@@ -43,7 +43,8 @@ ALM_DEV Seq load_seq(const SeqBatch& b, const PagedKV& kv, int s) {
   const int hi = max(lo, min(__ldg(b.row_start + s + 1), b.n_rows));
   q.row0 = lo;
   q.n_new = hi - lo;
-  const long long cap = static_cast<long long>(b.table_pages) * kv.page_size;
+  // (256 below 2^31, so that the end of a tile behind the last position is a number)
+  const long long cap = min(static_cast<long long>(b.table_pages) * kv.page_size, 0x7fffff00ll);
   const int len = max(0, __ldg(b.kv_len + s));
   q.n_kv = len > cap ? static_cast<int>(cap) : len;
   const int t = b.slots ? __ldg(b.slots + s) : s;

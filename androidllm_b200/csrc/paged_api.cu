@@ -140,7 +140,8 @@ ALM_API int alm_rope_append(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq
   TRY(check_kv(kv_, &kv));
   TRY(check_batch(batch, &b));
   REQ(v->heads >= 1 && v->heads <= 65536, "heads must be in 1..65536");
-  REQ(v->q_dev && v->k_dev && v->v_dev && v->q_out_dev && v->rope_dev, "null argument");
+  const bool none = b.n_seq == 0 || b.n_rows == 0;   // nothing to do: the tensors may be empty
+  REQ(none || (v->q_dev && v->k_dev && v->v_dev && v->q_out_dev && v->rope_dev), "null argument");
   REQ(aligned16(v->q_dev) && aligned16(v->k_dev) && aligned16(v->v_dev) && aligned16(v->q_out_dev) &&
           aligned16(v->rope_dev) && aligned16(v->q_norm_dev) && aligned16(v->k_norm_dev),
       "tensors must be 16-byte aligned");
@@ -156,7 +157,7 @@ ALM_API int alm_rope_append(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq
   int device, n_sms, *err;
   cudaStream_t st;
   TRY(alm_internal_ctx_paged(ctx, &device, &n_sms, &st, &err));
-  if (b.n_seq == 0 || b.n_rows == 0) return ALM_OK;
+  if (none) return ALM_OK;
   RopeAppend a;
   a.q = static_cast<const char*>(v->q_dev);
   a.k = static_cast<const char*>(v->k_dev);
@@ -196,20 +197,22 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   SeqBatch b;
   TRY(check_kv(kv_, &kv));
   TRY(check_batch(batch, &b));
-  REQ(v->q_dev && v->out_dev && v->work_dev, "null argument");
+  const bool none = b.n_seq == 0 || b.n_rows == 0;   // nothing to do: the tensors may be empty
+  REQ(none || (v->q_dev && v->out_dev), "null argument");
+  REQ(v->work_dev, "null argument");
   REQ(v->heads >= 1 && v->heads % kv.kv_heads == 0, "heads must be a multiple of kv_heads");
   REQ(v->heads / kv.kv_heads <= 128, "at most 128 query heads may share a K/V head");
   REQ(aligned16(v->q_dev) && aligned16(v->out_dev), "tensors must be 16-byte aligned");
   REQ(vec8(v->q_row) && vec8(v->q_head) && vec8(v->out_row) && vec8(v->out_head),
       "row and head strides must be multiples of 8 elements");
   REQ(v->window >= 0, "window must not be negative");
-  REQ(v->scale > 0.f && std::isfinite(v->scale), "scale must be positive and finite");
+  REQ(v->scale > 0.f && v->scale <= 1e30f, "scale must be positive and at most 1e30");
   REQ((reinterpret_cast<uintptr_t>(v->work_dev) & 255) == 0, "the work area must be 256-byte aligned");
   int device, n_sms, *err;
   cudaStream_t st;
   TRY(alm_internal_ctx_paged(ctx, &device, &n_sms, &st, &err));
   REQ(v->work_bytes >= attn_paged_work_bytes(n_sms, kv.head_dim), "the work area is too small (alm_attn_paged_work)");
-  if (b.n_seq == 0 || b.n_rows == 0) return ALM_OK;
+  if (none) return ALM_OK;
   AttnPaged a;
   a.q = static_cast<const char*>(v->q_dev);
   a.q_row = v->q_row * 2, a.q_head = v->q_head * 2;

@@ -108,7 +108,7 @@ def _dense(shape, stride):
     n = 1
     for d, s in zip(reversed(shape), reversed(stride)):
         if d != 1 and s != n:
-            return False
+            return 0 in shape
         n *= d
     return True
 

@@ -900,3 +900,145 @@ def test_operators_on_a_models_own_cache(model_dirs, golden_models):
     # the other slot is untouched
     k1, _ = kv.read(0, 0, 32, slot=1)
     assert not k1.any()
+
+
+def test_empty_batches_do_nothing(ctx):
+    k = torch.zeros(2, 1, 16, 64, device="cuda", dtype=torch.float16)
+    kv, work = paged.PagedKV(k, k.clone()), paged.AttnWorkspace(ctx, 2, 1, 64)
+    table = torch.zeros(1, 2, device="cuda", dtype=torch.int32)
+    for n_seq in (0, 1):
+        seqs = paged.SeqBatch(ints([0] * (n_seq + 1)), ints([5] * n_seq), table, n_rows=0)
+        q = torch.zeros(0, 2, 64, device="cuda", dtype=torch.float16)
+        one = torch.zeros(0, 1, 64, device="cuda", dtype=torch.float16)
+        paged.attn_paged(ctx, kv, seqs, q, torch.empty_like(q), work)
+        paged.rope_append(ctx, kv, seqs, q, one, one, table_of(4, 64, torch.float32), torch.empty_like(q))
+    f = lambda *s: torch.zeros(*s, device="cuda")
+    paged.verify(ctx, ints([0]), f(0, 10).half(), ints([]).view(0, 2), None, f(0, 3).double(), f(0), ints([]).view(0, 3),
+                 ints([]))
+    # sequences without rows: nothing accepted, nothing emitted
+    tok, acc = torch.full((2, 1), 9, device="cuda", dtype=torch.int32), ints([9, 9])
+    paged.verify(ctx, ints([0, 0, 0]), f(0, 10).half(), ints([]).view(2, 0), None, f(2, 1).double(), f(2), tok, acc)
+    ctx.sync()
+    assert tok.tolist() == [[-1], [-1]] and acc.tolist() == [0, 0] and not k.any()
+
+
+def test_attend_rows_with_a_nan_query(ctx):
+    """A NaN in a row's query spoils that row of that head alone."""
+    for rows in (3, 100):
+        b = Batch([rows], [rows + 200], 16, 2, 64, torch.float16, seed=50)
+        q = b.randn(b.n_rows, 4, 64)
+        ref, _ = attend(ctx, b, q)
+        q[1, 2, 5] = float("nan")
+        out, _ = attend(ctx, b, q)
+        ctx.sync()
+        assert torch.isnan(out[1, 2]).all()
+        out[1, 2] = ref[1, 2]
+        assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("rows", [1, 90])
+def test_attend_odd_query_strides(ctx, rows):
+    """Rows closer than heads, one row repeated by a stride of 0, and a tensor of one head."""
+    b = Batch([rows], [rows + 60], 16, 1, 64, torch.float16, seed=51, tail=0)
+    q = b.randn(1, 4, 64)
+    wide = q.expand(rows, 4, 64)                       # row stride 0
+    out, _ = attend(ctx, b, wide, want_lse=False, out=torch.full((rows, 4, 64), 77.0, device="cuda", dtype=q.dtype))
+    ctx.sync()
+    check_result(b, wide, out, None)
+    one = b.randn(rows, 1, 64)
+    check_attend(ctx, b, one)
+
+
+def test_captured_after_a_copy_and_before_one(ctx):
+    """The operators' launches overlap the previous kernel's end; copies and fills around them stay ordered."""
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        c = ops.Context(0, st.cuda_stream)
+        b = Batch([4], [300], 16, 2, 64, torch.float16, seed=52, tail=0)
+        src, q = b.randn(4, 8, 64), torch.zeros(4, 4, 64, device="cuda", dtype=torch.float16)
+        new = torch.zeros(4, 4, 64, device="cuda", dtype=torch.float16)
+        out, kept = torch.zeros_like(q), torch.zeros_like(q)
+        work, table = paged.AttnWorkspace(c, 4, 2, 64), table_of(300, 64, torch.float32)
+
+        def step():
+            q.copy_(src[:, :4])
+            new.copy_(src[:, 4:])
+            paged.rope_append(c, b.kv, b.seqs, q, new[:, :2], new[:, 2:], table, q)
+            paged.attn_paged(c, b.kv, b.seqs, q, out, work)
+            kept.copy_(out)
+            q.zero_()
+            out.zero_()
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            step()
+        for _ in range(3):
+            src.copy_(b.randn(4, 8, 64))
+            g.replay()
+            c.sync()
+            pos = torch.arange(296, 300, device="cuda")
+            turned_q = turned(src[:, :4], None, table, pos, 64, False, 0).half()
+            ref, tol, _, _ = formula(b, turned_q, 64 ** -0.5)
+            # one more half step a query value: the rotation's own rounding may fall to the other side
+            slack = 2.0 ** -10 * 64 ** -0.5 * 64 * 4
+            assert ((kept.double() - ref).abs() <= tol + slack * 4).all() and not out.any() and not q.any()
+            step()
+            c.sync()
+
+
+def test_two_contexts_at_once():
+    """Calls of two contexts on two streams, without waiting in between."""
+    todo = []
+    for i in range(2):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            c = ops.Context(0, st.cuda_stream)
+            b = Batch([7, 300], [5000, 700], 16, 2, 128, torch.bfloat16, seed=60 + i)
+            q = b.randn(b.n_rows, 14, 128)
+            ref, _ = attend(c, b, q)
+            todo.append((st, c, b, q, paged.AttnWorkspace(c, 14, 2, 128), ref))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for i, (st, c, b, q, work, _) in enumerate(todo):
+            with torch.cuda.stream(st):
+                outs[i].append(attend(c, b, q, work=work)[0])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, todo[i][5]) for o in outs[i])
+
+
+def test_cuda_array_interface_arrays(ctx):
+    class Cai:
+        def __init__(self, t):
+            self.t = t
+            self.shape = tuple(t.shape)
+            kind = {torch.float16: "<f2", torch.int32: "<i4", torch.float32: "<f4"}[t.dtype]
+            size = t.element_size()
+            self.__cuda_array_interface__ = {"data": (t.data_ptr(), False), "shape": self.shape, "typestr": kind,
+                                             "strides": tuple(s * size for s in t.stride()), "version": 3}
+    b = Batch([2], [40], 16, 2, 64, torch.float16, seed=53)
+    q = b.randn(b.n_rows, 4, 64)
+    ref, _ = attend(ctx, b, q)
+    kv = paged.PagedKV(Cai(b.k), Cai(b.v))
+    seqs = paged.SeqBatch(Cai(ints(b.start)), Cai(ints(b.lens)), Cai(b.table), n_rows=b.n_rows, max_rows=2)
+    out = torch.full_like(q, 77.0)
+    paged.attn_paged(ctx, kv, seqs, Cai(q), Cai(out), paged.AttnWorkspace(ctx, 4, 2, 64))
+    ctx.sync()
+    assert torch.equal(out, ref)
+
+
+def test_row_starts_that_do_not_rise_are_harmless(ctx):
+    """Rows claimed by no sequence or by a falling start are not computed; nothing is read out of range."""
+    b = Batch([3, 2], [30, 20], 16, 1, 64, torch.float16, seed=54)
+    q = b.randn(b.n_rows, 2, 64)
+    for start in ([0, 3, 1], [5, 0, 2], [-4, 3, 5], [0, 3, 10 ** 9]):
+        b.seqs._keep[0].copy_(ints(start))
+        attend(ctx, b, q)
+        x = b.randn(b.n_rows, 4, 64)
+        paged.rope_append(ctx, b.kv, b.seqs, x[:, :2], x[:, 2:3], x[:, 3:], table_of(64, 64, torch.float32),
+                          torch.empty(b.n_rows, 2, 64, device="cuda", dtype=torch.float16))
+        try:
+            ctx.sync()
+        except ALMError:
+            pass

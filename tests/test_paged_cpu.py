@@ -117,7 +117,7 @@ def test_append_refusals(kw, word):
     (dict(heads=0), "heads"), (dict(heads=5), "multiple"), (dict(heads=258), "128"), (dict(out_dev=None), "null"),
     (dict(work_dev=None), "null"), (dict(q_dev=P + 8), "aligned"), (dict(out_head=65), "stride"),
     (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(work_dev=P + 128), "256-byte"), ({}, "null ctx")])
+    (dict(scale=float("inf")), "scale"), (dict(scale=2e30), "scale"), (dict(scale=float("nan")), "scale"), (dict(work_dev=P + 128), "256-byte"), ({}, "null ctx")])
 def test_attention_refusals(kw, word):
     _refused(lib.alm_attn_paged(None, _ref(_kv()), _ref(_batch()), _ref(_attn(**kw))), word)
 
@@ -221,3 +221,18 @@ def test_python_verify_refuses(kw, err):
     a.update(kw)
     with pytest.raises(err):
         paged.verify(NoContext, **a)
+
+
+@pytest.mark.parametrize("args,pack", [
+    (RopeAppendArgs, paged._ROPE_ARGS), (AttnPagedArgs, paged._ATTN_ARGS), (VerifyArgs, paged._VERIFY_ARGS)])
+def test_packed_arguments_are_the_structs(args, pack):
+    """The calls' packed bytes fill the header's structs field by field."""
+    vals = [i + 1 if t is not ctypes.c_float else 0.5 * (i + 1) for i, (_, t) in enumerate(args._fields_)]
+    raw = pack(*vals)
+    assert len(raw) == ctypes.sizeof(args)
+    got = args.from_buffer_copy(raw)
+    assert [getattr(got, n) for n, _ in args._fields_] == vals
+
+
+def test_empty_arrays_are_contiguous():
+    assert paged._dense((2, 0), (1, 1)) and paged._dense((0, 5), (7, 1)) and not paged._dense((2, 3), (4, 1))
