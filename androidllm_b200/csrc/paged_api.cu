@@ -76,6 +76,7 @@ struct OnDevice {
   }
 };
 
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool vec8(int64_t stride) { return stride % 8 == 0; }
 
@@ -108,6 +109,8 @@ int check_batch(const alm_seq_batch* v, SeqBatch* b) {
   REQ(v->n_seq >= 0 && v->n_seq <= 4096, "n_seq must be in 0..4096");
   REQ(v->n_rows >= 0 && v->max_rows >= 0, "n_rows and max_rows must not be negative");
   REQ(v->n_seq == 0 || v->n_rows == 0 || (v->row_start_dev && v->kv_len_dev && v->page_table_dev), "null argument");
+  REQ(aligned4(v->row_start_dev) && aligned4(v->kv_len_dev) && aligned4(v->page_table_dev) && aligned4(v->slots_dev),
+      "the batch's arrays must be 4-byte aligned");
   REQ(v->table_rows >= (v->slots_dev ? 1 : v->n_seq), "the page table needs a row for every sequence");
   REQ(v->table_pages >= 0 && v->page_stride >= v->table_pages, "page_stride must be at least table_pages");
   b->n_seq = v->n_seq;
@@ -203,6 +206,7 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   REQ(v->heads >= 1 && v->heads % kv.kv_heads == 0, "heads must be a multiple of kv_heads");
   REQ(v->heads / kv.kv_heads <= 128, "at most 128 query heads may share a K/V head");
   REQ(aligned16(v->q_dev) && aligned16(v->out_dev), "tensors must be 16-byte aligned");
+  REQ(aligned4(v->lse_dev), "lse must be 4-byte aligned");
   REQ(vec8(v->q_row) && vec8(v->q_head) && vec8(v->out_row) && vec8(v->out_head),
       "row and head strides must be multiples of 8 elements");
   REQ(v->window >= 0, "window must not be negative");
@@ -255,6 +259,10 @@ ALM_API int alm_verify(alm_ctx* ctx, const alm_verify_args* v) {
   REQ(v->logits_row >= v->vocab || v->n_rows <= 1, "logits_row must be at least vocab");
   const int item = v->logits_dtype == ALM_F32 ? 4 : 2;
   REQ((reinterpret_cast<uintptr_t>(v->logits_dev) % item) == 0, "logits must be aligned to their type");
+  REQ(aligned4(v->row_start_dev) && aligned4(v->draft_tokens_dev) && aligned4(v->draft_probs_dev) &&
+          aligned4(v->temperature_dev) && aligned4(v->min_p_dev) && aligned4(v->tokens_dev) &&
+          aligned4(v->n_accepted_dev) && aligned4(v->p_draft_dev) && (reinterpret_cast<uintptr_t>(v->uniforms_dev) & 7) == 0,
+      "arrays must be aligned to their type");
   int device, n_sms, *err;
   cudaStream_t st;
   TRY(alm_internal_ctx_paged(ctx, &device, &n_sms, &st, &err));

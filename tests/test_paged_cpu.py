@@ -88,7 +88,9 @@ BAD_KV = [(dict(k_dev=None), "null"), (dict(dtype=2), "fp16 or bf16"), (dict(dty
           (dict(v_dev=P + 8), "aligned")]
 BAD_BATCH = [(dict(n_seq=-1), "n_seq"), (dict(n_seq=4097, table_rows=5000), "n_seq"), (dict(n_rows=-1), "n_rows"),
              (dict(max_rows=-1), "max_rows"), (dict(kv_len_dev=None), "null"), (dict(table_rows=1), "page table"),
-             (dict(slots_dev=P, table_rows=0), "page table"), (dict(page_stride=3), "page_stride")]
+             (dict(slots_dev=P, table_rows=0), "page table"), (dict(page_stride=3), "page_stride"),
+             (dict(row_start_dev=P + 2), "aligned"), (dict(page_table_dev=P + 1), "aligned"),
+             (dict(slots_dev=P + 2), "aligned")]
 
 
 @pytest.mark.parametrize("kw,word", BAD_KV)
@@ -117,7 +119,8 @@ def test_append_refusals(kw, word):
     (dict(heads=0), "heads"), (dict(heads=5), "multiple"), (dict(heads=258), "128"), (dict(out_dev=None), "null"),
     (dict(work_dev=None), "null"), (dict(q_dev=P + 8), "aligned"), (dict(out_head=65), "stride"),
     (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(scale=2e30), "scale"), (dict(scale=float("nan")), "scale"), (dict(work_dev=P + 128), "256-byte"), ({}, "null ctx")])
+    (dict(scale=float("inf")), "scale"), (dict(scale=2e30), "scale"), (dict(scale=float("nan")), "scale"), (dict(work_dev=P + 128), "256-byte"),
+    (dict(lse_dev=P + 2), "aligned"), ({}, "null ctx")])
 def test_attention_refusals(kw, word):
     _refused(lib.alm_attn_paged(None, _ref(_kv()), _ref(_batch()), _ref(_attn(**kw))), word)
 
@@ -127,7 +130,8 @@ def test_attention_refusals(kw, word):
     (dict(vocab=0), "vocab"), (dict(vocab=(1 << 24) + 1), "vocab"), (dict(logits_dtype=7), "type"),
     (dict(row_start_dev=None), "null"), (dict(logits_dev=None), "null"), (dict(draft_tokens_dev=None), "null"),
     (dict(uniforms_dev=None), "null"), (dict(temperature_dev=None), "null"), (dict(logits_row=99), "logits_row"),
-    (dict(logits_dev=P + 1), "aligned"), ({}, "null ctx")])
+    (dict(logits_dev=P + 1), "aligned"), (dict(uniforms_dev=P + 4), "aligned"), (dict(draft_probs_dev=P + 2), "aligned"),
+    (dict(tokens_dev=P + 2), "aligned"), ({}, "null ctx")])
 def test_verify_refusals(kw, word):
     _refused(lib.alm_verify(None, _ref(_verify(**kw))), word)
 
