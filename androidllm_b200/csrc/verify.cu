@@ -37,7 +37,7 @@ constexpr int kVerBlock = 8 * kWarp;   // entries a warp takes at a time
 constexpr double kNear = 1e-4;
 
 struct VerShared {
-  double table[64];     // 2^(i / 64)
+  double table[256 * 16];   // 2^(i / 256), 16 copies side by side
   float wm[kVerRows][kVerWarps];
   double ws[kVerRows][kVerWarps];
   int wi[kVerRows][kVerWarps];
@@ -48,11 +48,14 @@ struct VerShared {
   // rows of the whole vocabulary
   float row_m[kVerRows];
   double row_z[kVerRows];
-  int row_i[kVerRows];
+  int row_i[kVerRows];   // greedy: the maximum's place; min-p: an entry at the border
   double dsum[kVerWarps];
   double cta_d[2];      // two slots in turn: one is read while the next is written
   double cta_r[2][kVerWarps];   // the residual's sums by warp, in index order (by attempt)
   int cta_last[2];              // last index with a positive residual, or -1
+  int warp_last[kVerWarps];
+  int cta_over;                 // a lane has more than one entry at the draft's border
+  int found;
 };
 
 ALM_DEV float ex2f_(float x) {
@@ -61,126 +64,81 @@ ALM_DEV float ex2f_(float x) {
   return y;
 }
 
-// exp((l - top) / T) in 64 bits, c = 64 log2(e) / T: with t = (l - top) c =
-// n + g, n whole and |g| <= 1/2, it is 2^(n div 64) 2^((n mod 64) / 64)
-// 2^(g / 64); the middle factor comes from a table, the last from its Taylor
-// series to degree 5, whose remainder is below (ln 2 / 128)^6 / 720 = 4e-17
-// (Tang's table-driven method).  12 instructions of the 64-bit pipe, about a
-// third of the library function's.  NaN counts as -inf, +inf logits (l == top)
-// share the mass; below 2^-1000 the result is 0.
-ALM_DEV double exp64(double t, const double* table) {   // 2^(t / 64)
-  constexpr double kMagic = 6755399441055744.0;   // 1.5 * 2^52: adding it rounds to a whole number
-  constexpr double a1 = 0.693147180559945309417 / 64, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3, a4 = a3 * a1 / 4,
-                   a5 = a4 * a1 / 5;
-  // no branch: eight of these run side by side, and the 64-bit pipe's latency is long
-  const bool some = t > -64000.0;
-  const double tt = some ? t : 0.0;
-  const double r = tt + kMagic;
-  const int n = __double2loint(r);
-  const double g = tt - (r - kMagic);
-  double p = fma(g, a5, a4);
-  p = fma(g, p, a3);
-  p = fma(g, p, a2);
-  p = fma(g, p, a1);
-  p = fma(g, p, 1.0);
-  const double e = p * table[n & 63];
-  const double w = __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
-  return some ? w : 0.0;
-}
-ALM_DEV double weight64(float l, float top, double c, const double* table) {
-  const double e = exp64((static_cast<double>(l) - static_cast<double>(top)) * c, table);
-  return l == top && l > kNegInf ? 1.0 : e;
+// exp((l - top) / T) in 64 bits, c = 256 log2(e) / T: with t = (l - top) c =
+// n + g, n whole and |g| <= 0.56 (n comes from 32 bits), it is 2^(n div 256)
+// 2^((n mod 256) / 256) 2^(g / 256); the middle factor comes from a table, the
+// last from its Taylor series to degree 4, whose remainder is below
+// (0.56 ln 2 / 256)^5 / 120 = 7e-17 (Tang's table-driven method).  8
+// instructions of the 64-bit pipe and a conversion.  The table has a copy for
+// each lane of a half-warp, in banks of its own: random entries of one copy
+// cost 6 turns of the shared memory instead of 2, which bound these passes.
+// NaN counts as -inf, +inf logits (l == top) share the mass; below 2^-1000 the
+// result is 0.
+constexpr int kExpTable = 256, kExpCopies = 16;
+struct Exp64 {
+  const double* table;   // this lane's copy
+  double top_d, c;
+  float top, c_f;
+  ALM_DEV double operator()(float l) const {
+    constexpr double a1 = 0.693147180559945309417 / kExpTable, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3, a4 = a3 * a1 / 4;
+    // no branch: eight of these run side by side, and the 64-bit pipe's latency is long
+    const float tf = (l - top) * c_f;
+    const bool some = tf > -1000.f * kExpTable;
+    const int n = some ? __float_as_int(tf + 12582912.f) - 0x4b400000 : 0;   // 1.5 2^23: its last bit is 1
+    const double n_d = __hiloint2double(0x43300000, n ^ 0x80000000) - 4503601774854144.0;   // 2^52 + 2^31
+    const double g = fma(static_cast<double>(l) - top_d, c, -n_d);
+    double p = fma(g, a4, a3);
+    p = fma(g, p, a2);
+    p = fma(g, p, a1);
+    p = fma(g, p, 1.0);
+    const double e = p * table[(n & (kExpTable - 1)) * kExpCopies];
+    const double w = __hiloint2double(__double2hiint(e) + ((n >> 8) << 20), __double2loint(e));
+    return l == top ? 1.0 : some ? w : 0.0;
+  }
+};
+
+template <typename T>
+ALM_DEV float value_of(uint32_t b) {
+  if constexpr (std::is_same<T, half>::value) return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
+  else return __uint_as_float(sizeof(T) == 4 ? b : b << 16);
 }
 
-// 16-bit logits have few leading parts: l = h + r with h the value without its
-// low bits and r what they add, so exp((l - top) / T) = exp((h - top) / T)
-// exp(r / T), two table entries and one product in 64 bits instead of the 25
-// instructions above.  h has one entry per sign, exponent and leading
-// mantissa bits, r one per sign, exponent and low bits.
+// Entries j .. j + 7 of a row as they lie in memory; -inf behind the slice's end.
 template <typename T>
-struct Split {   // fp32: no tables
-  static constexpr int kHi = 0, kLo = 0;
-  ALM_DEV static int hi(uint32_t) { return 0; }
-  ALM_DEV static int lo(uint32_t) { return 0; }
-  ALM_DEV static void parts(int, float&, bool&) {}
-  ALM_DEV static double rest(int) { return 0.0; }
-};
-template <>
-struct Split<half> {   // 5 + 5 bits of the mantissa
-  static constexpr int kHi = 2048, kLo = 2048;
-  ALM_DEV static int hi(uint32_t b) { return b >> 5; }
-  ALM_DEV static int lo(uint32_t b) { return (b >> 10) << 5 | (b & 31); }
-  ALM_DEV static float value(uint32_t b) { return __half2float(__ushort_as_half(static_cast<unsigned short>(b))); }
-  ALM_DEV static void parts(int i, float& v, bool& finite) {
-    v = value(i << 5);
-    finite = (i >> 5 & 31) != 31;
+struct Raw8 {
+  uint4 x[sizeof(T) / 2];
+  ALM_DEV uint32_t word(int i) const {
+    const uint4& u = x[i / 4];
+    return i % 4 == 0 ? u.x : i % 4 == 1 ? u.y : i % 4 == 2 ? u.z : u.w;
   }
-  ALM_DEV static double rest(int i) {
-    const uint32_t se = i >> 5;
-    if ((se & 31) == 31) return 0.0;
-    return static_cast<double>(value(se << 10 | (i & 31))) - static_cast<double>(value(se << 10));
+  ALM_DEV uint32_t bits(int i) const {
+    if constexpr (sizeof(T) == 4) return word(i);
+    else return i % 2 ? word(i / 2) >> 16 : word(i / 2) & 0xffffu;
   }
 };
-template <>
-struct Split<__nv_bfloat16> {   // 3 + 4 bits of the mantissa; r for exponents 2^-63 .. 2^32
-  static constexpr int kHi = 4096, kLo = 2 * 96 * 16;
-  ALM_DEV static int hi(uint32_t b) { return b >> 4; }
-  ALM_DEV static int lo(uint32_t b) {
-    const int e = min(max(static_cast<int>(b >> 7 & 255) - 64, 0), 95);
-    return ((b >> 15) * 96 + e) << 4 | (b & 15);
-  }
-  ALM_DEV static float value(uint32_t b) { return __uint_as_float(b << 16); }
-  ALM_DEV static void parts(int i, float& v, bool& finite) {
-    v = value(i << 4);
-    finite = (i >> 3 & 255) != 255;
-  }
-  ALM_DEV static double rest(int i) {
-    const int se = i >> 4, sign = se / 96;
-    const uint32_t base = static_cast<uint32_t>(sign << 15 | (se % 96 + 64) << 7);
-    return static_cast<double>(value(base | (i & 15))) - static_cast<double>(value(base));
-  }
-};
-// Where the tables hold: both factors far from overflow, and no low bits
-// that matter outside the exponents above.  (Weights below e^-630 of the
-// largest may count as zero.)
-ALM_DEV bool tables_hold(float top, float temp) {
-  return fabsf(top) <= 2000.f * temp && temp >= 2.5e-4f && temp <= 1e4f;
-}
-
-// The bits of entries j .. j + 7 of a row; those of -inf behind the slice's end.
 template <typename T>
-ALM_DEV void load8(const T* l, int j, int end, bool vec, uint32_t (&v)[8]) {
+ALM_DEV Raw8<T> load8(const T* l, int j, int end, bool vec) {
   constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, half>::value ? 0xfc00u : 0xff80u;
+  Raw8<T> r;
   if (vec && j + 8 <= end) {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(l + j));
-    if constexpr (sizeof(T) == 4) {
-      const uint4 y = __ldg(reinterpret_cast<const uint4*>(l + j) + 1);
-      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-    } else {
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[2 * i] = w[i] & 0xffffu, v[2 * i + 1] = w[i] >> 16;
-    }
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) r.x[i] = __ldg(reinterpret_cast<const uint4*>(l + j) + i);
   } else {
+    uint32_t v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if constexpr (sizeof(T) == 4) v[i] = j + i < end ? __ldg(reinterpret_cast<const unsigned*>(l) + j + i) : kNone;
       else v[i] = j + i < end ? __ldg(reinterpret_cast<const unsigned short*>(l) + j + i) : kNone;
     }
+    if constexpr (sizeof(T) == 4) {
+      r.x[0] = make_uint4(v[0], v[1], v[2], v[3]);
+      r.x[1] = make_uint4(v[4], v[5], v[6], v[7]);
+    } else {
+      r.x[0] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    }
   }
+  return r;
 }
-template <typename T>
-ALM_DEV float value_of(uint32_t b) {
-  if constexpr (sizeof(T) == 4) return __uint_as_float(b);
-  else return Split<T>::value(b);
-}
-ALM_DEV void load8f(const float* l, int j, int end, bool vec, float (&v)[8]) {
-  uint32_t b[8];
-  load8(l, j, end, vec, b);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(b[i]);
-}
-
 ALM_DEV double warp_sum64(double z) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
@@ -210,7 +168,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
   const bool greedy = !(temp > 0.f);
   // an infinite temperature still leaves -inf (and the rest of a row with +inf) out
   const double inv_t = greedy ? 1.0 : fmax(1.0 / static_cast<double>(temp), 1e-37);
-  const double c64 = 64 * 1.4426950408889634074 * inv_t;
+  const double c64 = kExpTable * 1.4426950408889634074 * inv_t;
   const double min_p = !greedy && a.min_p ? static_cast<double>(__ldg(a.min_p + s)) : 0.0;
   int* tokens = a.tokens + static_cast<size_t>(s) * (a.k_max + 1);
   if (n_row == 0) {   // the same for the whole cluster
@@ -224,12 +182,46 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
   const int v0 = min(a.vocab, cta * width), v1 = min(a.vocab, v0 + width);
   const float k_log2 = static_cast<float>(1.4426950408889634 * inv_t);
   const bool vec = a.vec != 0;
-  if (tid < 64) sh.table[tid] = exp2(tid / 64.0);
+  if (!greedy && tid < kExpTable) {
+    const double e = exp2(tid / static_cast<double>(kExpTable));
+    for (int i = 0; i < kExpCopies; ++i) sh.table[tid * kExpCopies + (i + tid) % kExpCopies] = e;
+  }
 
   auto row_ptr = [&](int i) { return reinterpret_cast<const T*>(a.logits + (row0 + i) * a.logits_row); };
 
-  // Maximum and 32-bit sum (greedy: first place of the maximum) of every row's
-  // slice.  The rows' blocks of 256 entries form one line that the warps share.
+  // Goes through this CTA's slice of every row: the rows' blocks of 256 entries
+  // form one line that the warps share evenly, and a warp's next blocks are
+  // under way while it computes on the last ones.
+  const int n_blk = (v1 - v0 + kVerBlock - 1) / kVerBlock;
+  auto all_rows = [&](auto&& block, auto&& row_done) {
+    constexpr int kDeep = sizeof(T) == 4 ? 2 : 4;   // blocks in flight
+    const int b1 = n_row * n_blk * (warp + 1) / kVerWarps;
+    int blk = n_row * n_blk * warp / kVerWarps;
+    if (blk >= b1) return;
+    Raw8<T> now[kDeep], next[kDeep];
+    auto fetch = [&](Raw8<T> (&r)[kDeep], int blk, int i, int row_end) {
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d)
+        if (blk + d < row_end) r[d] = load8(row_ptr(i), v0 + (blk + d - i * n_blk) * kVerBlock + lane * 8, v1, vec);
+    };
+    int i = blk / n_blk, row_end = min(b1, (i + 1) * n_blk);
+    fetch(now, blk, i, row_end);
+    while (blk < b1) {
+      const bool ends = blk + kDeep >= row_end;
+      const int nb = ends ? row_end : blk + kDeep;
+      const int ni = ends ? i + 1 : i, nend = ends ? min(b1, row_end + n_blk) : row_end;
+      if (nb < b1) fetch(next, nb, ni, nend);
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d)
+        if (blk + d < row_end) block(i, v0 + (blk + d - i * n_blk) * kVerBlock + lane * 8, now[d]);
+      if (ends) row_done(i);
+      blk = nb, i = ni, row_end = nend;
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) now[d] = next[d];
+    }
+  };
+
+  // Maximum and 32-bit sum (greedy: first place of the maximum) of every row.
   for (int i = tid; i < n_row * kVerWarps; i += kVerThreads) {
     sh.wm[i / kVerWarps][i % kVerWarps] = kNegInf;
     sh.ws[i / kVerWarps][i % kVerWarps] = 0.0;
@@ -237,25 +229,13 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
   }
   __syncthreads();
   {
-    const int n_blk = (v1 - v0 + kVerBlock - 1) / kVerBlock;
-    const int b1 = n_row * n_blk * (warp + 1) / kVerWarps;
-    constexpr int kDeep = sizeof(T) == 4 ? 2 : 4;   // blocks in flight
-    for (int blk = n_row * n_blk * warp / kVerWarps; blk < b1;) {
-      const int i = blk / n_blk;
-      const int row_end = min(b1, (i + 1) * n_blk);
-      const T* l = row_ptr(i);
-      float m = kNegInf, z = 0.f;
-      int at = 0x7fffffff;
-      while (blk < row_end) {
-        uint32_t v[kDeep][8];
-#pragma unroll
-        for (int d = 0; d < kDeep; ++d)
-          load8(l, v0 + (blk + d - i * n_blk) * kVerBlock + lane * 8, blk + d < row_end ? v1 : 0, vec, v[d]);
-#pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
+    float m = kNegInf, z = 0.f;
+    int at = 0x7fffffff;
+    all_rows(
+        [&](int, int j, const Raw8<T>& v) {
           float f[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) f[q] = value_of<T>(v[d][q]);
+          for (int q = 0; q < 8; ++q) f[q] = value_of<T>(v.bits(q));
           float top = f[0];
 #pragma unroll
           for (int q = 1; q < 8; ++q) top = fmaxf(top, f[q]);   // a NaN is passed over
@@ -264,9 +244,9 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
               m = top;
 #pragma unroll
               for (int q = 7; q >= 0; --q)
-                if (f[q] == top) at = v0 + (blk + d - i * n_blk) * kVerBlock + lane * 8 + q;
+                if (f[q] == top) at = j + q;
             }
-            continue;
+            return;
           }
           if (top > m) {
             z *= ex2f_((m - top) * k_log2);
@@ -288,20 +268,18 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
               sum += !(f[q] > kNegInf) ? 0.f : f[q] == m ? 1.f : ex2f_((f[q] - m) * k_log2);
           }
           z += sum;
-        }
-        blk += kDeep;
-      }
-      blk = row_end;
-      if (greedy) {
+        },
+        [&](int i) {
+          if (greedy) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-          join_first(m, at, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, at, o));
-      }
-      const float top = warp_max(m);
-      const double zd = warp_sum(scaled(z, m, top, k_log2));
-      m = top;
-      if (lane == 0) sh.wm[i][warp] = m, sh.ws[i][warp] = zd, sh.wi[i][warp] = at;
-    }
+            for (int o = 16; o > 0; o >>= 1)
+              join_first(m, at, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, at, o));
+          }
+          const float top = warp_max(m);
+          const double zd = warp_sum(scaled(z, m, top, k_log2));
+          if (lane == 0) sh.wm[i][warp] = top, sh.ws[i][warp] = zd, sh.wi[i][warp] = at;
+          m = kNegInf, z = 0.f, at = 0x7fffffff;
+        });
   }
   __syncthreads();
   // a warp a row: the CTA's warps, then the cluster's CTAs, a lane each
@@ -335,31 +313,14 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
   }
   __syncthreads();
 
-  // 64-bit weights of row i: through the tables where they hold
-  extern __shared__ __align__(16) double tables[];
-  double *const t_hi = tables, *const t_lo = tables + Split<T>::kHi;
-  int tab_row = -1;          // the row the tables are made for
-  bool tab = false;          // ... and whether they are used
-  auto make_tables = [&](int i) {   // by the whole CTA
-    tab_row = i;
-    const float top = sh.row_m[i];
-    tab = Split<T>::kHi > 0 && tables_hold(top, temp);
-    if (!tab) return;
-    __syncthreads();         // the last row's are no longer read
-    for (int j = tid; j < Split<T>::kHi; j += kVerThreads) {
-      float v = 0.f;
-      bool finite = false;
-      Split<T>::parts(j, v, finite);
-      // (entries above the maximum are not read)
-      t_hi[j] = finite && v <= top + fabsf(top) ? exp64((static_cast<double>(v) - static_cast<double>(top)) * c64, sh.table) : 0.0;
-    }
-    for (int j = tid; j < Split<T>::kLo; j += kVerThreads) t_lo[j] = exp64(Split<T>::rest(j) * c64, sh.table);
-    __syncthreads();
+  // 64-bit weights of row i
+  auto weights = [&](int i) {
+    // (a row of nothing but -inf: no entry equals the maximum)
+    const float top = sh.row_m[i] > kNegInf ? sh.row_m[i] : __int_as_float(0x7fffffff);
+    return Exp64{sh.table + lane % kExpCopies, top, c64, top, static_cast<float>(c64)};
   };
-  auto wt = [&](uint32_t bits, float top) {   // of row tab_row
-    double e;
-    if (tab) e = t_hi[Split<T>::hi(bits)] * t_lo[Split<T>::lo(bits)];
-    else e = weight64(value_of<T>(bits), top, c64, sh.table);
+  auto wt = [&](const Exp64& w, uint32_t bits) {
+    const double e = w(value_of<T>(bits));
     return e < min_p ? 0.0 : e;
   };
   auto bits_at = [&](int i, int j) -> uint32_t {
@@ -373,10 +334,9 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
   auto cluster_sum = [&](auto&& f, const T* l) {
     double z = 0.0;
     for (int j = v0 + tid * 8; j < v1; j += kVerThreads * 8) {
-      uint32_t v[8];
-      load8(l, j, v1, vec, v);
+      const Raw8<T> v = load8(l, j, v1, vec);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) z += f(v[q]);
+      for (int q = 0; q < 8; ++q) z += f(v.bits(q));
     }
     z = warp_sum64(z);
     if (lane == 0) sh.dsum[warp] = z;
@@ -392,43 +352,39 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
     return warp_sum64(part);
   };
   auto exact_sum = [&](int i) {
-    const float top = sh.row_m[i];
-    if (tab_row != i) make_tables(i);
-    return cluster_sum([&](uint32_t v) { return wt(v, top); }, row_ptr(i));
+    const Exp64 w = weights(i);
+    return cluster_sum([&](uint32_t v) { return wt(w, v); }, row_ptr(i));
   };
   // Min-p: the 32-bit sums again without the entries below it, now that the
-  // maxima are known.  row_i tells whether an entry lies too near the border.
+  // maxima are known.  row_i then tells whether an entry lies too near the border.
   if (min_p > 0.0) {
-    const float cut = static_cast<float>(min_p), lo = cut * (1.f - 1e-4f), hi = cut * (1.f + 1e-4f);
-    const int n_blk = (v1 - v0 + kVerBlock - 1) / kVerBlock;
-    const int b1 = n_row * n_blk * (warp + 1) / kVerWarps;
+    // the 32-bit weights' error at the border, threefold: 1.3e-7 a unit of log2, and 3e-7
+    const float cut = static_cast<float>(min_p), band = cut * 1e-6f * (1.f + fabsf(log2f(cut)));
+    const float lo = cut - band, hi = cut + band;
     for (int i = tid; i < n_row * kVerWarps; i += kVerThreads) {
       sh.ws[i / kVerWarps][i % kVerWarps] = 0.0;
       sh.wi[i / kVerWarps][i % kVerWarps] = 0;
     }
     __syncthreads();
-    for (int blk = n_row * n_blk * warp / kVerWarps; blk < b1;) {
-      const int i = blk / n_blk, row_end = min(b1, (i + 1) * n_blk);
-      const T* l = row_ptr(i);
-      const float top = sh.row_m[i];
-      float z = 0.f;
-      bool near = false;
-#pragma unroll 4
-      for (; blk < row_end; ++blk) {
-        uint32_t v[8];
-        load8(l, v0 + (blk - i * n_blk) * kVerBlock + lane * 8, v1, vec, v);
+    float z = 0.f;
+    bool near = false;
+    all_rows(
+        [&](int i, int, const Raw8<T>& v) {
+          const float top = sh.row_m[i];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float f = value_of<T>(v[q]);
-          const float e = !(f > kNegInf) ? 0.f : f == top ? 1.f : ex2f_((f - top) * k_log2);
-          near |= e >= lo && e <= hi;
-          z += e < cut ? 0.f : e;
-        }
-      }
-      const double zd = warp_sum64(z);
-      near = __any_sync(0xffffffffu, near);
-      if (lane == 0) sh.ws[i][warp] = zd, sh.wi[i][warp] = near;
-    }
+          for (int q = 0; q < 8; ++q) {
+            const float f = value_of<T>(v.bits(q));
+            const float e = !(f > kNegInf) ? 0.f : f == top ? 1.f : ex2f_((f - top) * k_log2);
+            near |= e >= lo && e <= hi;
+            z += e < cut ? 0.f : e;
+          }
+        },
+        [&](int i) {
+          const double zd = warp_sum(z);
+          near = __any_sync(0xffffffffu, near);
+          if (lane == 0) sh.ws[i][warp] = zd, sh.wi[i][warp] = near;
+          z = 0.f, near = false;
+        });
     cl.sync();       // (the CTA's barrier too; the first sums have been read)
     for (int i = warp; i < n_row; i += kVerWarps) {
       const double z = warp_sum64(lane < kVerWarps ? sh.ws[i][lane] : 0.0);
@@ -462,8 +418,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
       if (greedy) {
         p = in && top > kNegInf && xi == sh.row_i[lane] ? 1.0 : 0.0;
       } else {
-        double e = in ? weight64(value_of<T>(bits_at(lane, xi)), top, c64, sh.table) : 0.0;
-        if (e < min_p) e = 0.0;
+        const double e = in && top > kNegInf ? wt(weights(lane), bits_at(lane, xi)) : 0.0;
         const double q =
             !a.q ? 1.0 : in ? static_cast<double>(__ldg(a.q + s * a.q_seq + lane * a.q_step + xi)) : 0.0;
         uq = __ldg(a.u + static_cast<size_t>(s) * (a.k_max + 1) + lane) * q;
@@ -479,7 +434,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
         const double zx = exact_sum(acc);
         bool ok = false;
         if (lane == acc) {
-          const double e = in ? wt(bits_at(acc, xi), sh.row_m[acc]) : 0.0;   // by the sum's own weights
+          const double e = in ? wt(weights(acc), bits_at(acc, xi)) : 0.0;
           z = zx;
           p = e > 0.0 ? e / zx : 0.0;
           ok = uq < p;
@@ -495,7 +450,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
       if (min_p > 0.0 && sh.row_i[i] != 0 && !greedy) {
         const double zx = exact_sum(i);
         if (lane == i) {
-          const double e = in ? wt(bits_at(i, xi), sh.row_m[i]) : 0.0;
+          const double e = in ? wt(weights(i), bits_at(i, xi)) : 0.0;
           p = e > 0.0 ? e / zx : 0.0;
         }
       }
@@ -514,9 +469,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
   if (greedy || !(top > kNegInf)) {
     if (cta == 0 && tid == 0) tokens[acc] = top > kNegInf ? sh.row_i[acc] : -1;
   } else {
-    const double z = have_z ? z_stop : exact_sum(acc);
-    if (tab_row != acc) make_tables(acc);
-    const double inv_z = 1.0 / z;
+    const Exp64 weight = weights(acc);
     const T* l = row_ptr(acc);
     const float* q = a.q && acc < k ? a.q + s * a.q_seq + acc * a.q_step : nullptr;
     const bool q_vec = q && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
@@ -525,31 +478,95 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
     // a warp owns a run of entries; the runs of all warps and CTAs are in index order
     const int run = ((width + kVerWarps - 1) / kVerWarps + kVerBlock - 1) / kVerBlock * kVerBlock;
     const int j0 = min(v1, v0 + warp * run), j1 = min(v1, j0 + run);
-    for (int use_q = 1; use_q >= 0; --use_q) {
-      // what a lane's 8 entries leave after the draft's share
-      auto rest8 = [&](int j, double (&r)[8]) {
-        uint32_t v[8];
-        float w[8];
-        load8(l, j, j1, vec, v);
-        if (use_q && q) load8f(q, j, j1, q_vec, w);
+    // One pass finds Z and the residual sums: with z the 32-bit sum and P the
+    // entries with e > q z,
+    //   sum over P of (e / Z - q) = (D - (Z - z) B) / Z,  D = sum of e - q z, B = sum of q,
+    // since no entry changes sides between z and Z but those within 2^-15 e of
+    // the border; a lane keeps one of these for afterwards.  A lane with two, or
+    // a z further from Z than that allows, and the sums are made again from Z.
+    double z = z_stop, rest = 0.0;
+    int rest_last = -1;
+    bool fused = false;
+    if (!have_z) {
+      if (q)   // its first use: all of the warp's lines at once
+        for (int j = j0 + lane * 32; j < j1; j += kWarp * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + j));
+      const double zs = sh.row_z[acc];
+      double zl = 0.0, part = 0.0;
+      int border = -1;
+      bool over = false;
+      for (int j = j0 + lane * 8; j < j1; j += kVerBlock) {
+        const Raw8<T> v = load8(l, j, j1, vec);
+        Raw8<float> w;
+        if (q) w = load8(q, j, j1, q_vec);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          double e = wt(v[i], top) * inv_z;
+          const double e = wt(weight, v.bits(i));
+          zl += e;
+          if (q) {
+            const double wd = static_cast<double>(value_of<float>(w.bits(i))), d = fma(-wd, zs, e);
+            const bool near = (__double2hiint(d) & 0x7fffffff) < __double2hiint(e) - (15 << 20);
+            const bool in = !near && d > 0.0 && j + i < j1;
+            over |= near && border >= 0;
+            border = near ? j + i : border;
+            rest += in ? d : 0.0;
+            part += in ? wd : 0.0;
+            rest_last = in ? j + i : rest_last;
+          } else if (e > 0.0 && j + i != drop) {
+            rest += e;
+            rest_last = j + i;
+          }
+        }
+      }
+      double t = warp_sum64(zl);
+      if (tid == 0) sh.cta_over = 0;
+      __syncthreads();
+      if (lane == 0) sh.dsum[warp] = t;
+      if (over) sh.cta_over = 1;
+      __syncthreads();
+      if (warp == 0) {
+        t = warp_sum64(lane < kVerWarps ? sh.dsum[lane] : 0.0);
+        if (lane == 0) sh.cta_d[turn] = t;
+      }
+      cl.sync();
+      const VerShared* o = cl.map_shared_rank(&sh, min(lane, n_cta - 1));
+      z = warp_sum64(lane < n_cta ? o->cta_d[turn] : 0.0);
+      fused = !__any_sync(0xffffffffu, o->cta_over) && fabs(z - zs) <= 1e-5 * z;
+      turn ^= 1;
+      rest = fmax(rest - (z - zs) * part, 0.0) / z;
+      if (border >= 0) {
+        const double r = wt(weight, bits_at(acc, border)) / z - static_cast<double>(__ldg(q + border));
+        if (r > 0.0) {
+          rest += r;
+          rest_last = max(rest_last, border);
+        }
+      }
+    }
+    const double inv_z = 1.0 / z;
+    for (int use_q = 1; use_q >= 0; --use_q) {
+      // what entries j .. j + 7, of those below end, leave after the draft's share
+      auto rest8 = [&](int j, int end, double (&r)[8]) {
+        const Raw8<T> v = load8(l, j, end, vec);
+        Raw8<float> w;
+        if (use_q && q) w = load8(q, j, end, q_vec);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          double e = wt(weight, v.bits(i)) * inv_z;
           if (use_q && q) {
             // (a NaN or infinite share leaves nothing)
-            e = fmax(e - static_cast<double>(w[i]), 0.0);
-            if (j + i >= j1) e = 0.0;
+            e = fmax(e - static_cast<double>(value_of<float>(w.bits(i))), 0.0);
+            if (j + i >= end) e = 0.0;
           } else if (use_q && j + i == drop) {
             e = 0.0;
           }
           r[i] = e;
         }
       };
-      double sum = 0.0;
-      int last = -1;
-      for (int j = j0 + lane * 8; j < j1; j += kVerBlock) {
+      const bool done = use_q && fused;
+      double sum = done ? rest : 0.0;
+      int last = done ? rest_last : -1;
+      for (int j = done ? j1 : j0 + lane * 8; j < j1; j += kVerBlock) {
         double r[8];
-        rest8(j, r);
+        rest8(j, j1, r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           sum += r[i];
@@ -565,6 +582,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
       __syncthreads();
       if (lane == 0) {
         sh.dsum[warp] = sum;
+        sh.warp_last[warp] = last;
         if (last >= 0) atomicMax(&sh.cta_last[use_q], last);
       }
       __syncthreads();
@@ -585,17 +603,20 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
         if (c == cta) base = total;
         total += __shfl_sync(0xffffffffu, cta_sum, c);
       }
-      const double before = warp > 0 ? base + sh.cta_r[use_q][warp - 1] : base;
-      const double end = base + sh.cta_r[use_q][warp];
       if (total > 0.0 || use_q == 0) {
-        // the one warp whose run the goal lies in
         const double goal = u * total;
-        if (before <= goal && end > goal) {
-          double at = before;
-          int found = -1;
-          for (int b = j0; b < j1 && found < 0; b += kVerBlock) {
+        const double* run_end = sh.cta_r[use_q];
+        if (base <= goal && base + run_end[kVerWarps - 1] > goal) {   // in this CTA's slice: all its warps look for it
+          int of = 0;   // the warp whose run the goal lies in
+          while (!(base + run_end[of] > goal)) ++of;
+          double at = of > 0 ? base + run_end[of - 1] : base;
+          const int a0 = min(v1, v0 + of * run), a1 = min(v1, a0 + run);
+          if (tid == 0) sh.found = 0x7fffffff;
+          bool found = false;
+          for (int b = a0; b < a1 && !found; b += kVerBlock * kVerWarps) {
             double r[8];
-            rest8(b + lane * 8, r);
+            const int j = b + warp * kVerBlock + lane * 8;
+            rest8(j, a1, r);
             double mine = 0.0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) mine += r[i];
@@ -605,19 +626,27 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
               const double y = __shfl_up_sync(0xffffffffu, scan, o);
               if (lane >= o) scan += y;
             }
-            double run_sum = at + (scan - mine);
-            int hit = -1;
+            __syncthreads();   // the last round's sums have been read
+            if (lane == kWarp - 1) sh.dsum[warp] = scan;
+            __syncthreads();
+            double run_sum = at;
+            for (int w = 0; w < kVerWarps; ++w) {
+              if (w == warp) run_sum = at + (scan - mine);
+              at += sh.dsum[w];
+            }
+            int hit = 0x7fffffff;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               run_sum += r[i];
-              if (hit < 0 && r[i] > 0.0 && run_sum > goal) hit = b + lane * 8 + i;
+              if (hit == 0x7fffffff && r[i] > 0.0 && run_sum > goal) hit = j + i;
             }
-            const unsigned any = __ballot_sync(0xffffffffu, hit >= 0);
-            if (any) found = __shfl_sync(0xffffffffu, hit, __ffs(any) - 1);
-            at += __shfl_sync(0xffffffffu, scan, kWarp - 1);
+            hit = __reduce_min_sync(0xffffffffu, hit);
+            if (lane == 0 && hit != 0x7fffffff) atomicMin(&sh.found, hit);
+            __syncthreads();
+            found = sh.found != 0x7fffffff;
           }
           // rounding can leave the walk's end just short of the run's sum
-          if (lane == 0) tokens[acc] = found >= 0 ? found : last;
+          if (tid == 0) tokens[acc] = found ? sh.found : sh.warp_last[of];
         }
         // a draw of 1, or rounding at the row's end: the last entry with mass
         if (!(total > goal) && cta == 0 && tid == 0) tokens[acc] = row_last;
@@ -629,16 +658,11 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
 }
 
 template <typename T>
-constexpr int table_bytes() {
-  return (Split<T>::kHi + Split<T>::kLo) * static_cast<int>(sizeof(double));
-}
-
-template <typename T>
 cudaError_t launch_t(const Verify& a, cudaStream_t st) {
   // few sequences: 16 CTAs each, so that a row's slices stay short; many: 8
   // (the portable size, which more GPCs can place)
   const int ctas = a.n_seq <= 8 ? 16 : 8;
-  OpLaunch l(dim3(a.n_seq * ctas, 1, 1), kVerThreads, table_bytes<T>(), st, ctas);
+  OpLaunch l(dim3(a.n_seq * ctas, 1, 1), kVerThreads, 0, st, ctas);
   return cudaLaunchKernelEx(&l.cfg, verify_kernel<T>, a);
 }
 
@@ -646,10 +670,7 @@ cudaError_t launch_t(const Verify& a, cudaStream_t st) {
 
 template <typename T>
 static cudaError_t verify_attrs_t() {
-  cudaError_t e = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, table_bytes<T>());
-  return e;
+  return cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 cudaError_t verify_init_attrs() {
   cudaError_t e = verify_attrs_t<half>();
