@@ -72,28 +72,43 @@ ALM_DEV float ex2f_(float x) {
 // instructions of the 64-bit pipe and a conversion.  The table has a copy for
 // each lane of a half-warp, in banks of its own: random entries of one copy
 // cost 6 turns of the shared memory instead of 2, which bound these passes.
-// NaN counts as -inf, +inf logits (l == top) share the mass; below 2^-1000 the
-// result is 0.
+// NaN counts as -inf, +inf logits (l == top) share the mass.  An entry below
+// `least` (min-p, 2^-999 if there is none) weighs 0.
+//
+// kPlain: the maximum and `low`, the logit that weighs 2^-1000, are finite
+// numbers: -inf and NaN are raised to `low`, which takes 9 instructions fewer
+// than telling them apart (the 64-bit passes are bound by the issue of their
+// instructions).  The two forms agree in every bit.
 constexpr int kExpTable = 256, kExpCopies = 16;
+template <bool kPlain>
 struct Exp64 {
   const double* table;   // this lane's copy
-  double top_d, c;
-  float top, c_f;
+  double top_d, c, least;
+  float top, c_f, low;
   ALM_DEV double operator()(float l) const {
     constexpr double a1 = 0.693147180559945309417 / kExpTable, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3, a4 = a3 * a1 / 4;
     // no branch: eight of these run side by side, and the 64-bit pipe's latency is long
-    const float tf = (l - top) * c_f;
-    const bool some = tf > -1000.f * kExpTable;
-    const int n = some ? __float_as_int(tf + 12582912.f) - 0x4b400000 : 0;   // 1.5 2^23: its last bit is 1
-    const double n_d = __hiloint2double(0x43300000, n ^ 0x80000000) - 4503601774854144.0;   // 2^52 + 2^31
-    const double g = fma(static_cast<double>(l) - top_d, c, -n_d);
+    bool some = true;
+    if (kPlain) {
+      l = fmaxf(l, low);
+    } else {
+      some = (l - top) * c_f > -1000.f * kExpTable;
+      if (l == top) some = l > kNegInf;
+    }
+    float x = l - top;
+    if (!kPlain && (!some || l == top)) x = 0.f;
+    const int n = __float_as_int(fmaf(x, c_f, 12582912.f));   // 1.5 2^23, whose last bit is 1: n + 0x4b400000
+    const double n_d = __hiloint2double(0x43300000, n + 0x34c00000) - 4503601774854144.0;   // 2^52 + 2^31
+    double d = static_cast<double>(l) - top_d;
+    if (!kPlain && l == top) d = 0.0;
+    const double g = fma(d, c, -n_d);
     double p = fma(g, a4, a3);
     p = fma(g, p, a2);
     p = fma(g, p, a1);
     p = fma(g, p, 1.0);
     const double e = p * table[(n & (kExpTable - 1)) * kExpCopies];
-    const double w = __hiloint2double(__double2hiint(e) + ((n >> 8) << 20), __double2loint(e));
-    return l == top ? 1.0 : some ? w : 0.0;
+    const double w = __hiloint2double(__double2hiint(e) + ((n & 0xfff00) << 12), __double2loint(e));
+    return !(w >= least) || !some ? 0.0 : w;
   }
 };
 
@@ -103,7 +118,7 @@ ALM_DEV float value_of(uint32_t b) {
   else return __uint_as_float(sizeof(T) == 4 ? b : b << 16);
 }
 
-// Entries j .. j + 7 of a row as they lie in memory; -inf behind the slice's end.
+// Entries j .. j + 7 of a row as they lie in memory; -inf (`fill`) behind the slice's end.
 template <typename T>
 struct Raw8 {
   uint4 x[sizeof(T) / 2];
@@ -117,8 +132,9 @@ struct Raw8 {
   }
 };
 template <typename T>
-ALM_DEV Raw8<T> load8(const T* l, int j, int end, bool vec) {
-  constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, half>::value ? 0xfc00u : 0xff80u;
+constexpr uint32_t neg_inf() { return sizeof(T) == 4 ? 0xff800000u : std::is_same<T, half>::value ? 0xfc00u : 0xff80u; }
+template <typename T>
+ALM_DEV Raw8<T> load8(const T* l, int j, int end, bool vec, uint32_t fill = neg_inf<T>()) {
   Raw8<T> r;
   if (vec && j + 8 <= end) {
 #pragma unroll
@@ -127,8 +143,8 @@ ALM_DEV Raw8<T> load8(const T* l, int j, int end, bool vec) {
     uint32_t v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if constexpr (sizeof(T) == 4) v[i] = j + i < end ? __ldg(reinterpret_cast<const unsigned*>(l) + j + i) : kNone;
-      else v[i] = j + i < end ? __ldg(reinterpret_cast<const unsigned short*>(l) + j + i) : kNone;
+      if constexpr (sizeof(T) == 4) v[i] = j + i < end ? __ldg(reinterpret_cast<const unsigned*>(l) + j + i) : fill;
+      else v[i] = j + i < end ? __ldg(reinterpret_cast<const unsigned short*>(l) + j + i) : fill;
     }
     if constexpr (sizeof(T) == 4) {
       r.x[0] = make_uint4(v[0], v[1], v[2], v[3]);
@@ -313,15 +329,17 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
   }
   __syncthreads();
 
-  // 64-bit weights of row i
-  auto weights = [&](int i) {
-    // (a row of nothing but -inf: no entry equals the maximum)
-    const float top = sh.row_m[i] > kNegInf ? sh.row_m[i] : __int_as_float(0x7fffffff);
-    return Exp64{sh.table + lane % kExpCopies, top, c64, top, static_cast<float>(c64)};
+  // 64-bit weights of row i, and f called with them in the form that holds
+  const float c_f = fminf(static_cast<float>(c64), 1e38f);
+  const double least = fmax(min_p, 0x1p-999);
+  auto weights = [&](int i, auto plain) {
+    const float top = sh.row_m[i];
+    return Exp64<decltype(plain)::value>{sh.table + lane % kExpCopies, top, c64, least, top, c_f,
+                                         top - 1000.f * kExpTable / c_f};
   };
-  auto wt = [&](const Exp64& w, uint32_t bits) {
-    const double e = w(value_of<T>(bits));
-    return e < min_p ? 0.0 : e;
+  auto with_weights = [&](int i, auto&& f) {
+    if (fabsf(sh.row_m[i]) + 1000.f * kExpTable / c_f < 1e38f && c_f < 1e30f) f(weights(i, std::true_type()));
+    else f(weights(i, std::false_type()));
   };
   auto bits_at = [&](int i, int j) -> uint32_t {
     if constexpr (sizeof(T) == 4) return __ldg(reinterpret_cast<const unsigned*>(row_ptr(i)) + j);
@@ -352,15 +370,17 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
     return warp_sum64(part);
   };
   auto exact_sum = [&](int i) {
-    const Exp64 w = weights(i);
-    return cluster_sum([&](uint32_t v) { return wt(w, v); }, row_ptr(i));
+    double z = 0.0;
+    with_weights(i, [&](const auto& w) {
+      z = cluster_sum([&](uint32_t v) { return w(value_of<T>(v)); }, row_ptr(i));
+    });
+    return z;
   };
   // Min-p: the 32-bit sums again without the entries below it, now that the
   // maxima are known.  row_i then tells whether an entry lies too near the border.
   if (min_p > 0.0) {
     // the 32-bit weights' error at the border, threefold: 1.3e-7 a unit of log2, and 3e-7
     const float cut = static_cast<float>(min_p), band = cut * 1e-6f * (1.f + fabsf(log2f(cut)));
-    const float lo = cut - band, hi = cut + band;
     for (int i = tid; i < n_row * kVerWarps; i += kVerThreads) {
       sh.ws[i / kVerWarps][i % kVerWarps] = 0.0;
       sh.wi[i / kVerWarps][i % kVerWarps] = 0;
@@ -371,12 +391,13 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
     all_rows(
         [&](int i, int, const Raw8<T>& v) {
           const float top = sh.row_m[i];
+          const bool inf = !(top < -kNegInf);
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const float f = value_of<T>(v.bits(q));
-            const float e = !(f > kNegInf) ? 0.f : f == top ? 1.f : ex2f_((f - top) * k_log2);
-            near |= e >= lo && e <= hi;
-            z += e < cut ? 0.f : e;
+            const float e = inf && f == top ? 1.f : ex2f_((f - top) * k_log2);   // NaN: below every bound
+            near |= fabsf(e - cut) <= band;
+            z += e >= cut ? e : 0.f;
           }
         },
         [&](int i) {
@@ -418,7 +439,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
       if (greedy) {
         p = in && top > kNegInf && xi == sh.row_i[lane] ? 1.0 : 0.0;
       } else {
-        const double e = in && top > kNegInf ? wt(weights(lane), bits_at(lane, xi)) : 0.0;
+        const double e = in && top > kNegInf ? weights(lane, std::false_type())(value_of<T>(bits_at(lane, xi))) : 0.0;
         const double q =
             !a.q ? 1.0 : in ? static_cast<double>(__ldg(a.q + s * a.q_seq + lane * a.q_step + xi)) : 0.0;
         uq = __ldg(a.u + static_cast<size_t>(s) * (a.k_max + 1) + lane) * q;
@@ -434,7 +455,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
         const double zx = exact_sum(acc);
         bool ok = false;
         if (lane == acc) {
-          const double e = in ? wt(weights(acc), bits_at(acc, xi)) : 0.0;
+          const double e = in ? weights(acc, std::false_type())(value_of<T>(bits_at(acc, xi))) : 0.0;
           z = zx;
           p = e > 0.0 ? e / zx : 0.0;
           ok = uq < p;
@@ -450,7 +471,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
       if (min_p > 0.0 && sh.row_i[i] != 0 && !greedy) {
         const double zx = exact_sum(i);
         if (lane == i) {
-          const double e = in ? wt(weights(i), bits_at(i, xi)) : 0.0;
+          const double e = in ? weights(i, std::false_type())(value_of<T>(bits_at(i, xi))) : 0.0;
           p = e > 0.0 ? e / zx : 0.0;
         }
       }
@@ -469,7 +490,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
   if (greedy || !(top > kNegInf)) {
     if (cta == 0 && tid == 0) tokens[acc] = top > kNegInf ? sh.row_i[acc] : -1;
   } else {
-    const Exp64 weight = weights(acc);
+    with_weights(acc, [&](const auto& weight) {
     const T* l = row_ptr(acc);
     const float* q = a.q && acc < k ? a.q + s * a.q_seq + acc * a.q_step : nullptr;
     const bool q_vec = q && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
@@ -497,24 +518,29 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
       for (int j = j0 + lane * 8; j < j1; j += kVerBlock) {
         const Raw8<T> v = load8(l, j, j1, vec);
         Raw8<float> w;
-        if (q) w = load8(q, j, j1, q_vec);
+        if (q) w = load8(q, j, j1, q_vec, 0u);
+        unsigned close = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const double e = wt(weight, v.bits(i));
+          const double e = weight(value_of<T>(v.bits(i)));
           zl += e;
           if (q) {
             const double wd = static_cast<double>(value_of<float>(w.bits(i))), d = fma(-wd, zs, e);
             const bool near = (__double2hiint(d) & 0x7fffffff) < __double2hiint(e) - (15 << 20);
-            const bool in = !near && d > 0.0 && j + i < j1;
-            over |= near && border >= 0;
-            border = near ? j + i : border;
-            rest += in ? d : 0.0;
-            part += in ? wd : 0.0;
-            rest_last = in ? j + i : rest_last;
+            if (near) close |= 1u << i;
+            if (!near && d > 0.0) {
+              rest += d;
+              part += wd;
+              rest_last = j + i;
+            }
           } else if (e > 0.0 && j + i != drop) {
             rest += e;
             rest_last = j + i;
           }
+        }
+        if (close) {
+          over |= border >= 0 || (close & (close - 1));
+          border = j + __ffs(close) - 1;
         }
       }
       double t = warp_sum64(zl);
@@ -534,7 +560,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
       turn ^= 1;
       rest = fmax(rest - (z - zs) * part, 0.0) / z;
       if (border >= 0) {
-        const double r = wt(weight, bits_at(acc, border)) / z - static_cast<double>(__ldg(q + border));
+        const double r = weight(value_of<T>(bits_at(acc, border))) / z - static_cast<double>(__ldg(q + border));
         if (r > 0.0) {
           rest += r;
           rest_last = max(rest_last, border);
@@ -547,14 +573,13 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
       auto rest8 = [&](int j, int end, double (&r)[8]) {
         const Raw8<T> v = load8(l, j, end, vec);
         Raw8<float> w;
-        if (use_q && q) w = load8(q, j, end, q_vec);
+        if (use_q && q) w = load8(q, j, end, q_vec, 0u);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          double e = wt(weight, v.bits(i)) * inv_z;
+          double e = weight(value_of<T>(v.bits(i))) * inv_z;
           if (use_q && q) {
             // (a NaN or infinite share leaves nothing)
             e = fmax(e - static_cast<double>(value_of<float>(w.bits(i))), 0.0);
-            if (j + i >= end) e = 0.0;
           } else if (use_q && j + i == drop) {
             e = 0.0;
           }
@@ -653,6 +678,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
         break;
       }
     }
+    });
   }
   cl.sync();   // no CTA leaves while another reads its shared memory
 }
