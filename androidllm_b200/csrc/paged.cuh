@@ -148,6 +148,7 @@ struct Verify {
   int* tokens;
   int* n_accepted;
   float* p_draft;
+  int n_sms;
 };
 
 // dtype: ALM_F16 / ALM_BF16 / ALM_F32

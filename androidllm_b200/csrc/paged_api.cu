@@ -282,6 +282,7 @@ ALM_API int alm_verify(alm_ctx* ctx, const alm_verify_args* v) {
   a.tokens = v->tokens_dev;
   a.n_accepted = v->n_accepted_dev;
   a.p_draft = v->p_draft_dev;
+  a.n_sms = n_sms;
   OnDevice on(device);
   return cuda_status(launch_verify(a, v->logits_dtype, st), "verify");
 }

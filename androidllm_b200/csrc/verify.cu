@@ -168,8 +168,12 @@ ALM_DEV void join_first(float& m, int& at, float om, int oi) {
   m = fmaxf(m, om);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) {
+// kPerSm: CTAs an SM holds at once.  Two hide latency where there are more CTAs
+// than SMs (64 sequences: 74 us against 98 us with one); one leaves a thread
+// 128 registers, which serves fewer CTAs better (1 x 4: 21.9 against 23.2 us,
+// 13 x 1-7: 17.0 against 17.6 us).
+template <typename T, int kPerSm>
+__global__ void __launch_bounds__(kVerThreads, kPerSm) verify_kernel(const Verify a) {
   cg::cluster_group cl = cg::this_cluster();
   __shared__ VerShared sh;
   grid_dep_wait();
@@ -686,17 +690,21 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const Verify a) 
 template <typename T>
 cudaError_t launch_t(const Verify& a, cudaStream_t st) {
   // few sequences: 16 CTAs each, so that a row's slices stay short; many: 8
-  // (the portable size, which more GPCs can place)
+  // (the portable size, which more GPCs can place; 64 sequences: 74 us, with 4
+  // 78 us)
   const int ctas = a.n_seq <= 8 ? 16 : 8;
   OpLaunch l(dim3(a.n_seq * ctas, 1, 1), kVerThreads, 0, st, ctas);
-  return cudaLaunchKernelEx(&l.cfg, verify_kernel<T>, a);
+  return a.n_seq * ctas <= a.n_sms ? cudaLaunchKernelEx(&l.cfg, verify_kernel<T, 1>, a)
+                                   : cudaLaunchKernelEx(&l.cfg, verify_kernel<T, 2>, a);
 }
 
 }  // namespace
 
 template <typename T>
 static cudaError_t verify_attrs_t() {
-  return cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  const cudaError_t e = cudaFuncSetAttribute(verify_kernel<T, 1>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e != cudaSuccess
+             ? e : cudaFuncSetAttribute(verify_kernel<T, 2>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 cudaError_t verify_init_attrs() {
   cudaError_t e = verify_attrs_t<half>();

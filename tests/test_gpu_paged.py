@@ -569,6 +569,7 @@ def weights(l, t, mp):
         return np.zeros(l.size)
     with np.errstate(invalid="ignore"):
         e = np.where(l == top, 1.0, np.exp((l - top) / float(t)))
+    e[l < top] = np.where(np.isinf(l[l < top]) | np.isinf(top), 0.0, e[l < top])   # left out at T = inf too
     e[e < float(mp)] = 0
     return e
 
@@ -1042,3 +1043,33 @@ def test_row_starts_that_do_not_rise_are_harmless(ctx):
             ctx.sync()
         except ALMError:
             pass
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("n_seq", [5, 40])          # CTAs fewer and more than SMs
+def test_verify_infinities_at_every_temperature(ctx, dtype, n_seq):
+    rng, start, lg, draft, q, u = verify_case(70, [2] * n_seq, 2, 600)
+    lg[3:6, 5::7] = -np.inf
+    lg[6:9, [4, 90]] = np.inf
+    lg[7, 91] = np.nan
+    lg[9:12] = -np.inf
+    u[3] = 0.0
+    logits = torch.tensor(lg, device="cuda").to(DT[dtype])
+    for temp in (1e-36, 1e-3, 1.0, 1e33, np.inf):
+        for min_p in (0.0, 0.3, 1.0):
+            check_verify(ctx, start, logits, draft, q, u, np.full(n_seq, temp), np.full(n_seq, min_p))
+
+
+@pytest.mark.parametrize("noise", [1e-6, 1e-5, 1e-4, 1e-3])
+def test_verify_drafts_close_to_the_model(ctx, noise):
+    """q off p by factors of 1 +- noise: many entries at the residual's border, then some, then few."""
+    rng = np.random.default_rng(71)
+    n_seq, k, vocab = 24, 2, 20011
+    start = np.arange(n_seq + 1) * (k + 1)
+    lg = torch.tensor(rng.standard_normal((n_seq * (k + 1), vocab)) * 2, device="cuda").half()
+    p = torch.softmax(lg.double(), -1).view(n_seq, k + 1, vocab)[:, :k].cpu().numpy()
+    q = (p * (1 + noise * rng.standard_normal(p.shape))).astype(np.float32)
+    draft = rng.integers(0, vocab, (n_seq, k))
+    u = rng.random((n_seq, k + 1))
+    u[:, :k] = 1.0 + 1e-2                    # refuse at once: the residual decides
+    check_verify(ctx, start, lg, draft, q, u, np.ones(n_seq), None)
