@@ -11,13 +11,19 @@
 // exponentials (relative error below 1e-5: at most 6e-8 of |x| <= 104 from the
 // product and the instruction's 2^-22 per term), which decides all but the
 // comparisons within kNear of equality; those, and the row the token is drawn
-// from, sum Z again in 64 bits, with a table-driven exponential (below).
+// from, sum Z again with 64-bit weights.
 //
-// HBM bounds large batches (every row's logits once; the drawn row again from
-// L2), latency small ones: the CTAs of a cluster own consecutive slices of
-// the vocabulary and exchange maxima and sums through distributed shared
-// memory.  A lane takes 8 consecutive entries at a time, a warp 256, so that
-// a draw is found by one scan over the warps' sums and one over a warp's lanes.
+// The CTAs of a cluster own consecutive slices of the vocabulary and exchange
+// maxima and sums through distributed shared memory.  A lane takes 8
+// consecutive entries at a time, a warp 256, so that a draw is found by one
+// scan over the warps' sums and one over blocks of 256.
+//
+// Every row's logits come from HBM once, the drawn row's again from L2; at 64 x
+// 0-4 drafts of 151936 tokens that would be 12 us.  It takes 72 us (1 TB/s):
+// the serial steps inside a cluster (50 us: a pass over 1 to 5 rows, 3-9 us;
+// their join, 2 us; min-p again over all rows, 2-9 us; the 64-bit pass, 9 us;
+// the draw, 5 us) run on 36 clusters at a time, in two waves.  One session's
+// 4 drafts take 22 us, five barriers across the cluster and the passes' latency.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -208,6 +214,12 @@ __global__ void __launch_bounds__(kVerThreads, kPerSm) verify_kernel(const Verif
   }
 
   auto row_ptr = [&](int i) { return reinterpret_cast<const T*>(a.logits + (row0 + i) * a.logits_row); };
+
+  // the drafted tokens, one a lane; their draft probabilities are fetched meanwhile
+  const int* x = a.draft + static_cast<size_t>(s) * a.k_max;
+  const int xi = lane < k ? __ldg(x + lane) : -1;
+  auto qx = [&] { return a.q + s * a.q_seq + lane * a.q_step + xi; };
+  if (a.q && xi >= 0 && xi < a.vocab && warp == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(qx()));
 
   // Goes through this CTA's slice of every row: the rows' blocks of 256 entries
   // form one line that the warps share evenly, and a warp's next blocks are
@@ -428,24 +440,21 @@ __global__ void __launch_bounds__(kVerThreads, kPerSm) verify_kernel(const Verif
 
   // Acceptance: lane i weighs token i (every warp alike), then the tokens are
   // gone through in order; what the 32-bit sums leave open is summed in 64 bits.
-  const int* x = a.draft + static_cast<size_t>(s) * a.k_max;
   int acc = 0;
   double z_stop = 0.0;
   bool have_z = false;
   {
     double p = 0.0, uq = 0.0, z = 0.0;
-    int xi = -1;
-    bool in = false, open = false;   // open: not decided by the 32-bit sum
+    const bool in = xi >= 0 && xi < a.vocab;
+    bool open = false;   // not decided by the 32-bit sum
     if (lane < k) {
-      xi = __ldg(x + lane);
-      in = xi >= 0 && xi < a.vocab;
       const float top = sh.row_m[lane];
       if (greedy) {
         p = in && top > kNegInf && xi == sh.row_i[lane] ? 1.0 : 0.0;
       } else {
         const double e = in && top > kNegInf ? weights(lane, std::false_type())(value_of<T>(bits_at(lane, xi))) : 0.0;
         const double q =
-            !a.q ? 1.0 : in ? static_cast<double>(__ldg(a.q + s * a.q_seq + lane * a.q_step + xi)) : 0.0;
+            !a.q ? 1.0 : in ? static_cast<double>(__ldg(qx())) : 0.0;
         uq = __ldg(a.u + static_cast<size_t>(s) * (a.k_max + 1) + lane) * q;
         z = sh.row_z[lane];
         p = e > 0.0 ? e / z : 0.0;
