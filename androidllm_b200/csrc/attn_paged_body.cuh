@@ -17,6 +17,12 @@
 // CTA: 8 warps as WM x WK.  Warp (wm, wk) computes rows 16 wm .. 16 wm + 15
 // on the wk-th slice of each tile, with its own running statistics;
 // the WK slices are merged at a unit's end through the stage just consumed.
+//
+// 64 sequences of 1 .. 8191 positions, one token each (28 heads over 4 K/V
+// heads of 128, 127 MB): 39 us, 3.2 TB/s; filled by cp.async from the computing
+// warps it was 52 us.  The stream itself runs near HBM's rate; the start
+// (lengths, shares, the first tile), the units' merges and the join take the
+// rest.  One sequence of 700: 9.9 us, all of it these latencies.
 #pragma once
 #include <algorithm>
 

@@ -14,17 +14,22 @@
 // tiles of one block, joined at the unit's end.
 //
 // Warps 0-3 and 4-7: softmax of stream 0 and 1, one row a thread.  Warps 8 and
-// 11: issue the products of stream 0 and 1 (a thread's issue of the 16 products
-// of a tile and its waits take about as long as the tensor core does, so one
-// for both streams held them up: 336 us against 290 us at 4 x 2047 rows).  Warp 9:
-// loads K and V tiles with TMA, one box per page piece and 64 columns, into a
-// ring of tiles.  Warp 10: loads Q.
+// 11: issue the products of stream 0 and 1.  Warp 9: loads K and V tiles with
+// TMA, one box per page piece and 64 columns, into a ring of tiles.  Warp 10:
+// loads Q.
 //
 // The reference maximum m follows the row's maximum only when that has grown
 // by more than kSlack (in powers of two): weights stay below 2^kSlack, and the
-// rescaling of O, which has to wait for the last product, is rare.  Tensor
-// and exponential units bound long chunks (at 128 x 128 x 128 both take
-// about 512 cycles of an SM), HBM short ones.
+// rescaling of O, which has to wait for the last product, is rare.
+//
+// At 128 x 128 x 128 a tile's products and its exponentials both take about
+// 1024 cycles of an SM, so the streams take turns at the exponential unit
+// (without turns both wait for it at once and the tensor core idles: 351 us
+// against 285 us at 4 x 2047 rows, 28 heads over 4 of 128).  4 x 2047 rows
+// take 270 us (930 TFLOP/s, 55% of a large library product's rate): a stream's
+// chain of product, tensor-memory read, maximum, exponentials, write and
+// product is 3540 cycles a step of both streams, 2048 of them tensor work.
+// 1 x 7 rows over 131 thousand positions (HBM-bound): 70 us, 3.85 TB/s.
 #pragma once
 
 #include "attn_paged_body.cuh"

@@ -6,17 +6,21 @@
 // All units, in the order sequence, token block, head, lie on one line of T
 // places: kUnitCost places for what a unit costs beside its tiles (its first
 // scores, its result), then one a tile.  CTA i of n takes the tiles of places
-// [T i / n, T (i + 1) / n).  Every CTA gets the same share whatever the lengths are, with lengths that only the device
-// knows, and the split points depend on nothing but the batch, so results do
-// not change from run to run.  A unit cut by a share's end leaves one partial
-// result per CTA; a CTA owns at most two of those (its first and last unit).
+// [T i / n, T (i + 1) / n).  Every CTA gets the same share whatever the lengths
+// are, with lengths that only the device knows, and the split points depend on
+// nothing but the batch, so results do not change from run to run.  A unit cut
+// by a share's end leaves one partial result per CTA; a CTA owns at most two of
+// those (its first and last unit).
 #pragma once
 #include "paged.cuh"
 
 namespace alm {
 
 constexpr int kSchedThreads = 256;   // threads that run sched_init (warps 0 .. 7)
-constexpr int kUnitCost = 2;         // in tiles: measured 1 / 2 / 3 at 4 x 2047 prefill rows: 367 / 285 / 283 us
+// In tiles.  0 / 1 / 2 / 4 take 371 / 302 / 268 / 268 us at 4 x 2047 rows, 62 /
+// 38.1 / 38.8 / 44.3 us at 64 decodes, 27.7 / 27.5 / 26.1 / 27.8 us at 9 chunks
+// of 1 to 701 rows.
+constexpr int kUnitCost = 2;
 
 struct Unit {
   int s, mb, h;       // sequence, token block, K/V head

@@ -1,8 +1,8 @@
 // Entry points of the operators of a batched step on device data
 // (alm_kv_view, alm_rope_append, alm_attn_paged, alm_verify): argument checks
-// on the host (arguments before the context), then one launch (two where partial results are joined) on the
-// context's stream.  Nothing here waits for the GPU or allocates, so the
-// calls can be captured.
+// on the host (arguments before the context), then one launch (attention: two,
+// the second joins partial results) on the context's stream.  Nothing here
+// waits for the GPU or allocates, so the calls can be captured.
 #include <cmath>
 #include <string>
 
@@ -37,7 +37,15 @@ cudaError_t paged_init_attrs() {
 }
 
 // Sequences of more rows than this (tokens times the heads that share a K/V
-// head) take the tcgen05 kernel.
+// head) take the tcgen05 kernel.  Measured with 4 K/V heads of 128, mma.sync
+// against tcgen05, us:
+//   rows            16             32             40             64            128
+//   8 x 4000    23.7 / 30.2    24.8 / 30.8    38.5 / 30.7    39.1 / 31.0    55.8 / 34.4
+//   1 x 16000   22.6 / 29.4    23.7 / 29.6    30.6 / 29.8    31.3 / 30.4    49.5 / 40.7
+//   64 x 1000   36.6 / 52.3    39.9 / 52.6    69.5 / 54.0    71.5 / 54.4   102.8 / 56.9
+// (With its TMA producer at 64 rows too the mma.sync kernel would take 31.5 /
+// 27.3 / 53.2 at 40 rows, but 81 against 70 us at 49 rows of 131 thousand
+// positions.)
 constexpr long long kTcMinRows = 32;
 
 // Two partial results a CTA, of the largest row block; a record a CTA.
