@@ -1,7 +1,7 @@
 // Attention of a pass's new rows over the paged cache (alm_attn_paged): the
-// mma.sync kernel for few rows a sequence, and the kernel that joins the
-// partial results of units cut between CTAs.  Instantiated for fp16
-// and bf16 in attn_paged_f16.cu and attn_paged_bf16.cu.
+// mma.sync kernel for few rows a sequence, and the join of the partial results
+// of units cut between CTAs (by the last of them, or by a kernel).
+// Instantiated for fp16 and bf16 in attn_paged_f16.cu and attn_paged_bf16.cu.
 //
 //   o_i = sum_j exp(c (s_ij - m_i)) v_j / sum_j exp(c (s_ij - m_i)),  s = q.k,
 //   c = scale, over the positions j that row i sees; m_i = max_j s_ij.
@@ -22,7 +22,7 @@
 // heads of 128, 127 MB): 39 us, 3.2 TB/s; filled by cp.async from the computing
 // warps it was 52 us.  The stream itself runs near HBM's rate; the start
 // (lengths, shares, the first tile), the units' merges and the join take the
-// rest.  One sequence of 700: 9.9 us, all of it these latencies.
+// rest.  One sequence of 700: 11 us, all of it these latencies.
 #pragma once
 #include <algorithm>
 
@@ -137,6 +137,79 @@ ALM_DEV int4 record_of(const Unit& u, int cta, int n_cta, long long total) {
   return make_int4(last - cta + 1, u.row0, u.n_tok, u.h);
 }
 
+// V consecutive fp32 values behind L1 (another SM wrote them).
+template <int V>
+ALM_DEV void load_row(const float* p, float (&v)[V]) {
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(p + i));
+      v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+    }
+  } else if constexpr (V == 2) {
+    const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
+    v[0] = x.x, v[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = __ldcg(p + i);
+  }
+}
+
+// Joins the partial results of the unit that CTA `cta` began, rows row_first,
+// row_first + row_step, ..: a warp a row, partials added in CTA order.  A unit's
+// ROWS rows are blocks of BLK rows, whole tokens each.
+template <typename T, int HD, int ROWS, int BLK>
+__device__ __noinline__ void join_rows(const AttnPaged& a, int cta, int4 rec, int row_first, int row_step) {
+  constexpr int V = HD / 32;
+  const int lane = threadIdx.x % kWarp;
+  const int tq = BLK / a.group;
+  const int n = rec.x, row0 = rec.y, n_tok = rec.z, kv_head = rec.w;
+  auto part = [&](int i) { return partial_at<HD>(a.work, ROWS, cta + i, i == 0 ? 1 : 0); };
+  for (int row = row_first; row < ROWS; row += row_step) {
+    const int tk = row % BLK / a.group, tok = row / BLK * tq + tk;
+    const int head = kv_head * a.group + row % BLK - tk * a.group;
+    if (tk >= tq || tok >= n_tok) continue;
+    float m = kNegInf;
+    for (int i = lane; i < n; i += kWarp) m = fmaxf(m, __ldcg(part(i) + ROWS * HD + row));
+    m = warp_max(m);
+    const float base = m == kNegInf ? 0.f : m;
+    float l = 0.f, o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += kWarp) {
+      float w = 0.f, li = 0.f;
+      if (i0 + lane < n) {
+        const float* p = part(i0 + lane) + ROWS * HD;
+        w = ex2((__ldcg(p + row) - base) * a.scale_log2);
+        li = __ldcg(p + ROWS + row);
+      }
+      const int k = min(kWarp, n - i0);
+#pragma unroll 8
+      for (int i = 0; i < k; ++i) {
+        const float f = __shfl_sync(0xffffffffu, w, i);
+        l = fmaf(__shfl_sync(0xffffffffu, li, i), f, l);
+        float v[V];
+        load_row<V>(part(i0 + i) + row * HD + lane * V, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = fmaf(v[j], f, o[j]);
+      }
+    }
+    const float inv = m == kNegInf && l == 0.f ? 0.f : 1.f / l;
+    T* dst = reinterpret_cast<T*>(a.out + (row0 + tok) * a.out_row + head * a.out_head) + lane * V;
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+      for (int j = 0; j < V; j += 2)
+        reinterpret_cast<uint32_t*>(dst)[j / 2] = Elem<T>::pack(o[j] * inv, o[j + 1] * inv);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) dst[j] = Elem<T>::down(o[j] * inv);
+    }
+    if (a.lse && lane == 0)
+      a.lse[(row0 + tok) * a.lse_row + head] =
+          m == kNegInf ? kNegInf : (m * a.scale_log2 + log2f(l)) * 0.693147180559945309f;
+  }
+}
+
 // One row by one warp straight from the formula, skipping every position the
 // row does not see: for rows whose sums are not finite though their weights
 // are, since a hidden position's infinity or NaN times a zero weight spoils a
@@ -193,6 +266,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   __shared__ float st_m[kWK][kRows], st_l[kWK][kRows];
   __shared__ float row_m[kRows], row_l[kRows];
   __shared__ int row_bad[kRows];
+  __shared__ int joins;
 
   grid_dep_wait();
   grid_dep_launch();
@@ -567,6 +641,20 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         }
       }
     }
+    if (!whole && a.arrived) {
+      // the last of the unit's CTAs to come here joins their results
+      const int first = t_first == 0 ? cta : static_cast<int>(((u.start + 1) * n_cta - 1) / total);
+      const int4 rec = record_of(u, first, n_cta, total);
+      sync();
+      if (tid == 0) {   // (releases what the barrier has gathered, and acquires for it)
+        unsigned before;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.arrived + first) : "memory");
+        joins = before + 1 == static_cast<unsigned>(rec.x);
+        if (joins) a.arrived[first] = 0;
+      }
+      sync();
+      if (joins) join_rows<T, HD, kRows, kRows>(a, first, rec, warp, kPagedWarps);
+    }
     if (!u.more(x1)) break;
     next_unit<kTile>(b, kv, tpu, a.window, u);
     t = t_first = 0;
@@ -578,80 +666,16 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   if (bad_page) *err = 1;
 }
 
-// V consecutive fp32 values behind L1 (another SM wrote them).
-template <int V>
-ALM_DEV void load_row(const float* p, float (&v)[V]) {
-  if constexpr (V % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(p + i));
-      v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
-    }
-  } else if constexpr (V == 2) {
-    const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
-    v[0] = x.x, v[1] = x.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = __ldcg(p + i);
-  }
-}
-
 // Joins the partial results of the unit that CTA blockIdx.x began and did not
-// finish, as its record says: a warp a row, partials added in CTA order.  A
-// unit's ROWS rows are blocks of BLK rows, whole tokens each.
+// finish, as its record says.
 template <typename T, int HD, int ROWS, int BLK>
 __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const __grid_constant__ AttnPaged a) {
-  constexpr int V = HD / 32, kWarps = kJoinThreads / kWarp;
-  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp, cta = blockIdx.x;
-  const int tq = BLK / a.group;
+  constexpr int kWarps = kJoinThreads / kWarp;
+  const int warp = threadIdx.x / kWarp, cta = blockIdx.x;
   grid_dep_wait();
   const int4 rec = __ldcg(join_record(a, cta));
-  const int n = rec.x, row0 = rec.y, n_tok = rec.z, kv_head = rec.w;
-  if (n == 0) return;
-  auto part = [&](int i) { return partial_at<HD>(a.work, ROWS, cta + i, i == 0 ? 1 : 0); };
-  for (int row = blockIdx.y * kWarps + warp; row < ROWS; row += gridDim.y * kWarps) {
-    const int tk = row % BLK / a.group, tok = row / BLK * tq + tk;
-    const int head = kv_head * a.group + row % BLK - tk * a.group;
-    if (tk >= tq || tok >= n_tok) continue;
-    float m = kNegInf;
-    for (int i = lane; i < n; i += kWarp) m = fmaxf(m, __ldcg(part(i) + ROWS * HD + row));
-    m = warp_max(m);
-    const float base = m == kNegInf ? 0.f : m;
-    float l = 0.f, o[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = 0.f;
-    for (int i0 = 0; i0 < n; i0 += kWarp) {
-      float w = 0.f, li = 0.f;
-      if (i0 + lane < n) {
-        const float* p = part(i0 + lane) + ROWS * HD;
-        w = ex2((__ldcg(p + row) - base) * a.scale_log2);
-        li = __ldcg(p + ROWS + row);
-      }
-      const int k = min(kWarp, n - i0);
-#pragma unroll 8
-      for (int i = 0; i < k; ++i) {
-        const float f = __shfl_sync(0xffffffffu, w, i);
-        l = fmaf(__shfl_sync(0xffffffffu, li, i), f, l);
-        float v[V];
-        load_row<V>(part(i0 + i) + row * HD + lane * V, v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = fmaf(v[j], f, o[j]);
-      }
-    }
-    const float inv = m == kNegInf && l == 0.f ? 0.f : 1.f / l;
-    T* dst = reinterpret_cast<T*>(a.out + (row0 + tok) * a.out_row + head * a.out_head) + lane * V;
-    if constexpr (V % 2 == 0) {
-#pragma unroll
-      for (int j = 0; j < V; j += 2)
-        reinterpret_cast<uint32_t*>(dst)[j / 2] = Elem<T>::pack(o[j] * inv, o[j + 1] * inv);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) dst[j] = Elem<T>::down(o[j] * inv);
-    }
-    if (a.lse && lane == 0)
-      a.lse[(row0 + tok) * a.lse_row + head] =
-          m == kNegInf ? kNegInf : (m * a.scale_log2 + log2f(l)) * 0.693147180559945309f;
-  }
+  if (rec.x == 0) return;
+  join_rows<T, HD, ROWS, BLK>(a, cta, rec, blockIdx.y * kWarps + warp, gridDim.y * kWarps);
 }
 
 template <typename T, int HD, int WM, bool TMA = false>
@@ -698,7 +722,7 @@ cudaError_t launch_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& k
   if (TMA && (!encode_pages<T>(&km, kv.k, kv, box) || !encode_pages<T>(&vm, kv.v, kv, box))) return cudaErrorInvalidValue;
   OpLaunch l(dim3(a.n_cta, 1, 1), S::kThreads, S::kSmem, st);
   const cudaError_t e = cudaLaunchKernelEx(&l.cfg, attn_paged_kernel<T, HD, WM, TMA>, km, vm, a, b, kv, box, err);
-  return e != cudaSuccess ? e : launch_join<T, HD, S::kRows, S::kRows>(a, st);
+  return e != cudaSuccess || a.arrived ? e : launch_join<T, HD, S::kRows, S::kRows>(a, st);
 }
 
 // The smallest row block that holds the longest sequence's rows: K and V are

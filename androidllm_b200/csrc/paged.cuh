@@ -130,6 +130,7 @@ struct AttnPaged {
   float scale_log2;            // scale * log2(e)
   char* work;                  // partial results
   void* records;               // 16 bytes a CTA
+  unsigned* arrived;           // a counter a CTA, zero between calls; null: the join kernel follows
   int n_cta;                   // CTAs that share the tiles
 };
 

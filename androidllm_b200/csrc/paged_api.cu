@@ -1,8 +1,9 @@
 // Entry points of the operators of a batched step on device data
 // (alm_kv_view, alm_rope_append, alm_attn_paged, alm_verify): argument checks
-// on the host (arguments before the context), then one launch (attention: two,
-// the second joins partial results) on the context's stream.  Nothing here
+// on the host (arguments before the context), then one launch (attention of
+// more than a few rows: two, the second joins partial results) on the context's stream.  Nothing here
 // waits for the GPU or allocates, so the calls can be captured.
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -48,12 +49,23 @@ cudaError_t paged_init_attrs() {
 // positions.)
 constexpr long long kTcMinRows = 32;
 
-// Two partial results a CTA, of the largest row block; a record a CTA.
+// Sequences of at most this many rows: the last of a unit's CTAs joins their
+// results, a warp a row.  More rows are joined by a kernel of their own, which
+// spreads them over more CTAs but costs a launch (4 us of the host's time).
+// Joined there against by the kernel, 4 K/V heads of 128, us:
+//   rows           8             16            32
+//   3 x 100     7.2 / 8.6     7.5 / 8.9     8.6 / 10.1
+//   2 x 4000   13.9 / 14.9   17.1 / 15.4   24.1 / 16.7
+//   1 x 16000  20.0 / 21.8   26.3 / 22.2   38.8 / 23.8
+//   64 x 1000  36.5 / 36.1   39.9 / 37.4   46.1 / 40.2
+constexpr long long kJoinHere = 8;
+
+// Two partial results a CTA, of the largest row block; a record and a counter a CTA.
 size_t attn_paged_part_bytes(int n_sms, int head_dim) {
   return static_cast<size_t>(n_sms) * 2 * 256 * (head_dim + 2) * sizeof(float);
 }
 size_t attn_paged_work_bytes(int n_sms, int head_dim) {
-  return attn_paged_part_bytes(n_sms, head_dim) + static_cast<size_t>(n_sms) * 16;
+  return attn_paged_part_bytes(n_sms, head_dim) + static_cast<size_t>(n_sms) * 20;
 }
 }  // namespace alm
 
@@ -241,6 +253,7 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   a.n_cta = n_sms;
   OnDevice on(device);
   const long long rows = static_cast<long long>(b.max_rows) * a.group;
+  a.arrived = nullptr;
   const bool bf = kv_->dtype == ALM_BF16;
   if (rows > kTcMinRows && attn_paged_tc_fits(a, b, kv)) {
     const int nq = rows > 128 ? 2 : 1;
@@ -248,6 +261,8 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
                           : launch_attn_paged_tc_f16(a, b, kv, nq, err, st),
                        "attn_paged");
   }
+  if (rows <= kJoinHere)
+    a.arrived = reinterpret_cast<unsigned*>(static_cast<char*>(a.records) + n_sms * 16);
   return cuda_status(bf ? launch_attn_paged_bf16(a, b, kv, err, st) : launch_attn_paged_f16(a, b, kv, err, st),
                      "attn_paged");
 }

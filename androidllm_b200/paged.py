@@ -248,13 +248,15 @@ class SeqBatch:
 
 class AttnWorkspace:
     """Work area of ``attn_paged`` (partial results of sequences that several
-    CTAs share), for any batch of these heads.  Calls that can overlap on the
+    CTAs share, counters of those that are ready), for any batch of these heads.  Calls that can overlap on the
     GPU, graphs replayed on different streams among them, need one each."""
 
     def __init__(self, ctx, heads, kv_heads, head_dim):
         n = ctypes.c_size_t()
         check(lib.alm_attn_paged_work(ctx.h, int(heads), int(kv_heads), int(head_dim), ctypes.byref(n)))
         self.buf = DeviceBuffer(ctx, n.value)
+        zeros = np.zeros(min(n.value, 4096), np.uint8)   # the counters at its end
+        check(lib.alm_copy_h2d(ctx.h, self.buf.h.value + n.value - zeros.size, zeros.ctypes.data, zeros.size))
         self.pointer, self.nbytes, self.device = self.buf.h.value, n.value, ctx.device
 
 
