@@ -451,7 +451,8 @@ ALM_API int alm_kv_view(alm_kv* kv, int layer, alm_paged_kv* view, const int32_t
  * rot_dim (a multiple of 16, at most head_dim) values of a head are rotated:
  * values i and i + rot_dim / 2 together, or 2i and 2i + 1 (interleaved = 1).
  * q goes to q_out_dev (which may be q_dev itself with the same strides),
- * K and unrotated V to the pages.  Arithmetic in fp32, rounded once.
+ * K and unrotated V to the pages (sequences of one call that share a page must
+ * not write the same position of it: which of them stays is not defined).  Arithmetic in fp32, rounded once.
  * A row whose position is negative or not below rope_rows, or whose page is
  * outside the table or the pool, is not written and is recorded for
  * alm_ctx_sync.  Runs on the context's stream without waiting. */
