@@ -743,7 +743,7 @@ cudaError_t launch_tc(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, 
     return cudaErrorInvalidValue;
   OpLaunch l(dim3(a.n_cta, 1, 1), kTcPagedThreads, S::kSmem, st);
   const cudaError_t e = cudaLaunchKernelEx(&l.cfg, attn_paged_tc_kernel<T, HD, NQ>, km, vm, qm, a, b, kv, box, err);
-  return e != cudaSuccess ? e : launch_join<T, HD, NQ * 128, 128>(a, st);
+  return e != cudaSuccess ? e : launch_join<T, HD, NQ * 128, 128>(a, b, kv, NQ * (128 / a.group), st);
 }
 
 template <typename T>

@@ -250,7 +250,7 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   a.scale_log2 = v->scale * 1.4426950408889634f;
   a.work = static_cast<char*>(v->work_dev);
   a.records = a.work + attn_paged_part_bytes(n_sms, kv.head_dim);
-  a.n_cta = n_sms;
+  a.n_cta = std::min(n_sms, 160);
   OnDevice on(device);
   const long long rows = static_cast<long long>(b.max_rows) * a.group;
   a.arrived = nullptr;
@@ -261,7 +261,7 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
                           : launch_attn_paged_tc_f16(a, b, kv, nq, err, st),
                        "attn_paged");
   }
-  if (rows <= kJoinHere)
+  if (rows <= kJoinHere && kv.head_dim <= 128)   // (the 16-row kernel)
     a.arrived = reinterpret_cast<unsigned*>(static_cast<char*>(a.records) + n_sms * 16);
   return cuda_status(bf ? launch_attn_paged_bf16(a, b, kv, err, st) : launch_attn_paged_f16(a, b, kv, err, st),
                      "attn_paged");
