@@ -33,7 +33,6 @@ namespace alm {
 
 constexpr int kPagedThreads = 256;
 constexpr int kJoinThreads = 128;
-constexpr int kFewUnits = 8;
 constexpr int kMaxCtas = 160;        // CTAs that share the tiles, at most
 constexpr int kPagedWarps = kPagedThreads / kWarp;
 
@@ -159,8 +158,8 @@ ALM_DEV void load_row(const float* p, float (&v)[V]) {
 
 // One row of the unit that CTA `cta` began, by a warp: the sum of its partial
 // results i_lo .. i_hi - 1 (in CTA order), weighed for the maximum of all of
-// them.  (A unit's ROWS rows are blocks of BLK rows, whole tokens each.)
-template <int HD, int ROWS>
+// them, kDeep of them under way at a time.  (A unit's ROWS rows are blocks of BLK rows, whole tokens each.)
+template <int HD, int ROWS, int kDeep>
 ALM_DEV void join_part(const AttnPaged& a, int cta, int n, int row, int i_lo, int i_hi, float& m, float& l,
                        float (&o)[HD / 32]) {
   constexpr int V = HD / 32;
@@ -181,14 +180,19 @@ ALM_DEV void join_part(const AttnPaged& a, int cta, int n, int row, int i_lo, in
       li = __ldcg(p + ROWS + row);
     }
     const int k = min(kWarp, i_hi - i0);
-#pragma unroll 8
-    for (int i = 0; i < k; ++i) {
-      const float f = __shfl_sync(0xffffffffu, w, i);
-      l = fmaf(__shfl_sync(0xffffffffu, li, i), f, l);
-      float v[V];
-      load_row<V>(part(i0 + i) + row * HD + lane * V, v);
+    for (int i = 0; i < k; i += kDeep) {
+      float v[kDeep][V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = fmaf(v[j], f, o[j]);
+      for (int q = 0; q < kDeep; ++q)
+        if (i + q < k) load_row<V>(part(i0 + i + q) + row * HD + lane * V, v[q]);
+#pragma unroll
+      for (int q = 0; q < kDeep; ++q) {
+        if (i + q >= k) break;
+        const float f = __shfl_sync(0xffffffffu, w, i + q);
+        l = fmaf(__shfl_sync(0xffffffffu, li, i + q), f, l);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = fmaf(v[q][j], f, o[j]);
+      }
     }
   }
 }
@@ -211,21 +215,21 @@ ALM_DEV void join_store(const AttnPaged& a, int row, int head, float m, float l,
         m == kNegInf ? kNegInf : (m * a.scale_log2 + log2f(l)) * 0.693147180559945309f;
 }
 // All rows of a unit by n_warps warps, a warp a row.
-template <typename T, int HD, int ROWS, int BLK>
+template <typename T, int HD, int ROWS, int BLK, int kDeep>
 ALM_DEV void join_unit(const AttnPaged& a, int cta, int4 rec, int warp, int n_warps) {
   const int tq = BLK / a.group;
   for (int row = warp; row < ROWS; row += n_warps) {
     const int tk = row % BLK / a.group, tok = row / BLK * tq + tk;
     if (tk >= tq || tok >= rec.z) continue;
     float m, l, o[HD / 32];
-    join_part<HD, ROWS>(a, cta, rec.x, row, 0, rec.x, m, l, o);
+    join_part<HD, ROWS, kDeep>(a, cta, rec.x, row, 0, rec.x, m, l, o);
     join_store<T, HD>(a, rec.y + tok, rec.w * a.group + row % BLK - tk * a.group, m, l, o);
   }
 }
 // (out of line: the attention kernel needs its registers)
 template <typename T, int HD, int ROWS>
 __device__ __noinline__ void join_unit_here(const AttnPaged& a, int cta, int4 rec, int warp) {
-  join_unit<T, HD, ROWS, ROWS>(a, cta, rec, warp, kPagedWarps);
+  join_unit<T, HD, ROWS, ROWS, 4>(a, cta, rec, warp, kPagedWarps);
 }
 
 // One row by one warp straight from the formula, skipping every position the
@@ -694,7 +698,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const __g
   grid_dep_wait();
   const int4 rec = __ldcg(join_record(a, blockIdx.x));
   if (rec.x == 0) return;
-  join_unit<T, HD, ROWS, BLK>(a, blockIdx.x, rec, blockIdx.y * kWarps + threadIdx.x / kWarp, gridDim.y * kWarps);
+  join_unit<T, HD, ROWS, BLK, 8>(a, blockIdx.x, rec, blockIdx.y * kWarps + threadIdx.x / kWarp, gridDim.y * kWarps);
 }
 
 // The same for few units, each of many CTAs: the units' rows form one line, a
@@ -742,7 +746,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_few_kernel(const
     const int tok = j / a.group, hh = j - tok * a.group;
     float m, l, o[V];
     const int tq = BLK / a.group, row = tok / tq * BLK + tok % tq * a.group + hh;
-    join_part<HD, ROWS>(a, cta, r.x, row, r.x * warp / kWarps, r.x * (warp + 1) / kWarps, m, l, o);
+    join_part<HD, ROWS, 8>(a, cta, r.x, row, r.x * warp / kWarps, r.x * (warp + 1) / kWarps, m, l, o);
 #pragma unroll
     for (int q = 0; q < V; ++q) part_o[warp][q * kWarp + lane] = o[q];
     if (lane == 0) part_l[warp] = l;

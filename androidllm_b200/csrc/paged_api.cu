@@ -50,15 +50,12 @@ cudaError_t paged_init_attrs() {
 constexpr long long kTcMinRows = 32;
 
 // Sequences of at most this many rows: the last of a unit's CTAs joins their
-// results, a warp a row.  More rows are joined by a kernel of their own, which
-// spreads them over more CTAs but costs a launch (4 us of the host's time).
-// Joined there against by the kernel, 4 K/V heads of 128, us:
-//   rows           8             16            32
-//   3 x 100     7.2 / 8.6     7.5 / 8.9     8.6 / 10.1
-//   2 x 4000   13.9 / 14.9   17.1 / 15.4   24.1 / 16.7
-//   1 x 16000  20.0 / 21.8   26.3 / 22.2   38.8 / 23.8
-//   64 x 1000  36.5 / 36.1   39.9 / 37.4   46.1 / 40.2
-constexpr long long kJoinHere = 8;
+// results, a warp a row.  More rows, and few units of long sequences (many
+// partials a row), are joined by a kernel of their own, which spreads them over
+// more CTAs but costs a launch (4 us of the host's time).  Joined there against
+// by the kernel, 8 rows a K/V head, 4 heads of 128: 3 x 100 7.4 / 9.1 us, 64 x
+// 1000 36.3 / 36.8 us, 2 x 4000 14.0 / 13.5 us, 1 x 16000 20.0 / 17.0 us.
+constexpr long long kJoinHere = 8, kLongTable = 4096;
 
 // Two partial results a CTA, of the largest row block; a record and a counter a CTA.
 size_t attn_paged_part_bytes(int n_sms, int head_dim) {
@@ -261,7 +258,9 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
                           : launch_attn_paged_tc_f16(a, b, kv, nq, err, st),
                        "attn_paged");
   }
-  if (rows <= kJoinHere && kv.head_dim <= 128)   // (the 16-row kernel)
+  const bool few_long = b.n_seq * kv.kv_heads <= kFewUnits &&
+                        static_cast<long long>(b.table_pages) * kv.page_size >= kLongTable;
+  if (rows <= kJoinHere && kv.head_dim <= 128 && !few_long)   // (the 16-row kernel)
     a.arrived = reinterpret_cast<unsigned*>(static_cast<char*>(a.records) + n_sms * 16);
   return cuda_status(bf ? launch_attn_paged_bf16(a, b, kv, err, st) : launch_attn_paged_f16(a, b, kv, err, st),
                      "attn_paged");
