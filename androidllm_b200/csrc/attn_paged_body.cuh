@@ -33,7 +33,6 @@ namespace alm {
 
 constexpr int kPagedThreads = 256;
 constexpr int kJoinThreads = 128;
-constexpr int kMaxCtas = 160;        // CTAs that share the tiles, at most
 constexpr int kPagedWarps = kPagedThreads / kWarp;
 
 template <typename T>
@@ -156,12 +155,11 @@ ALM_DEV void load_row(const float* p, float (&v)[V]) {
   }
 }
 
-// One row of the unit that CTA `cta` began, by a warp: the sum of its partial
-// results i_lo .. i_hi - 1 (in CTA order), weighed for the maximum of all of
-// them, kDeep of them under way at a time.  (A unit's ROWS rows are blocks of BLK rows, whole tokens each.)
+// One row of the unit that CTA `cta` began, by a warp: the sum of its n partial
+// results in CTA order, kDeep of them under way at a time (left to the compiler
+// two or three were: 8 x 5 rows 14.4 us instead of 11.8).
 template <int HD, int ROWS, int kDeep>
-ALM_DEV void join_part(const AttnPaged& a, int cta, int n, int row, int i_lo, int i_hi, float& m, float& l,
-                       float (&o)[HD / 32]) {
+ALM_DEV void join_part(const AttnPaged& a, int cta, int n, int row, float& m, float& l, float (&o)[HD / 32]) {
   constexpr int V = HD / 32;
   const int lane = threadIdx.x % kWarp;
   auto part = [&](int i) { return partial_at<HD>(a.work, ROWS, cta + i, i == 0 ? 1 : 0); };
@@ -172,14 +170,14 @@ ALM_DEV void join_part(const AttnPaged& a, int cta, int n, int row, int i_lo, in
   l = 0.f;
 #pragma unroll
   for (int j = 0; j < V; ++j) o[j] = 0.f;
-  for (int i0 = i_lo; i0 < i_hi; i0 += kWarp) {
+  for (int i0 = 0; i0 < n; i0 += kWarp) {
     float w = 0.f, li = 0.f;
-    if (i0 + lane < i_hi) {
+    if (i0 + lane < n) {
       const float* p = part(i0 + lane) + ROWS * HD;
       w = ex2((__ldcg(p + row) - base) * a.scale_log2);
       li = __ldcg(p + ROWS + row);
     }
-    const int k = min(kWarp, i_hi - i0);
+    const int k = min(kWarp, n - i0);
     for (int i = 0; i < k; i += kDeep) {
       float v[kDeep][V];
 #pragma unroll
@@ -214,7 +212,8 @@ ALM_DEV void join_store(const AttnPaged& a, int row, int head, float m, float l,
     a.lse[row * a.lse_row + head] =
         m == kNegInf ? kNegInf : (m * a.scale_log2 + log2f(l)) * 0.693147180559945309f;
 }
-// All rows of a unit by n_warps warps, a warp a row.
+// All rows of a unit by n_warps warps, a warp a row.  A unit's ROWS rows are
+// blocks of BLK rows, whole tokens each.
 template <typename T, int HD, int ROWS, int BLK, int kDeep>
 ALM_DEV void join_unit(const AttnPaged& a, int cta, int4 rec, int warp, int n_warps) {
   const int tq = BLK / a.group;
@@ -222,7 +221,7 @@ ALM_DEV void join_unit(const AttnPaged& a, int cta, int4 rec, int warp, int n_wa
     const int tk = row % BLK / a.group, tok = row / BLK * tq + tk;
     if (tk >= tq || tok >= rec.z) continue;
     float m, l, o[HD / 32];
-    join_part<HD, ROWS, kDeep>(a, cta, rec.x, row, 0, rec.x, m, l, o);
+    join_part<HD, ROWS, kDeep>(a, cta, rec.x, row, m, l, o);
     join_store<T, HD>(a, rec.y + tok, rec.w * a.group + row % BLK - tk * a.group, m, l, o);
   }
 }
@@ -701,68 +700,6 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const __g
   join_unit<T, HD, ROWS, BLK, 8>(a, blockIdx.x, rec, blockIdx.y * kWarps + threadIdx.x / kWarp, gridDim.y * kWarps);
 }
 
-// The same for few units, each of many CTAs: the units' rows form one line, a
-// block a row, and each of its warps adds a quarter of the row's partials (7
-// rows of 28 heads over 4, 131 thousand positions: 66 us in all, with the
-// kernel above 70 us; but 14.7 against 13.9 us at 8 x 5 rows).
-template <typename T, int HD, int ROWS, int BLK>
-__global__ void __launch_bounds__(kJoinThreads) attn_paged_join_few_kernel(const __grid_constant__ AttnPaged a) {
-  constexpr int V = HD / 32, kWarps = kJoinThreads / kWarp, kChunks = kMaxCtas / kWarp;
-  __shared__ float part_o[kWarps][HD], part_l[kWarps];
-  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-  grid_dep_wait();
-  int4 rec[kChunks];
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c)
-    rec[c] = c * kWarp + lane < a.n_cta ? __ldcg(join_record(a, c * kWarp + lane)) : make_int4(0, 0, 0, 0);
-  int upto[kChunks], total = 0;   // rows up to this lane's record, and of all
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    int scan = rec[c].x > 0 ? rec[c].z * a.group : 0;
-#pragma unroll
-    for (int o = 1; o < kWarp; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, scan, o);
-      if (lane >= o) scan += y;
-    }
-    upto[c] = total + scan;
-    total += __shfl_sync(0xffffffffu, scan, kWarp - 1);
-  }
-  for (int f = blockIdx.x; f < total; f += gridDim.x) {
-    int cta = -1, j = 0;
-    int4 r = make_int4(0, 0, 0, 0);
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const unsigned hit = __ballot_sync(0xffffffffu, f < upto[c]);
-      if (cta < 0 && hit) {
-        const int src = __ffs(hit) - 1;
-        cta = c * kWarp + src;
-        r.x = __shfl_sync(0xffffffffu, rec[c].x, src);
-        r.y = __shfl_sync(0xffffffffu, rec[c].y, src);
-        r.z = __shfl_sync(0xffffffffu, rec[c].z, src);
-        r.w = __shfl_sync(0xffffffffu, rec[c].w, src);
-        j = f - (__shfl_sync(0xffffffffu, upto[c], src) - r.z * a.group);
-      }
-    }
-    const int tok = j / a.group, hh = j - tok * a.group;
-    float m, l, o[V];
-    const int tq = BLK / a.group, row = tok / tq * BLK + tok % tq * a.group + hh;
-    join_part<HD, ROWS, 8>(a, cta, r.x, row, r.x * warp / kWarps, r.x * (warp + 1) / kWarps, m, l, o);
-#pragma unroll
-    for (int q = 0; q < V; ++q) part_o[warp][q * kWarp + lane] = o[q];
-    if (lane == 0) part_l[warp] = l;
-    __syncthreads();
-    if (warp == 0) {
-      for (int p = 1; p < kWarps; ++p) {
-        l += part_l[p];
-#pragma unroll
-        for (int q = 0; q < V; ++q) o[q] += part_o[p][q * kWarp + lane];
-      }
-      join_store<T, HD>(a, r.y + tok, r.w * a.group + hh, m, l, o);
-    }
-    __syncthreads();
-  }
-}
-
 template <typename T, int HD, int WM, bool TMA = false>
 cudaError_t paged_attr() {
   return cudaFuncSetAttribute(attn_paged_kernel<T, HD, WM, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -792,14 +729,8 @@ cudaError_t paged_attr_all() {
   return e;
 }
 
-// tokens: of a unit
 template <typename T, int HD, int ROWS, int BLK>
-cudaError_t launch_join(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, int tokens, cudaStream_t st) {
-  const long long units = static_cast<long long>(b.n_seq) * kv.kv_heads * ((b.max_rows + tokens - 1) / tokens);
-  if (units <= kFewUnits) {
-    OpLaunch l(dim3(std::min(ROWS * kFewUnits, 8 * a.n_cta), 1, 1), kJoinThreads, 0, st);
-    return cudaLaunchKernelEx(&l.cfg, attn_paged_join_few_kernel<T, HD, ROWS, BLK>, a);
-  }
+cudaError_t launch_join(const AttnPaged& a, cudaStream_t st) {
   // 16 blocks an owner at most: all of them are resident at once
   OpLaunch l(dim3(a.n_cta, std::min(ROWS / (kJoinThreads / kWarp), 16), 1), kJoinThreads, 0, st);
   return cudaLaunchKernelEx(&l.cfg, attn_paged_join_kernel<T, HD, ROWS, BLK>, a);
@@ -813,7 +744,7 @@ cudaError_t launch_paged(const AttnPaged& a, const SeqBatch& b, const PagedKV& k
   if (TMA && (!encode_pages<T>(&km, kv.k, kv, box) || !encode_pages<T>(&vm, kv.v, kv, box))) return cudaErrorInvalidValue;
   OpLaunch l(dim3(a.n_cta, 1, 1), S::kThreads, S::kSmem, st);
   const cudaError_t e = cudaLaunchKernelEx(&l.cfg, attn_paged_kernel<T, HD, WM, TMA>, km, vm, a, b, kv, box, err);
-  return e != cudaSuccess || a.arrived ? e : launch_join<T, HD, S::kRows, S::kRows>(a, b, kv, S::kRows / a.group, st);
+  return e != cudaSuccess || a.arrived ? e : launch_join<T, HD, S::kRows, S::kRows>(a, st);
 }
 
 // The smallest row block that holds the longest sequence's rows: K and V are

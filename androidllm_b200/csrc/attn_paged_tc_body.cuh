@@ -26,10 +26,11 @@
 // 1024 cycles of an SM, so the streams take turns at the exponential unit
 // (without turns both wait for it at once and the tensor core idles: 351 us
 // against 285 us at 4 x 2047 rows, 28 heads over 4 of 128).  4 x 2047 rows
-// take 270 us (930 TFLOP/s, 55% of a large library product's rate): a stream's
+// take 268 us (935 TFLOP/s, 56% of a large library product's rate): a stream's
 // chain of product, tensor-memory read, maximum, exponentials, write and
 // product is 3540 cycles a step of both streams, 2048 of them tensor work.
-// 1 x 7 rows over 131 thousand positions (HBM-bound): 70 us, 3.85 TB/s.
+// 1 x 7 rows over 131 thousand positions (HBM-bound): 65 us, 4.1 TB/s, 60 us
+// of it this kernel.
 #pragma once
 
 #include "attn_paged_body.cuh"
@@ -743,7 +744,7 @@ cudaError_t launch_tc(const AttnPaged& a, const SeqBatch& b, const PagedKV& kv, 
     return cudaErrorInvalidValue;
   OpLaunch l(dim3(a.n_cta, 1, 1), kTcPagedThreads, S::kSmem, st);
   const cudaError_t e = cudaLaunchKernelEx(&l.cfg, attn_paged_tc_kernel<T, HD, NQ>, km, vm, qm, a, b, kv, box, err);
-  return e != cudaSuccess ? e : launch_join<T, HD, NQ * 128, 128>(a, b, kv, NQ * (128 / a.group), st);
+  return e != cudaSuccess ? e : launch_join<T, HD, NQ * 128, 128>(a, st);
 }
 
 template <typename T>

@@ -119,8 +119,6 @@ struct RopeAppend {
   int rope_rows, rot;
 };
 
-constexpr int kFewUnits = 8;    // attention units (sequence, token block, K/V head) that are joined a block a row
-
 struct AttnPaged {
   const char* q;
   int64_t q_row, q_head;       // bytes

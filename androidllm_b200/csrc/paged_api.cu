@@ -1,7 +1,8 @@
 // Entry points of the operators of a batched step on device data
 // (alm_kv_view, alm_rope_append, alm_attn_paged, alm_verify): argument checks
 // on the host (arguments before the context), then one launch (attention of
-// more than a few rows: two, the second joins partial results) on the context's stream.  Nothing here
+// more than a few rows: two,
+// the second joins partial results) on the context's stream.  Nothing here
 // waits for the GPU or allocates, so the calls can be captured.
 #include <algorithm>
 #include <cmath>
@@ -41,11 +42,11 @@ cudaError_t paged_init_attrs() {
 // head) take the tcgen05 kernel.  Measured with 4 K/V heads of 128, mma.sync
 // against tcgen05, us:
 //   rows            16             32             40             64            128
-//   8 x 4000    23.7 / 30.2    24.8 / 30.8    38.5 / 30.7    39.1 / 31.0    55.8 / 34.4
-//   1 x 16000   22.6 / 29.4    23.7 / 29.6    30.6 / 29.8    31.3 / 30.4    49.5 / 40.7
-//   64 x 1000   36.6 / 52.3    39.9 / 52.6    69.5 / 54.0    71.5 / 54.4   102.8 / 56.9
-// (With its TMA producer at 64 rows too the mma.sync kernel would take 31.5 /
-// 27.3 / 53.2 at 40 rows, but 81 against 70 us at 49 rows of 131 thousand
+//   8 x 4000    22.2 / 28.2    22.9 / 28.3    37.2 / 29.1    38.2 / 29.5    54.0 / 31.9
+//   1 x 16000   16.9 / 24.6    17.8 / 24.7    25.8 / 25.2    26.4 / 25.4    34.8 / 26.1
+//   64 x 1000   36.9 / 50.9    39.0 / 51.2    69.4 / 53.1    72.1 / 54.3   104.1 / 57.9
+// (With its TMA producer at 64 rows too the mma.sync kernel takes as long as
+// the tcgen05 kernel there, and 16% longer at 49 rows of 131 thousand
 // positions.)
 constexpr long long kTcMinRows = 32;
 
@@ -55,7 +56,7 @@ constexpr long long kTcMinRows = 32;
 // more CTAs but costs a launch (4 us of the host's time).  Joined there against
 // by the kernel, 8 rows a K/V head, 4 heads of 128: 3 x 100 7.4 / 9.1 us, 64 x
 // 1000 36.3 / 36.8 us, 2 x 4000 14.0 / 13.5 us, 1 x 16000 20.0 / 17.0 us.
-constexpr long long kJoinHere = 8, kLongTable = 4096;
+constexpr long long kJoinHere = 8, kFewUnits = 8, kLongTable = 4096;
 
 // Two partial results a CTA, of the largest row block; a record and a counter a CTA.
 size_t attn_paged_part_bytes(int n_sms, int head_dim) {
@@ -247,7 +248,7 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   a.scale_log2 = v->scale * 1.4426950408889634f;
   a.work = static_cast<char*>(v->work_dev);
   a.records = a.work + attn_paged_part_bytes(n_sms, kv.head_dim);
-  a.n_cta = std::min(n_sms, 160);
+  a.n_cta = n_sms;
   OnDevice on(device);
   const long long rows = static_cast<long long>(b.max_rows) * a.group;
   a.arrived = nullptr;
