@@ -156,7 +156,6 @@ struct Verify {
 cudaError_t launch_rope_append(const RopeAppend& a, const SeqBatch& b, const PagedKV& kv, int dtype, int rope_dtype,
                                bool interleaved, int n_sms, int* err, cudaStream_t st);
 cudaError_t launch_verify(const Verify& a, int dtype, cudaStream_t st);
-size_t attn_paged_part_bytes(int n_sms, int head_dim);
 size_t attn_paged_work_bytes(int n_sms, int head_dim);
 cudaError_t paged_init_attrs();
 

@@ -1,9 +1,9 @@
 // Entry points of the operators of a batched step on device data
 // (alm_kv_view, alm_rope_append, alm_attn_paged, alm_verify): argument checks
 // on the host (arguments before the context), then one launch (attention of
-// more than a few rows: two,
-// the second joins partial results) on the context's stream.  Nothing here
-// waits for the GPU or allocates, so the calls can be captured.
+// more than a few rows: two, the second joins partial results) on the context's
+// stream.  Nothing here waits for the GPU or allocates, so the calls can be
+// captured.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -58,12 +58,12 @@ constexpr long long kTcMinRows = 32;
 // 1000 36.3 / 36.8 us, 2 x 4000 14.0 / 13.5 us, 1 x 16000 20.0 / 17.0 us.
 constexpr long long kJoinHere = 8, kFewUnits = 8, kLongTable = 4096;
 
-// Two partial results a CTA, of the largest row block; a record and a counter a CTA.
-size_t attn_paged_part_bytes(int n_sms, int head_dim) {
-  return static_cast<size_t>(n_sms) * 2 * 256 * (head_dim + 2) * sizeof(float);
-}
+// The work area: a counter and a record a CTA, at the same place for every head
+// dimension (the counters stay zero between calls), then two partial results a
+// CTA, of the largest row block.
+size_t attn_paged_head_bytes(int n_sms) { return (static_cast<size_t>(n_sms) * 20 + 255) / 256 * 256; }
 size_t attn_paged_work_bytes(int n_sms, int head_dim) {
-  return attn_paged_part_bytes(n_sms, head_dim) + static_cast<size_t>(n_sms) * 20;
+  return attn_paged_head_bytes(n_sms) + static_cast<size_t>(n_sms) * 2 * 256 * (head_dim + 2) * sizeof(float);
 }
 }  // namespace alm
 
@@ -246,8 +246,9 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   a.group = v->heads / kv.kv_heads;
   a.window = v->window;
   a.scale_log2 = v->scale * 1.4426950408889634f;
-  a.work = static_cast<char*>(v->work_dev);
-  a.records = a.work + attn_paged_part_bytes(n_sms, kv.head_dim);
+  char* const work = static_cast<char*>(v->work_dev);
+  a.records = work;
+  a.work = work + attn_paged_head_bytes(n_sms);
   a.n_cta = n_sms;
   OnDevice on(device);
   const long long rows = static_cast<long long>(b.max_rows) * a.group;
@@ -262,7 +263,7 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   const bool few_long = b.n_seq * kv.kv_heads <= kFewUnits &&
                         static_cast<long long>(b.table_pages) * kv.page_size >= kLongTable;
   if (rows <= kJoinHere && kv.head_dim <= 128 && !few_long)   // (the 16-row kernel)
-    a.arrived = reinterpret_cast<unsigned*>(static_cast<char*>(a.records) + n_sms * 16);
+    a.arrived = reinterpret_cast<unsigned*>(work + static_cast<size_t>(n_sms) * 16);
   return cuda_status(bf ? launch_attn_paged_bf16(a, b, kv, err, st) : launch_attn_paged_f16(a, b, kv, err, st),
                      "attn_paged");
 }

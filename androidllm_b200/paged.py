@@ -255,8 +255,7 @@ class AttnWorkspace:
         n = ctypes.c_size_t()
         check(lib.alm_attn_paged_work(ctx.h, int(heads), int(kv_heads), int(head_dim), ctypes.byref(n)))
         self.buf = DeviceBuffer(ctx, n.value)
-        zeros = np.zeros(min(n.value, 4096), np.uint8)   # the counters at its end
-        check(lib.alm_copy_h2d(ctx.h, self.buf.h.value + n.value - zeros.size, zeros.ctypes.data, zeros.size))
+        self.buf.upload(np.zeros(min(n.value, 1 << 16), np.uint8))   # the counters at its start
         self.pointer, self.nbytes, self.device = self.buf.h.value, n.value, ctx.device
 
 

@@ -1073,3 +1073,30 @@ def test_verify_drafts_close_to_the_model(ctx, noise):
     u = rng.random((n_seq, k + 1))
     u[:, :k] = 1.0 + 1e-2                    # refuse at once: the residual decides
     check_verify(ctx, start, lg, draft, q, u, np.ones(n_seq), None)
+
+
+def test_one_work_area_for_several_shapes(ctx):
+    """Calls in turn with other head dimensions, row counts and kernels through one area."""
+    work = paged.AttnWorkspace(ctx, 16, 2, 128)
+    cases = []
+    for i, (rows, n_kv, heads, hk, dim) in enumerate([(1, 700, 14, 2, 128), (1, 900, 14, 2, 64), (40, 900, 12, 2, 64),
+                                                      (1, 3000, 4, 1, 32), (4, 2000, 14, 2, 128), (1, 333, 8, 2, 96)]):
+        b = Batch([rows] * 3, [n_kv, n_kv // 2 + rows, rows], 16, hk, dim, torch.float16, seed=80 + i)
+        q = b.randn(b.n_rows, heads, dim)
+        cases.append((b, q, attend(ctx, b, q)[0]))
+    for _ in range(3):
+        for b, q, ref in cases:
+            out, _ = attend(ctx, b, q, work=work)
+            ctx.sync()
+            assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("table", [64, 400])
+def test_decode_rows_joined_either_way(ctx, table):
+    """One long sequence: a small page table has the last CTA join, a large one the kernel."""
+    b = Batch([1], [1000], 16, 2, 128, torch.bfloat16, seed=90)
+    wide = torch.zeros(1, table, device="cuda", dtype=torch.int32)
+    wide[:, :b.table.shape[1]] = b.table[:1]
+    b.seqs = paged.SeqBatch(ints(b.start), ints(b.lens), wide, n_rows=b.n_rows, max_rows=1)
+    q = b.randn(b.n_rows, 8, 128)
+    check_attend(ctx, b, q)
