@@ -661,6 +661,9 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           }
         }
       }
+      // every warp has read its rows' marks before the next unit's end clears
+      // them (a TMA ring lets a warp run whole units ahead of another)
+      sync();
     }
     if constexpr (WM == 1) {
       if (!whole && a.arrived) {

@@ -1100,3 +1100,26 @@ def test_decode_rows_joined_either_way(ctx, table):
     b.seqs = paged.SeqBatch(ints(b.start), ints(b.lens), wide, n_rows=b.n_rows, max_rows=1)
     q = b.randn(b.n_rows, 8, 128)
     check_attend(ctx, b, q)
+
+
+# ---- values that are not finite, beside units that follow ----------------------
+def not_finite_at(b, s, pos, value, col=None):
+    """Makes V of sequence s at this position not finite (every column, or one)."""
+    page = int(b.table[b.slot[s], pos // b.page])
+    b.v[page, :, pos % b.page, slice(None) if col is None else col] = value
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("most", [16, 30])
+def test_attend_hidden_nan_in_many_short_units(ctx, dim, most):
+    """Each CTA runs through units whose every row has a NaN just before its
+    window: the rows recomputed at one unit's end are not lost to the next."""
+    n = 700
+    rows = [most - i % 4 for i in range(n)]
+    lens = [r + 20 + (i * 29) % 90 for i, r in enumerate(rows)]
+    b = Batch(rows, lens, 16, 1, dim, torch.float16, seed=41)
+    for s in range(n):
+        not_finite_at(b, s, lens[s] - rows[s] - 6, float("nan"))
+    q = b.randn(b.n_rows, 1, dim)
+    for _ in range(3):
+        check_attend(ctx, b, q, window=6)
