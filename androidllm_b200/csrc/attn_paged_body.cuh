@@ -415,7 +415,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       const int row = wm * 16 + g + 8 * j;
       const int tok = row / a.group, hh = row - tok * a.group;
       const bool live = tok < u.n_tok;
-      hi[j] = live ? u.pos0 + tok : -1;
+      hi[j] = live ? max(u.pos0 + tok, -1) : -1;
       const char* q = a.q + (u.row0 + tok) * a.q_row + (u.h * a.group + hh) * a.q_head;
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k) {
@@ -480,7 +480,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
           Elem<T>::mma(s[n + 1], qf[k], b2, b3);
         }
       // positions that some row of the block does not see
-      if (p0 + kChunk - 1 > u.pos0 || (a.window > 0 && p0 <= u.pos0 + u.n_tok - 1 - a.window)) {
+      if (p0 + kChunk - 1 > u.pos0 || (a.window > 0 && p0 <= max(u.pos0 + u.n_tok - 1, -1) - a.window)) {
 #pragma unroll
         for (int n = 0; n < kChunk / 8; ++n)
 #pragma unroll

@@ -436,9 +436,9 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         if (go) next();                                  // early: its lengths are loads
         const int tk = r / a.group, tok = blk * tq + tk, head = cu.h * a.group + r - tk * a.group;
         const bool live = tk < tq && tok < cu.n_tok;
-        const int hi = live ? cu.pos0 + tok : -1;       // last position the row sees
+        const int hi = live ? max(cu.pos0 + tok, -1) : -1;   // last position the row sees
         // of the block: the first token's position and the last's
-        const int pos_a = cu.pos0 + blk * tq, pos_b = min(pos_a + tq, cu.pos0 + cu.n_tok) - 1;
+        const int pos_a = cu.pos0 + blk * tq, pos_b = max(min(pos_a + tq, cu.pos0 + cu.n_tok) - 1, -1);
         const bool any_live = __any_sync(0xffffffffu, live);
         float m = kNegInf, l = 0.f;
         int n_mine = 0;
@@ -456,7 +456,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
             tc_ld32(t_s + 32, sr[1]);
             const int p0 = (cu.t0 + t) * S::kTile;
             const bool mask = p0 + S::kTile - 1 > pos_a || (a.window > 0 && p0 <= pos_b - a.window);
-            const int n_hi = hi - p0, n_lo = hi - a.window - p0;   // columns > n_hi, and with a window <= n_lo, are hidden
+            const int n_hi = hi - p0, n_lo = max(n_hi, -1) - a.window;   // columns > n_hi, and with a window <= n_lo, are hidden
             auto hide = [&](int h) {
 #pragma unroll
               for (int i = 64 * h; i < 64 * h + 64; ++i)

@@ -50,7 +50,7 @@ template <int TILE>
 ALM_DEV void block_tiles(const Seq& q, int tpu, int window, int mb, int& t0, int& n_tile) {
   const int first = q.n_kv - q.n_new + mb * tpu;
   const int last = min(first + tpu, q.n_kv) - 1;   // last token's position, n_kv - 1 at most
-  const int lo = window > 0 ? max(0, first - window + 1) : 0;
+  const int lo = window > 0 && first >= window ? first - window + 1 : 0;   // (first may be far below 0)
   t0 = lo / TILE;
   n_tile = last < 0 ? 1 : last / TILE - t0 + 1;
   if (last < 0) t0 = 0;

@@ -244,7 +244,10 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   a.lse_row = v->lse_row;
   a.heads = v->heads;
   a.group = v->heads / kv.kv_heads;
-  a.window = v->window;
+  // a window as long as the table hides nothing (and the kernels' 32-bit
+  // differences of a position and the window stay in range)
+  const long long cap = std::min(static_cast<long long>(b.table_pages) * kv.page_size, 0x7fffff00ll);
+  a.window = v->window >= cap ? 0 : v->window;
   a.scale_log2 = v->scale * 1.4426950408889634f;
   char* const work = static_cast<char*>(v->work_dev);
   a.records = work;

@@ -1123,3 +1123,16 @@ def test_attend_hidden_nan_in_many_short_units(ctx, dim, most):
     q = b.randn(b.n_rows, 1, dim)
     for _ in range(3):
         check_attend(ctx, b, q, window=6)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 200, 1024, 60])
+@pytest.mark.parametrize("rows,lens", [([6], [3]), ([6, 1, 40], [2, 900, 9]), ([300, 5], [100, 700])])
+@pytest.mark.parametrize("dim", [64, 96])
+def test_attend_windows_beyond_every_position(ctx, window, rows, lens, dim):
+    """A window near 2^31 hides nothing, also where rows lie before position 0."""
+    b = Batch(rows, lens, 16, 2, dim, torch.float16, seed=42, first=1)
+    q = b.randn(b.n_rows, 8, dim)
+    out = check_attend(ctx, b, q, window=window)
+    if window > 1000:
+        plain, _ = attend(ctx, b, q)
+        assert torch.equal(out, plain)
