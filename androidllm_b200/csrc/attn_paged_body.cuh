@@ -307,7 +307,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   }
   if (!TMA || warp < kPagedWarps)
     sched_init<kTile>(
-        b, kv, tpu, a.window, sched,
+        b, kv, tpu, a.window, sched, err,
         [&](long long total) {
           const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
           return cta < n ? share(total, cta, n) : -1ll;

@@ -179,7 +179,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
   grid_dep_launch();
   if (warp < 8) {
     sched_init<S::kTile>(
-        b, kv, tpu, a.window, sh.sched,
+        b, kv, tpu, a.window, sh.sched, err,
         [&](long long total) {
           const int n = static_cast<int>(min(static_cast<long long>(a.n_cta), total));
           return cta < n ? share(total, cta, n) : -1ll;

@@ -72,9 +72,10 @@ ALM_DEV long long seq_tiles(const Seq& q, int tpu, int window) {
 constexpr int kManyBlocks = 8;
 
 // The line's length and the sequence that holds place goal(total): every one
-// of the first kSchedThreads threads calls it; sync() is their barrier.
+// of the first kSchedThreads threads calls it; sync() is their barrier.  The
+// first CTA reports sequences that their row of the table does not hold.
 template <int TILE, typename Goal, typename Sync>
-ALM_DEV void sched_init(const SeqBatch& b, const PagedKV& kv, int tpu, int window, SchedShared& sh, Goal goal,
+ALM_DEV void sched_init(const SeqBatch& b, const PagedKV& kv, int tpu, int window, SchedShared& sh, int* err, Goal goal,
                         Sync sync) {
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
   // thread t sums sequences [t per, (t + 1) per); per is 1 up to 256 sequences
@@ -83,8 +84,10 @@ ALM_DEV void sched_init(const SeqBatch& b, const PagedKV& kv, int tpu, int windo
     Seq q;
     q.n_new = 0;
     q.n_kv = 0;
+    q.fits = true;
     if (s < b.n_seq) q = load_seq(b, kv, s);
     const bool in = q.n_new > 0;
+    if (in && !q.fits && blockIdx.x == 0) *err = 1;
     const bool many = in && q.n_new > kManyBlocks * tpu;
     long long n = in && !many ? seq_tiles<TILE>(q, tpu, window) : 0;
     unsigned todo = __ballot_sync(0xffffffffu, many);

@@ -31,9 +31,12 @@ struct SeqBatch {
 
 // What a sequence's entries say, clamped to what exists: rows [row0, row0 +
 // n_new), the last of n_kv positions (n_new > n_kv leaves rows at negative
-// positions), its row of the page table (null: no such row).
+// positions), its row of the page table (null: no such row).  A sequence longer
+// than its row of the table has no position (fits is false): the places of its
+// rows are not known.
 struct Seq {
   int row0, n_new, n_kv;
+  bool fits;
   const int* pages;
 };
 
@@ -46,7 +49,8 @@ ALM_DEV Seq load_seq(const SeqBatch& b, const PagedKV& kv, int s) {
   // (256 below 2^31, so that the end of a tile behind the last position is a number)
   const long long cap = min(static_cast<long long>(b.table_pages) * kv.page_size, 0x7fffff00ll);
   const int len = max(0, __ldg(b.kv_len + s));
-  q.n_kv = len > cap ? static_cast<int>(cap) : len;
+  q.fits = len <= cap;
+  q.n_kv = q.fits ? len : 0;
   const int t = b.slots ? __ldg(b.slots + s) : s;
   q.pages = t >= 0 && t < b.table_rows ? b.table + static_cast<size_t>(t) * b.page_stride : nullptr;
   return q;

@@ -82,7 +82,7 @@ ALM_DEV int2 place_of(const RopeAppend& a, const SeqBatch& b, const PagedKV& kv,
   if (lo >= b.n_seq || __ldg(b.row_start + lo) > r) return make_int2(0, -2);
   const Seq q = load_seq(b, kv, lo);
   const int pos = q.n_kv - q.n_new + (r - q.row0);
-  if (pos < 0 || pos >= q.n_kv || pos >= a.rope_rows || q.pages == nullptr || __ldg(b.kv_len + lo) != q.n_kv)
+  if (pos < 0 || pos >= q.n_kv || pos >= a.rope_rows || q.pages == nullptr)   // (too long a sequence has no position)
     return make_int2(0, -1);
   const int page = __ldg(q.pages + page_of(kv, pos));
   return make_int2(pos, page >= 0 && page < kv.n_pages ? page : -1);

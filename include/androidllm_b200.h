@@ -425,7 +425,9 @@ typedef struct alm_paged_kv {
  * sequence s lies on page page_table_dev[t * page_stride + p / page_size]
  * with t = s, or slots_dev[s] when slots_dev is not NULL; the table has
  * table_rows rows of table_pages valid entries each, and positions behind
- * table_pages * page_size do not exist.  max_rows: a bound on the rows of
+ * table_pages * page_size do not exist: the rows of a sequence that is longer
+ * are not written to the cache, see nothing, and are recorded for
+ * alm_ctx_sync.  max_rows: a bound on the rows of
  * one sequence (it chooses the kernel; a sequence with more rows is still
  * computed).  n_seq is at most 4096. */
 typedef struct alm_seq_batch {
@@ -477,7 +479,8 @@ ALM_API int alm_rope_append(alm_ctx* ctx, const alm_paged_kv* kv, const alm_seq_
  * type, strides in elements, multiples of 8, 16-byte aligned; out_dev must
  * not overlap q_dev.  lse_dev (optional, fp32, (n_rows, heads), row stride
  * lse_row): log of the sum of exp(scale * q.k).  A row that sees no position
- * (its position is negative) gets zeros and -inf.  Values behind a
+ * (its position is negative, or its sequence is longer than its row of the
+ * table) gets zeros and -inf.  Values behind a
  * sequence's end and of pages of other sequences never reach a result, NaN
  * and infinities included; nor does a value at a position that a row does not
  * see.  A page outside the pool is read as zeros and recorded for

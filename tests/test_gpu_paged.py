@@ -1136,3 +1136,25 @@ def test_attend_windows_beyond_every_position(ctx, window, rows, lens, dim):
     if window > 1000:
         plain, _ = attend(ctx, b, q)
         assert torch.equal(out, plain)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 120])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_attend_length_beyond_the_table_is_reported(ctx, rows, dim):
+    """A sequence longer than its row of the table: its rows see nothing, and the next sync says so."""
+    b = Batch([rows, rows], [400, 500], 16, 2, dim, torch.float16, seed=43)
+    b.table[0] = b.table[0, 0]                       # every entry a page of the pool
+    q = b.randn(b.n_rows, 4, dim)
+    good, good_lse = attend(ctx, b, q)
+    ctx.sync()
+    for n in (b.table.shape[1] * 16 + 1, 2 ** 31 - 1):
+        b.seqs._keep[1].copy_(ints([n, 500]))
+        out, lse = attend(ctx, b, q)
+        with pytest.raises(ALMError, match="outside its range"):
+            ctx.sync()
+        ctx.sync()                                   # reported once
+        assert (out[:rows] == 0).all() and (lse[:rows] == -math.inf).all()
+        assert torch.equal(out[rows:], good[rows:]) and torch.equal(lse[rows:], good_lse[rows:])
+    b.seqs._keep[1].copy_(ints([b.table.shape[1] * 16, 500]))
+    attend(ctx, b, q)
+    ctx.sync()                                       # the last position there is
