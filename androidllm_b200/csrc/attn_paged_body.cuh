@@ -137,6 +137,9 @@ ALM_DEV int4 record_of(const Unit& u, int cta, int n_cta, long long total) {
   return make_int4(last - cta + 1, u.row0, u.n_tok, u.h);
 }
 
+// x where it is infinite or NaN, else 0
+ALM_DEV float not_finite(float x) { return fabsf(x) < __int_as_float(0x7f800000) ? 0.f : x; }
+
 // V consecutive fp32 values behind L1 (another SM wrote them).
 template <int V>
 ALM_DEV void load_row(const float* p, float (&v)[V]) {
@@ -193,6 +196,22 @@ ALM_DEV void join_part(const AttnPaged& a, int cta, int n, int row, float& m, fl
       }
     }
   }
+  // an infinite part stays one, however small its weight
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < V; ++j) odd |= o[j] != o[j];
+  if (__any_sync(0xffffffffu, odd && l == l)) {
+    float x[V] = {};
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      float v[V];
+      load_row<V>(part(i) + row * HD + lane * V, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[j] += not_finite(v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = x[j] != 0.f ? x[j] : o[j];
+  }
 }
 template <typename T, int HD>
 ALM_DEV void join_store(const AttnPaged& a, int row, int head, float m, float l, const float (&o)[HD / 32]) {
@@ -231,45 +250,190 @@ __device__ __noinline__ void join_unit_here(const AttnPaged& a, int cta, int4 re
   join_unit<T, HD, ROWS, ROWS, 4>(a, cta, rec, warp, kPagedWarps);
 }
 
-// One row by one warp straight from the formula, skipping every position the
-// row does not see: for rows whose sums are not finite though their weights
-// are, since a hidden position's infinity or NaN times a zero weight spoils a
-// matrix product.
-template <typename T, int HD>
-__device__ __noinline__ void row_by_formula(const AttnPaged& a, const PagedKV& kv, const int* pages, int kv_head, int row,
-                                            int head, int p_lo, int p_hi, float (&o)[HD / 32], float& m, float& l) {
-  const int lane = threadIdx.x % kWarp;
-  const T* q = reinterpret_cast<const T*>(a.q + row * a.q_row + head * a.q_head);
-  float qv[HD / 32];
+// ---- infinities and NaN in V ----------------------------------------------------
+// A hidden position's weight is 0, and 0 times an infinity or NaN spoils its
+// column of the matrix product for rows that do not see it.  So a row whose sums
+// are not finite though its weights are is looked at again: a column of it in
+// which it sees an infinity or NaN is their sum (their weights are positive,
+// however small), and one in which it sees none is summed by the formula.  64
+// decodes over 2000 to 7670 positions, one of them with an infinity: 529 us
+// instead of 122.
+
+// A lane's V consecutive columns of a K or V row.
+template <typename T, int V>
+struct Columns {
+  static constexpr int kWords = V % 2 ? V : V / 2;
+  alignas(V == 8 ? 16 : V == 4 ? 8 : 4) uint32_t w[kWords];
+  ALM_DEV void load(const T* row) {
+    const T* p = row + threadIdx.x % kWarp * V;
+    if constexpr (V == 8) *reinterpret_cast<uint4*>(w) = __ldg(reinterpret_cast<const uint4*>(p));
+    else if constexpr (V == 4) *reinterpret_cast<uint2*>(w) = __ldg(reinterpret_cast<const uint2*>(p));
+    else if constexpr (V == 2) w[0] = __ldg(reinterpret_cast<const unsigned*>(p));
+    else
 #pragma unroll
-  for (int i = 0; i < HD / 32; ++i) {
-    qv[i] = Elem<T>::up(q[lane + 32 * i]);
-    o[i] = 0.f;
+      for (int i = 0; i < V; ++i) w[i] = __ldg(reinterpret_cast<const unsigned short*>(p) + i);
   }
-  m = kNegInf;
-  l = 0.f;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int p = p_lo; p <= p_hi; ++p) {
-      const int pi = page_of(kv, p);
-      const int page = pages ? __ldg(pages + pi) : -1;
-      const bool ok = page >= 0 && page < kv.n_pages;
-      const size_t off = ok ? kv_offset(kv, page, kv_head, p - pi * kv.page_size) : 0;
-      const T* k = reinterpret_cast<const T*>(kv.k) + off;
-      float s = 0.f;
+  ALM_DEV float at(int i) const {
+    const unsigned short h = static_cast<unsigned short>(V % 2 ? w[i] : i % 2 ? w[i / 2] >> 16 : w[i / 2]);
+    return Elem<T>::up(*reinterpret_cast<const T*>(&h));
+  }
+  // some bit is set where a value's exponent is all ones (infinity or NaN)
+  ALM_DEV uint32_t odd() const {
+    constexpr uint32_t kExp = std::is_same<T, half>::value ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t kOne = std::is_same<T, half>::value ? 0x04000400u : 0x00800080u;
+    uint32_t r = 0;
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) s = fmaf(qv[i], ok ? Elem<T>::up(k[lane + 32 * i]) : 0.f, s);
-      s = warp_sum(s);
-      if (pass == 0) {
-        m = fmaxf(m, s);
-        continue;
+    for (int i = 0; i < kWords; ++i) r |= (w[i] & kExp) + kOne;
+    return r & 0x80008000u;
+  }
+};
+
+// Byte offset of position p in K and V, -1 behind `end` and for pages outside the
+// pool.  (A lane finds a position's, and a warp then takes them from its lanes.)
+template <typename T>
+ALM_DEV long long place_at(const PagedKV& kv, const int* pages, int kv_head, int p, int end) {
+  if (p >= end || pages == nullptr) return -1;
+  const int pi = page_of(kv, p), page = __ldg(pages + pi);
+  if (page < 0 || page >= kv.n_pages) return -1;
+  return static_cast<long long>(kv_offset(kv, page, kv_head, p - pi * kv.page_size) * sizeof(T));
+}
+
+// Adds the infinities and NaN of V at positions [p0, p1) to x.  By a warp.
+template <typename T, int HD>
+ALM_DEV void gather_not_finite(const PagedKV& kv, const int* pages, int kv_head, int p0, int p1, float (&x)[HD / 32],
+                               volatile Waits* waits) {
+  constexpr int V = HD / 32, kDeep = 16;
+  const int lane = threadIdx.x % kWarp;
+  long long next = place_at<T>(kv, pages, kv_head, p0 + lane, p1);
+  for (int p = p0; p < p1; p += kWarp) {
+    const long long mine = next;
+    next = place_at<T>(kv, pages, kv_head, p + kWarp + lane, p1);
+    for (int j = 0; j < kWarp && p + j < p1; j += kDeep) {
+      // (the loads one after the other, so that all are under way together)
+      long long at[kDeep];
+      Columns<T, V> v[kDeep];
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) at[d] = __shfl_sync(0xffffffffu, mine, j + d);
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) v[d].load(reinterpret_cast<const T*>(kv.v + max(at[d], 0ll)));
+      uint32_t odd = 0;
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) odd |= at[d] < 0 ? 0 : v[d].odd();
+      if (__any_sync(0xffffffffu, odd != 0)) {
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[i] += at[d] < 0 ? 0.f : not_finite(v[d].at(i));
       }
-      const float w = ex2((s - m) * a.scale_log2);
-      l += w;
-      const T* v = reinterpret_cast<const T*>(kv.v) + off;
+    }
+    if (p % 4096 < kWarp) waits->beat = waits->beat + 1;
+  }
+}
+
+// Adds 2^(c (s - m)) inv V, V's infinities and NaN left out, at positions [p0, p1)
+// to o.  By a warp: the scores a position a lane, the sums V columns a lane.
+template <typename T, int HD>
+ALM_DEV void sum_by_formula(const AttnPaged& a, const PagedKV& kv, const int* pages, int kv_head, const T* q, int p0, int p1,
+                            float m, float inv, float (&o)[HD / 32], volatile Waits* waits) {
+  constexpr int V = HD / 32, kDeep = 8;
+  const int lane = threadIdx.x % kWarp;
+  for (int p = p0; p < p1; p += kWarp) {
+    const long long mine = place_at<T>(kv, pages, kv_head, p + lane, p1);
+    float w = 0.f;
+    if (mine >= 0) {
+      const uint4* k = reinterpret_cast<const uint4*>(kv.k + mine);
+      float s = 0.f;
+#pragma unroll 8
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 x = __ldg(k + c), y = __ldg(reinterpret_cast<const uint4*>(q) + c);
+        const T *xs = reinterpret_cast<const T*>(&x), *ys = reinterpret_cast<const T*>(&y);
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) o[i] = fmaf(w, ok ? Elem<T>::up(v[lane + 32 * i]) : 0.f, o[i]);
+        for (int i = 0; i < 8; ++i) s = fmaf(Elem<T>::up(xs[i]), Elem<T>::up(ys[i]), s);
+      }
+      w = ex2((s - m) * a.scale_log2) * inv;
+    }
+    for (int j = 0; j < kWarp && p + j < p1; j += kDeep) {
+      long long at[kDeep];
+      Columns<T, V> v[kDeep];
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) at[d] = max(__shfl_sync(0xffffffffu, mine, j + d), 0ll);
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) v[d].load(reinterpret_cast<const T*>(kv.v + at[d]));
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) {
+        const float f = __shfl_sync(0xffffffffu, w, j + d);   // 0 where there is no page
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float y = v[d].at(i);
+          o[i] = fmaf(f, fabsf(y) < __int_as_float(0x7f800000) ? y : 0.f, o[i]);
+        }
+      }
+    }
+    if (p % 1024 < kWarp) waits->beat = waits->beat + 1;
+  }
+}
+
+// Rows r0 + step i of a block (bits i of todo; first packed row row0, first
+// position pos0), of which the CTA has summed positions [p0, p1) and which lie in
+// `part` (or, if that is null, in the output): what is not finite in them
+// is put right.  Lane i brings its row's m and inv (1 / l, or 1 in a partial
+// result).  By a warp; what all the rows see is read once for them.
+template <typename T, int HD>
+__device__ __noinline__ void mend_rows(const AttnPaged& a_, const PagedKV& kv_, const int* pages, int kv_head, int row0, int pos0,
+                                       int r0, int step, unsigned todo, float m, float inv, int p0, int p1, float* part,
+                                       volatile Waits* waits) {
+  constexpr int V = HD / 32;
+  const AttnPaged a = a_;   // (in registers: the loops would load them from the arguments every time)
+  const PagedKV kv = kv_;
+  const int lane = threadIdx.x % kWarp;
+  auto pos_of = [&](int i) { return pos0 + (r0 + step * i) / a.group; };
+  auto from = [&](int pos) { return max(p0, a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0); };
+  auto upto = [&](int pos) { return min(p1, pos + 1); };
+  int c0 = from(pos_of(31 - __clz(todo))), c1 = upto(pos_of(__ffs(todo) - 1));   // seen by all of them
+  if (c0 >= c1) c0 = c1 = p1;
+  float all[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) all[i] = 0.f;
+  gather_not_finite<T, HD>(kv, pages, kv_head, c0, c1, all, waits);
+  for (; todo; todo &= todo - 1) {
+    const int src = __ffs(todo) - 1, r = r0 + step * src, tok = r / a.group, pos = pos0 + tok;
+    const int head = kv_head * a.group + r - tok * a.group, s0 = from(pos), s1 = upto(pos);
+    float x[V], o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = all[i], o[i] = 0.f;
+    gather_not_finite<T, HD>(kv, pages, kv_head, s0, min(s1, c0), x, waits);
+    gather_not_finite<T, HD>(kv, pages, kv_head, max(s0, c1), s1, x, waits);
+    T* dst = reinterpret_cast<T*>(a.out + (row0 + tok) * a.out_row + head * a.out_head) + lane * V;
+    float* dst32 = part ? part + r * HD + lane * V : nullptr;
+    bool open = false;
+    unsigned bad = 0;   // columns that are not finite
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (not_finite(part ? dst32[i] : Elem<T>::up(dst[i])) != 0.f) {
+        bad |= 1u << i;
+        open |= x[i] == 0.f;
+      }
+    const float mr = __shfl_sync(0xffffffffu, m, src), ir = __shfl_sync(0xffffffffu, inv, src);
+    if (__any_sync(0xffffffffu, open))
+      sum_by_formula<T, HD>(a, kv, pages, kv_head, reinterpret_cast<const T*>(a.q + (row0 + tok) * a.q_row + head * a.q_head),
+                            s0, s1, mr == kNegInf ? 0.f : mr, ir, o, waits);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float y = x[i] != 0.f ? x[i] : o[i];
+      if (x[i] == 0.f && !(bad >> i & 1)) continue;
+      if (part) dst32[i] = y;
+      else dst[i] = Elem<T>::down(y);
     }
   }
+}
+
+// Two packed values, zero where they are not finite.  (attn_paged_tc_body.cuh)
+template <typename T>
+ALM_DEV uint32_t finite_only(uint32_t x) {
+  constexpr uint32_t kExp = std::is_same<T, half>::value ? 0x7c00u : 0x7f80u;   // all ones: infinity or NaN
+  if ((x & kExp) == kExp) x &= 0xffff0000u;
+  if ((x >> 16 & kExp) == kExp) x &= 0xffffu;
+  return x;
 }
 
 template <typename T, int HD, int WM, bool TMA>
@@ -283,7 +447,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   char* const smem = TMA ? smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023) : smem_raw;
   __shared__ SchedShared sched;
   __shared__ uint64_t full[S::kStages], empty[S::kStages];
-  __shared__ int dead_flag;   // a wait ran out: everybody leaves
+  __shared__ Waits waits_;
   __shared__ float st_m[kWK][kRows], st_l[kWK][kRows];
   __shared__ float row_m[kRows], row_l[kRows];
   __shared__ int row_bad[kRows];
@@ -300,9 +464,9 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
     if constexpr (TMA) bar_sync(1, kPagedThreads);
     else __syncthreads();
   };
+  if (tid == 0) waits_.dead = waits_.beat = 0;
   if (TMA && tid == kPagedThreads) {
     for (int i = 0; i < S::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], kPagedWarps);
-    dead_flag = 0;
     fence_mbar_init();
   }
   if (!TMA || warp < kPagedWarps)
@@ -327,9 +491,9 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
   Unit lu = u;
   int lt = t, ltb = tb;
   const uint32_t smem0 = smem_addr(smem);
-  volatile int* dead = &dead_flag;
+  volatile Waits* waits = &waits_;
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) {   // the same answer for the whole warp
-    const bool ok = mbar_try_wait(bar, parity & 1) || slow_wait(bar, parity & 1, dead, err);
+    const bool ok = mbar_try_wait(bar, parity & 1) || slow_wait(bar, parity & 1, waits, err);
     return __all_sync(0xffffffffu, ok) != 0;
   };
   if (TMA && warp == kPagedWarps) {
@@ -638,29 +802,15 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
       if (lane == 0) mbar_arrive(&empty[stage]);
     }
     if (some_bad) {
-      for (int row = warp; row < kRows; row += kPagedWarps) {
-        if (!row_bad[row] || row_l[row] != row_l[row]) continue;   // a NaN score that it sees spoils the whole row
-        const int tok = row / a.group, hh = row - tok * a.group, head = u.h * a.group + hh;
-        const int last = u.pos0 + tok;
-        const int p_lo = max((u.t0 + t_first) * kTile, a.window > 0 ? last - a.window + 1 : 0);
-        const int p_hi = min((u.t0 + t + 1) * kTile - 1, last);
-        float ov[HD / 32], mm, ll;
-        row_by_formula<T, HD>(a, kv, u.pages, u.h, u.row0 + tok, head, p_lo, p_hi, ov, mm, ll);
-        T* dst = reinterpret_cast<T*>(a.out + (u.row0 + tok) * a.out_row + head * a.out_head);
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-          if (whole) dst[lane + 32 * i] = Elem<T>::down(p_hi < p_lo ? 0.f : ov[i] / ll);
-          else part[row * HD + lane + 32 * i] = ov[i];
-        }
-        if (lane == 0) {
-          if (!whole) {
-            part[kRows * HD + row] = mm;
-            part[kRows * HD + kRows + row] = ll;
-          } else if (a.lse) {
-            a.lse[(u.row0 + tok) * a.lse_row + head] = (mm * a.scale_log2 + log2f(ll)) * 0.693147180559945309f;
-          }
-        }
-      }
+      // rows warp, warp + 8, .., one a lane (a NaN score that it sees spoils the whole row)
+      const int row = warp + lane * kPagedWarps;
+      const float l_row = row < kRows && row_bad[row] ? row_l[row] : __int_as_float(0x7fffffff);
+      const bool odd = l_row == l_row;
+      const unsigned todo = __ballot_sync(0xffffffffu, odd);
+      if (todo)
+        mend_rows<T, HD>(a, kv, u.pages, u.h, u.row0, u.pos0, warp, kPagedWarps, todo, odd ? row_m[row] : 0.f,
+                         odd && whole ? 1.f / l_row : 1.f, (u.t0 + t_first) * kTile, (u.t0 + t + 1) * kTile,
+                         whole ? nullptr : part, waits);
       // every warp has read its rows' marks before the next unit's end clears
       // them (a TMA ring lets a warp run whole units ahead of another)
       sync();

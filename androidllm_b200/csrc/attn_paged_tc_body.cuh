@@ -65,7 +65,8 @@ struct TcShared {
   uint64_t full[10], empty[10];
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], pv_done[2];
   uint32_t tmem;
-  int dead;      // a wait ran out: everybody leaves
+  Waits waits;
+  int lost;      // sums that were not finite
 };
 
 ALM_DEV uint64_t sdesc128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -169,7 +170,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         mbar_init(&sh.p_full[i][0], 128), mbar_init(&sh.p_full[i][1], 128);
         mbar_init(&sh.pv_done[i], 1);
       }
-      sh.dead = 0;
+      sh.waits.dead = sh.waits.beat = sh.lost = 0;
       fence_mbar_init();
     }
     __syncwarp();
@@ -196,10 +197,10 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
   const long long x1 = cta < n_cta ? share(total, cta + 1, n_cta) : 0;
 
   if (tid == 0) *join_record(a, cta) = make_int4(0, 0, 0, 0);
-  volatile int* dead = &sh.dead;
+  volatile Waits* waits = &sh.waits;
   // Waits are bounded: one that runs out marks the CTA dead, and every role leaves.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    return mbar_try_wait(bar, parity & 1) || slow_wait(bar, parity & 1, dead, err);
+    return mbar_try_wait(bar, parity & 1) || slow_wait(bar, parity & 1, waits, err);
   };
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) {   // the same answer for the whole warp
     const bool ok = wait(bar, parity);
@@ -226,9 +227,23 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     }
     ALM_DEV bool more() const { return u.more(x1); }
   };
+  // The CTA goes through its share once and, when sums were not finite though
+  // their weights were, a second time with zeros for the infinities and NaN of V,
+  // which the rows that see them then get; the barriers' phases and the counters
+  // go on.  512 rows over 30,512 positions, 28 heads over 4 of 128: 243 us, 1400 us
+  // with one infinity.  (Two copies of the code: a flag instead costs the first
+  // pass 8%.)
+  auto again = [&] {
+    bar_sync(4, kTcPagedThreads);
+    return *static_cast<volatile int*>(&sh.lost) != 0;
+  };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
+    uint32_t fills[2] = {0, 0};   // warp 9: of each ring
+    uint32_t n_q = 0;             // warp 10: units so far
+    uint32_t n_p = 0, n_u = 0;    // warps 8 and 11: tiles and units of the stream so far
+    auto pass = [&](auto careful) {
     Walk w;
     if (x0 < x1 && w.start(b, kv, tpu, a.window, sh.sched, x0, x1)) {
     Unit& u = w.u;
@@ -237,7 +252,6 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     auto more = [&] { return w.more(); };
     if (warp == 9) {
       // ---- loads ---------------------------------------------------------------
-      uint32_t fills[2] = {0, 0};   // of each ring
       bool bad = false, quit = false;
       const int n_box = 128 / box_rows * S::kChunks;
       auto load = [&](const CUtensorMap* map, int t, int ring) {
@@ -277,12 +291,11 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       // ---- Q: the tokens' heads of one K/V head are a box (columns, heads,
       // tokens), which is the packed order of the block's rows; tokens of the
       // next sequence that it may hold fill rows that nothing is written from
-      uint32_t n = 0;
       const uint32_t bytes = static_cast<uint32_t>(tq * a.group) * 128 * S::kChunks;
       bool quit = false;
-      for (bool go = true; go && !quit; ++n) {
+      for (bool go = true; go && !quit; ++n_q) {
         for (int i = 0; i < NQ && !quit; ++i) {
-          if (!wait_warp(&sh.q_empty[i], n ^ 1)) {
+          if (!wait_warp(&sh.q_empty[i], n_q ^ 1)) {
             quit = true;
             break;
           }
@@ -308,7 +321,6 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       const uint32_t id_s = tc_idesc<T>(128, false), id_o = tc_idesc<T>(HD, true);
       const uint32_t qa = smem0 + q_blk * S::kTileBytes;
       const uint32_t d_s = tmem + S::kColS + i * 128, d_o = tmem + S::kColO + i * HD;
-      uint32_t n_p = 0, n_u = 0;                       // tiles and units of the stream so far
       // K and V of the stream's n-th tile are fills 2 n and 2 n + 1 of its ring
       const uint32_t ring = NQ == 2 ? 0 : i * S::kRing;
       int t = ta, t_first = ta;
@@ -355,6 +367,17 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
           fence_proxy_async_smem();
           __syncwarp();
         }
+        if (decltype(careful)::value && !quit) {   // (both streams of a shared tile write the same zeros here too)
+          uint4* v = reinterpret_cast<uint4*>(smem + (NQ + at) * S::kTileBytes);
+#pragma unroll 4
+          for (int j = lane; j < S::kTileBytes / 16; j += kWarp) {
+            const uint4 x = v[j];
+            const uint4 y = make_uint4(finite_only<T>(x.x), finite_only<T>(x.y), finite_only<T>(x.z), finite_only<T>(x.w));
+            if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) v[j] = y;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         // the next tile's K before the weights: it is there long since, and
         // then nothing stands between this product and the next
         if (!last) k_ready(n_p + 1);
@@ -390,7 +413,7 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       };
       bool go = enter();
       if (go) {
-        k_ready(0);
+        k_ready(n_p);
         qk(-1);
       }
       while (go && !quit) {
@@ -411,8 +434,16 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       }
     }
     }
+    };
+    pass(std::false_type());
+    if (again()) pass(std::true_type());
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    const int st = warp / 4;                         // stream
+    uint32_t n_s = 0;                                // tiles of this stream so far
+    uint32_t n_u = 0, n_done = 0;                    // units so far, and those with a tile
+    if (NQ == 2 && st == 1) bar_arrive(2, 256);      // stream 0 has the first turn
+    auto pass = [&](auto careful) {
     Walk w;
     if (x0 < x1 && w.start(b, kv, tpu, a.window, sh.sched, x0, x1)) {
       Unit& u = w.u;
@@ -420,15 +451,10 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       auto next = [&] { w.next(b, kv, tpu, a.window); };
       auto more = [&] { return w.more(); };
       // ---- softmax -------------------------------------------------------------
-      const int st = warp / 4;                         // stream
       const int r = tid % 128;                         // row of the block = lane of tensor memory
       const uint32_t t_s = tc_addr(tmem + S::kColS + st * 128, (warp % 4) * 32, 0);
       const uint32_t t_o = tc_addr(tmem + S::kColO + st * HD, (warp % 4) * 32, 0);
       const int blk = NQ == 2 ? st : 0;                // 128-row block of the unit
-      uint32_t n_s = 0;                                // tiles of this stream so far
-      if (NQ == 2 && st == 1) bar_arrive(2, 256);      // stream 0 has the first turn
-
-      uint32_t n_u = 0, n_done = 0;                    // units so far, and those with a tile
       for (bool go = true; go;) {
         const Unit cu = u;
         const int ca = ta, cb = tb;
@@ -590,11 +616,11 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
         // Rows leave through the load that spreads a row over four lanes (two
         // columns of every eight each), so that a store covers whole 32-byte
         // sectors of 8 rows instead of half ones of 32.
-        unsigned spoilt[2][2] = {};
+        unsigned mine4 = 0;   // four lanes speak for a row: those of this lane's
         if (any_live) {
           const unsigned live_rows = __ballot_sync(0xffffffffu, live);
           const int g = lane / 4, t4 = lane % 4;
-#pragma unroll
+#pragma unroll 1   // (unrolled, the loops above get fewer registers: a prefill takes 2% longer)
           for (int hh = 0; hh < 2; ++hh) {
             char* d[2];        // of rows 16 hh + g and 16 hh + g + 8
             float s0[2], s1[2], zero[2] = {0.f, 0.f};
@@ -645,12 +671,12 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
               }
             }
 #pragma unroll
-            for (int k = 0; k < 2; ++k) spoilt[hh][k] = __ballot_sync(0xffffffffu, zero[k] != 0.f);
+            for (int k = 0; k < 2; ++k) {
+              const unsigned spoilt = __ballot_sync(0xffffffffu, zero[k] != 0.f);
+              if (lane / 16 == hh && lane / 8 % 2 == k) mine4 = spoilt;
+            }
           }
         }
-        // four lanes speak for a row
-        const unsigned mine4 = (lane & 16) ? ((lane & 8) ? spoilt[1][1] : spoilt[1][0])
-                                           : ((lane & 8) ? spoilt[0][1] : spoilt[0][0]);
         const bool odd = ((mine4 >> (4 * (lane & 7))) & 15u) != 0;
         tc_fence_before();
         if (live) {
@@ -662,40 +688,23 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
                 none ? kNegInf : (m * a.scale_log2 + log2f(l)) * 0.693147180559945309f;
           }
         }
-        // rows whose sums are not finite, by the formula
-        unsigned todo = __ballot_sync(0xffffffffu, odd && live && l == l);   // (a NaN score spoils its whole row)
-        while (todo) {
-          const int src = __ffs(todo) - 1;
-          todo &= todo - 1;
-          const int tok_s = __shfl_sync(0xffffffffu, tok, src), head_s = __shfl_sync(0xffffffffu, head, src);
-          const int row_s = __shfl_sync(0xffffffffu, prow, src);
-          const int last = cu.pos0 + tok_s;
-          const int p_lo = max((cu.t0 + ca) * S::kTile, a.window > 0 ? last - a.window + 1 : 0);
-          const int p_hi = min((cu.t0 + cb) * S::kTile - 1, last);
-          float ov[HD / 32], mm, ll;
-          row_by_formula<T, HD>(a, kv, cu.pages, cu.h, cu.row0 + tok_s, head_s, p_lo, p_hi, ov, mm, ll);
-          T* d = reinterpret_cast<T*>(a.out + (cu.row0 + tok_s) * a.out_row + head_s * a.out_head);
-#pragma unroll
-          for (int i = 0; i < HD / 32; ++i) {
-            if (whole) d[lane + 32 * i] = Elem<T>::down(p_hi < p_lo ? 0.f : ov[i] / ll);
-            else part[row_s * HD + lane + 32 * i] = ov[i];
-          }
-          if (lane == 0) {
-            if (!whole) {
-              part[NQ * 128 * HD + row_s] = mm;
-              part[NQ * 128 * HD + NQ * 128 + row_s] = ll;
-            } else if (a.lse) {
-              a.lse[(cu.row0 + tok_s) * a.lse_row + head_s] =
-                  (mm * a.scale_log2 + log2f(ll)) * 0.693147180559945309f;
-            }
-          }
+        // (a NaN score spoils its whole row)
+        if (!decltype(careful)::value && odd && live && l == l) sh.lost = 1;
+        if (decltype(careful)::value && any_live) {
+          __syncwarp();   // the warp's rows lie in memory
+          mend_rows<T, HD>(a, kv, cu.pages, cu.h, cu.row0 + blk * tq, pos_a, r - lane, 1,
+                           __ballot_sync(0xffffffffu, live && l == l), m, inv, (cu.t0 + ca) * S::kTile,
+                           (cu.t0 + cb) * S::kTile, whole ? nullptr : part + blk * 128 * HD, waits);
         }
       }
     }
+    };
+    pass(std::false_type());
+    if (again()) pass(std::true_type());
   }
   // a wait that ran out has left products in flight: give them time, then free
   __syncthreads();
-  if (*dead && tid == 0) {
+  if (waits->dead && tid == 0) {
     mbar_wait(&sh.pv_done[0], 0), mbar_wait(&sh.pv_done[0], 1);
     mbar_wait(&sh.pv_done[1], 0), mbar_wait(&sh.pv_done[1], 1);
   }

@@ -43,15 +43,27 @@ ALM_DEV bool bar_or(int id, int n, bool p) {
 ALM_DEV void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 ALM_DEV void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
+// What the waits of a CTA have in common.  dead: one ran out, and everybody
+// leaves.  beat: counts the steps of work that no barrier shows (results with
+// infinities made again); a wait's time starts anew with each.
+struct Waits {
+  int dead, beat;
+};
 // The rest of a wait whose first look failed: true when the phase completed.
-ALM_DEV bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* err) {
-  const unsigned long long t0 = global_ns();
+ALM_DEV bool slow_wait(uint64_t* bar, uint32_t parity, volatile Waits* w, int* err) {
+  unsigned long long t0 = global_ns();
+  int beat = w->beat;
   for (unsigned i = 0; i < kSpinLimit; ++i) {
     if (mbar_try_wait_suspend(bar, parity)) return true;
-    if (*dead) return false;
+    if (w->dead) return false;
+    if (w->beat != beat) {
+      beat = w->beat;
+      t0 = global_ns();
+      i = 0;
+    }
     if (global_ns() - t0 > kWaitLimitNs) break;
   }
-  *dead = 1;
+  w->dead = 1;
   *err = 2;
   return false;
 }

@@ -1158,3 +1158,82 @@ def test_attend_length_beyond_the_table_is_reported(ctx, rows, dim):
     b.seqs._keep[1].copy_(ints([b.table.shape[1] * 16, 500]))
     attend(ctx, b, q)
     ctx.sync()                                       # the last position there is
+
+
+def check_not_finite(ctx, b, q, marks, window=0, times=1):
+    """Rows with infinities and NaN in V at marks = (sequence, position, column,
+    value): a row that sees one has it in that column (opposite infinities: NaN),
+    everything else is the formula's."""
+    for s, pos, col, value in marks:
+        not_finite_at(b, s, pos, value, col)
+    ref, tol, _, _ = formula(b, q, b.dim ** -0.5, window)
+    for s, pos, col, value in marks:
+        for r in range(b.rows[s]):
+            p = b.lens[s] - b.rows[s] + r
+            if pos <= p and not (window and pos <= p - window):
+                ref[b.start[s] + r, :, col] += value
+    own = slice(b.start[0], b.start[-1])
+    ref, tol = ref[own], tol[own]
+    some = torch.isfinite(ref)
+    for _ in range(times):
+        out, lse = attend(ctx, b, q, window)
+        ctx.sync()                                   # no wait ran out
+        got = out[own].double()
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        assert torch.equal(got[~some & ~torch.isnan(ref)], ref[~some & ~torch.isnan(ref)])
+        assert ((got - ref).abs()[some] <= tol[some]).all()
+        assert torch.isfinite(lse[own]).all()
+        assert (out[b.start[-1]:] == 77).all()
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 7, 28, 300])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_attend_infinities_over_a_long_context(ctx, dtype, rows, dim):
+    n = 30000 if dim in (64, 128) else 6000
+    b = Batch([rows, 2], [n + rows, 500], 16, 1, dim, DT[dtype], seed=45)
+    marks = [(0, n // 6, 7, INF), (0, n // 6 + 1, 8, -INF), (0, 3, 9, INF), (0, n - 9, 9, -INF), (0, n // 2, 31, NAN),
+             (0, n + rows // 2, 11, NAN), (0, n + rows // 2, 12, INF), (1, 450, 1, INF), (1, 499, 2, -INF)]
+    check_not_finite(ctx, b, b.randn(b.n_rows, 4, dim), marks, times=2)
+
+
+@pytest.mark.parametrize("window", [1, 40, 200, 1000])
+@pytest.mark.parametrize("rows", [[3, 7, 1], [70, 30, 300]])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_attend_infinities_at_the_window_border(ctx, window, rows, dim):
+    """Values that some rows of a block see and others do not, on both sides."""
+    lens = [r + n for r, n in zip(rows, (2000, 90, 700))]
+    b = Batch(rows, lens, 32, 2, dim, torch.float16, seed=46)
+    marks = []
+    for s in range(3):
+        for i, (back, value) in enumerate([(0, NAN), (rows[s] // 2, INF), (rows[s] + 1, -INF), (window, NAN),
+                                           (window + rows[s] // 2, INF), (window + rows[s], -INF), (1, -INF)]):
+            if 0 <= lens[s] - 1 - back:
+                marks.append((s, lens[s] - 1 - back, 5 * i + s, value))
+    check_not_finite(ctx, b, b.randn(b.n_rows, 6, dim), marks, window)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 60])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_infinity_of_a_tiny_weight(ctx, rows, dim):
+    """The weight of a visible infinity is never zero, also below what 16 or 32 bits hold."""
+    n = 40000
+    b = Batch([rows], [n], 16, 1, dim, torch.float16, seed=47)
+    q = b.randn(b.n_rows, 2, dim).abs() + 1
+    # weights of less than 2^-126 before position 12000
+    pages = b.table[0, :750].long()
+    b.k[pages] = -abs(b.k[pages]) - 8
+    check_not_finite(ctx, b, q, [(0, 100, 3, INF), (0, 11000, 4, -INF), (0, n - 1, 5, INF)])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [10, 50, 90])
+def test_attend_not_finite_in_every_unit(ctx, dim, rows):
+    """Many sequences, each with values that only some of its rows see: every unit is made twice."""
+    n = 300
+    b = Batch([rows - i % 3 for i in range(n)], [rows + (i * 37) % 400 for i in range(n)], 16, 1, dim, torch.bfloat16, seed=48)
+    marks = [(s, b.lens[s] - 1 - s % rows, s % 32, (INF, -INF, NAN)[s % 3]) for s in range(n)]
+    check_not_finite(ctx, b, b.randn(b.n_rows, 3, dim), marks, times=2)
