@@ -34,6 +34,12 @@ namespace alm {
 constexpr int kPagedThreads = 256;
 constexpr int kJoinThreads = 128;
 constexpr int kPagedWarps = kPagedThreads / kWarp;
+// A weight is 2^(c s - round(c m)), one multiply-add a score.  What round()
+// leaves scales a chunk's weights by up to 2^(2^-24 c m): 2^-14 at this
+// |c m|, a quarter of fp16's half step.  Beyond it (at 2^28 every weight would be
+// 0 or infinite) m is taken off the scores first: c (s - m) is 0 at the maximum
+// whatever c is.
+constexpr float kFarScore = 1024.f;
 
 template <typename T>
 struct Elem;
@@ -654,7 +660,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
             s[n][j] = seen ? s[n][j] : kNegInf;
           }
       }
-      float mc[2];
+      float mc[2], base[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float x_ = m[j];
@@ -662,16 +668,23 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_consta
         for (int n = 0; n < kChunk / 8; ++n) x_ = fmaxf(x_, fmaxf(s[n][2 * j], s[n][2 * j + 1]));
         x_ = fmaxf(x_, __shfl_xor_sync(0xffffffffu, x_, 1));
         x_ = fmaxf(x_, __shfl_xor_sync(0xffffffffu, x_, 2));
-        const float base = x_ == kNegInf ? 0.f : x_;   // nothing seen yet: every weight is exp(-inf)
-        const float f = ex2((m[j] - base) * a.scale_log2);
+        base[j] = x_ == kNegInf ? 0.f : x_;   // nothing seen yet: every weight is exp(-inf)
+        const float f = ex2((m[j] - base[j]) * a.scale_log2);
         m[j] = x_;
-        mc[j] = base * a.scale_log2;
+        mc[j] = base[j] * a.scale_log2;
         l[j] *= f;
 #pragma unroll
         for (int n = 0; n < HD / 8; ++n) {
           o[n][2 * j] *= f;
           o[n][2 * j + 1] *= f;
         }
+      }
+      if (__any_sync(0xffffffffu, fmaxf(fabsf(mc[0]), fabsf(mc[1])) > kFarScore)) {
+#pragma unroll
+        for (int n = 0; n < kChunk / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[n][j] -= base[j >> 1];
+        mc[0] = mc[1] = 0.f;
       }
 #pragma unroll
       for (int n = 0; n < kChunk / 8; ++n)

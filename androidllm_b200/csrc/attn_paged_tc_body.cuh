@@ -66,7 +66,7 @@ struct TcShared {
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], pv_done[2];
   uint32_t tmem;
   Waits waits;
-  int lost;      // sums that were not finite
+  int lost;      // sums that were not finite, or large scores: go through the share again
 };
 
 ALM_DEV uint64_t sdesc128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -227,10 +227,11 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     }
     ALM_DEV bool more() const { return u.more(x1); }
   };
-  // The CTA goes through its share once and, when sums were not finite though
-  // their weights were, a second time with zeros for the infinities and NaN of V,
-  // which the rows that see them then get; the barriers' phases and the counters
-  // go on.  512 rows over 30,512 positions, 28 heads over 4 of 128: 243 us, 1400 us
+  // The CTA goes through its share once.  It does so a second time when sums were
+  // not finite though their weights were, with zeros for the infinities and NaN of
+  // V, which the rows that see them then get; or when scores were beyond kFarScore,
+  // and takes the maximum off them before they are scaled.  The barriers' phases
+  // and the counters go on.  512 rows over 30,512 positions, 28 heads over 4 of 128: 243 us, 1400 us
   // with one infinity.  (Two copies of the code: a flag instead costs the first
   // pass 8%.)
   auto again = [&] {
@@ -503,13 +504,19 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
             tc_landed(sr[3]);
             if (mask) hide(1);
             row_top = fmaxf(row_top, max64(sr[2], sr[3]));
+            // (m moves rarely: no test in every tile; rows behind the block's tokens hold anything)
+            auto note_far = [&] {
+              if (!decltype(careful)::value && live && m != kNegInf && fabsf(m * a.scale_log2) > kFarScore) sh.lost = 1;
+            };
             if (n_mine == 0) {
               m = row_top;
+              note_far();
             } else {
               const bool grow = row_top > m && !((row_top - m) * a.scale_log2 <= kSlack);
               if (__any_sync(0xffffffffu, grow)) {
                 const float f = grow ? ex2((m - row_top) * a.scale_log2) : 1.f;
                 if (grow) m = row_top;
+                note_far();
                 l *= f;
                 // (the scores' commit covers the product before them, so O is at rest)
 #pragma unroll 1
@@ -523,8 +530,8 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
                 }
               }
             }
-            const float mc = m == kNegInf ? 0.f : m * a.scale_log2;
-            const uint64_t c2 = pair(a.scale_log2, a.scale_log2), m2 = pair(-mc, -mc);
+            const float base = m == kNegInf ? 0.f : m, mc = base * a.scale_log2;
+            const uint64_t c2 = pair(a.scale_log2, a.scale_log2), m2 = decltype(careful)::value ? pair(-base, -base) : pair(-mc, -mc);
             uint64_t sum[2] = {0, 0};   // (+0, +0)
             uint32_t pr[2][32];
             auto weights = [&](int h, int j0, int j1) {
@@ -532,8 +539,8 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
               for (int j = j0; j < j1; ++j) {
                 const int e = 64 * h + 2 * j;
                 float p, q;
-                unpair(fma2(pair(__uint_as_float(sr[e / 32][e % 32]), __uint_as_float(sr[e / 32][e % 32 + 1])), c2, m2),
-                       p, q);
+                const uint64_t s2 = pair(__uint_as_float(sr[e / 32][e % 32]), __uint_as_float(sr[e / 32][e % 32 + 1]));
+                unpair(decltype(careful)::value ? mul2(add2(s2, m2), c2) : fma2(s2, c2, m2), p, q);
                 p = ex2(p);
                 q = ex2(q);
                 sum[j & 1] = add2(sum[j & 1], pair(p, q));

@@ -1237,3 +1237,48 @@ def test_attend_not_finite_in_every_unit(ctx, dim, rows):
     b = Batch([rows - i % 3 for i in range(n)], [rows + (i * 37) % 400 for i in range(n)], 16, 1, dim, torch.bfloat16, seed=48)
     marks = [(s, b.lens[s] - 1 - s % rows, s % 32, (INF, -INF, NAN)[s % 3]) for s in range(n)]
     check_not_finite(ctx, b, b.randn(b.n_rows, 3, dim), marks, times=2)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,heads,dim", [([1, 3, 1], 4, 64), ([5, 1, 2], 12, 96), ([200, 90, 1], 4, 64),
+                                            ([40, 33, 2], 4, 128)])
+@pytest.mark.parametrize("scale", [1e7, 1e9, 1e30])
+def test_attend_scales_that_leave_one_weight(ctx, dtype, rows, heads, dim, scale):
+    """Whole-number scores times a large scale: a row is the mean of the V of its
+    largest scores.  Scores and weights (0 or 1) are exact, so the output is off by
+    its own half step, a quotient and a few sums; lse by three roundings of itself."""
+    lens = [r + n for r, n in zip(rows, (0, 700, 2))]
+    b = Batch(rows, lens, 16, 2, dim, DT[dtype], seed=44)
+    b.k.copy_(torch.randint(-3, 4, b.k.shape, generator=b.gen, device="cuda"))
+    q = torch.randint(-3, 4, (b.n_rows, heads, dim), generator=b.gen, device="cuda").to(DT[dtype])
+    out, lse = attend(ctx, b, q, scale=scale)
+    ctx.sync()
+    for s in range(3):
+        k, v = b.cached(s)
+        pos = torch.arange(lens[s] - rows[s], lens[s], device="cuda")
+        hidden = torch.arange(lens[s], device="cuda")[None] > pos[:, None]
+        for h in range(heads):
+            kh, vh = k[h // (heads // 2)], v[h // (heads // 2)]
+            sc = (q[b.start[s]:b.start[s + 1], h].double() @ kh.T).masked_fill(hidden, -math.inf)
+            top = sc.amax(1, keepdim=True)
+            w = (sc == top).double()
+            ref, big = (w @ vh) / w.sum(1, keepdim=True), (w @ vh.abs()) / w.sum(1, keepdim=True)
+            got = out[b.start[s]:b.start[s + 1], h].double()
+            tol = torch.finfo(DT[dtype]).eps / 2 * ref.abs() + 2.0 ** -20 * big + 2.0 ** -25
+            assert ((got - ref).abs() <= tol).all()
+            # (the scale is used in 32 bits, times log2 e and back)
+            rl = top[:, 0] * float(np.float32(scale)) + torch.log(w.sum(1))
+            assert ((lse[b.start[s]:b.start[s + 1], h].double() - rl).abs() <= 2.0 ** -20 * rl.abs() + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_attend_is_the_same_after_large_scores(ctx, rows):
+    """What an earlier call left on chip (here: large scores) changes no bit of a result."""
+    b = Batch([rows, rows], [2000, 300], 16, 2, 128, torch.float16, seed=49)
+    q = b.randn(b.n_rows, 14, 128)                   # 7 heads: two of 128 rows stay unused
+    first, first_lse = attend(ctx, b, q)
+    for scale in (1e9, 0.05, 1e30):
+        attend(ctx, b, (q.float() * 300).half(), scale=scale)
+        out, lse = attend(ctx, b, q)
+        assert torch.equal(out, first) and torch.equal(lse, first_lse)
+    ctx.sync()
