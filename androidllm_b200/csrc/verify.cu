@@ -8,10 +8,13 @@
 //
 // Answers are whole numbers, so values next to a border decide them: every
 // comparison is made in 64 bits.  Z of every row is first summed from 32-bit
-// exponentials (relative error below 1e-5: at most 6e-8 of |x| <= 104 from the
-// product and the instruction's 2^-22 per term), which decides all but the
-// comparisons within kNear of equality; those, and the row the token is drawn
-// from, sum Z again with 64-bit weights.
+// exponentials, which decides all but the comparisons within kNear + kNearBlock n
+// of equality, n the blocks of 8 entries that a lane adds up at most; those, and
+// the row the token is drawn from, sum Z again with 64-bit weights.  The sums'
+// relative error is below 1e-5 (at most 6e-8 of |x| <= 104 from the product and
+// the instruction's 2^-22 per term) and, for each block, 2^-24 for its addition
+// and 3e-7 for the factor when the maximum grows, or 8 additions of 2^-24 (min-p):
+// 5e-7.  n is 75 at 151,936 tokens, 8192 at the largest vocabulary.
 //
 // The CTAs of a cluster own consecutive slices of the vocabulary and exchange
 // maxima and sums through distributed shared memory.  A lane takes 8
@@ -40,7 +43,7 @@ constexpr int kVerThreads = 512;
 constexpr int kVerWarps = kVerThreads / kWarp;
 constexpr int kVerRows = 32;        // k_max + 1 at most
 constexpr int kVerBlock = 8 * kWarp;   // entries a warp takes at a time
-constexpr double kNear = 1e-4;
+constexpr double kNear = 1e-4, kNearBlock = 5e-7;
 
 struct VerShared {
   double table[256 * 16];   // 2^(i / 256), 16 copies side by side
@@ -443,6 +446,8 @@ __global__ void __launch_bounds__(kVerThreads, kPerSm) verify_kernel(const Verif
   int acc = 0;
   double z_stop = 0.0;
   bool have_z = false;
+  // (from the slices' width, not this CTA's slice: the cluster decides alike)
+  const double near_p = kNear + kNearBlock * ((width + kVerBlock - 1) / kVerBlock);
   {
     double p = 0.0, uq = 0.0, z = 0.0;
     const bool in = xi >= 0 && xi < a.vocab;
@@ -458,7 +463,7 @@ __global__ void __launch_bounds__(kVerThreads, kPerSm) verify_kernel(const Verif
         uq = __ldg(a.u + static_cast<size_t>(s) * (a.k_max + 1) + lane) * q;
         z = sh.row_z[lane];
         p = e > 0.0 ? e / z : 0.0;
-        open = fabs(uq - p) <= kNear * p || (min_p > 0.0 && sh.row_i[lane] != 0);
+        open = fabs(uq - p) <= near_p * p || (min_p > 0.0 && sh.row_i[lane] != 0);
       }
     }
     unsigned yes = __ballot_sync(0xffffffffu, lane < k && uq < p);
@@ -478,8 +483,9 @@ __global__ void __launch_bounds__(kVerThreads, kPerSm) verify_kernel(const Verif
       }
       if (!(yes >> acc & 1)) break;
     }
-    // (behind the first refusal p is reported from the 32-bit sums, but for
-    // entries at the min-p border, which only the 64-bit weights tell apart)
+    // (p is reported from the 32-bit sums where they decided and behind the first
+    // refusal, but for rows with entries at the min-p border, which only the
+    // 64-bit weights tell apart)
     for (int i = acc + 1; i < k; ++i)
       if (min_p > 0.0 && sh.row_i[i] != 0 && !greedy) {
         const double zx = exact_sum(i);

@@ -1282,3 +1282,33 @@ def test_attend_is_the_same_after_large_scores(ctx, rows):
         out, lse = attend(ctx, b, q)
         assert torch.equal(out, first) and torch.equal(lse, first_lse)
     ctx.sync()
+
+
+def test_verify_border_in_the_largest_vocabulary(ctx):
+    """2^24 tokens of one probability but one.  Added one at a time in 32 bits a
+    lane's 65536 weights of 0.998 fall short by 49% of a step each behind 2^15: by
+    1e-3 of the sum.  Draws closer to p than that are still decided right."""
+    vocab, k = 1 << 24, 15
+    logits = torch.zeros(k + 1, vocab, device="cuda", dtype=torch.float16)
+    logits[:, 5] = 1.0
+    c = 255.49 / 256
+    temp = np.float32(-1.0 / math.log(c))
+    c = math.exp(-1.0 / float(temp))
+    z = 1.0 + (vocab - 1) * c
+    n_seq = 9                                        # the other sequences have no rows
+    start = [0] + [k + 1] * n_seq
+    draft = np.full((n_seq, k), 12345)
+    for off, want in ((1 + 3e-4, 0), (1 - 3e-4, k), (1 + 1e-9, 0), (1 - 1e-9, k)):
+        u = np.full((n_seq, k + 1), c / z * off)
+        u[:, k] = 0.37
+        tok, acc, pd = run_verify(ctx, start, logits, draft, None, u, np.full(n_seq, temp), np.full(n_seq, 1e-3))
+        assert acc.tolist() == [want] + [0] * (n_seq - 1)
+        # the draw: after a refusal without the drafted token's mass
+        if want == k:
+            at = 0.37 * z
+            first = int((at - 1.0) // c) + 1         # token 5 weighs 1, those before it c each
+        else:
+            at = 0.37 * (z - c)
+            first = int((at - 1.0) // c) + 2
+        assert tok[0, want].item() == first and tok[0, :want].tolist() == [12345] * want
+        np.testing.assert_allclose(pd[0].cpu().numpy(), c / z, rtol=1e-4 + 5e-7 * 8192)
