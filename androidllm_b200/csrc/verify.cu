@@ -410,11 +410,11 @@ __global__ void __launch_bounds__(kVerThreads, kPerSm) verify_kernel(const Verif
     all_rows(
         [&](int i, int, const Raw8<T>& v) {
           const float top = sh.row_m[i];
-          const bool inf = !(top < -kNegInf);
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const float f = value_of<T>(v.bits(q));
-            const float e = inf && f == top ? 1.f : ex2f_((f - top) * k_log2);   // NaN: below every bound
+            // (0 times an infinite 1 / T, and inf - inf, are NaN; a NaN logit is below every bound)
+            const float e = f == top ? 1.f : ex2f_((f - top) * k_log2);
             near |= fabsf(e - cut) <= band;
             z += e >= cut ? e : 0.f;
           }

@@ -1312,3 +1312,17 @@ def test_verify_border_in_the_largest_vocabulary(ctx):
             first = int((at - 1.0) // c) + 2
         assert tok[0, want].item() == first and tok[0, :want].tolist() == [12345] * want
         np.testing.assert_allclose(pd[0].cpu().numpy(), c / z, rtol=1e-4 + 5e-7 * 8192)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_verify_denormal_temperatures(ctx, dtype):
+    """All mass on the largest logits, also where 1 / T leaves 32 bits."""
+    rng, start, lg, draft, q, u = verify_case(72, [2] * 6, 2, 600)
+    lg[3:6, 5::7] = -np.inf
+    lg[9:12] = -np.inf
+    lg = lg.astype(np.float16).astype(np.float64)
+    draft[0], draft[2] = lg[start[0]:start[0] + 2].argmax(1), lg[start[2]:start[2] + 2].argmax(1)
+    for temp in (1e-37, 1e-39, 1e-42, 1e-45):
+        for min_p in (0.0, 0.3, 1.0):
+            check_verify(ctx, start, torch.tensor(lg, device="cuda").to(DT[dtype]), draft, q, u, np.full(6, temp),
+                         np.full(6, min_p))
