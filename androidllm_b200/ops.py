@@ -547,7 +547,7 @@ class DeviceKV:
         """The page table on the device (a row per slot) for ``paged.SeqBatch``."""
         from . import paged
         _, table, rows, pages = self._view(0)
-        return paged.PageTable(table, rows, pages, self)
+        return paged.PageTable(table, rows, pages, self, self.model.ctx.device)
 
     def _view(self, layer):
         view, table, rows, pages = PagedKVView(), ctypes.c_void_p(), ctypes.c_int32(), ctypes.c_int32()

@@ -29,6 +29,13 @@ _CODES = {}                       # dtype object -> code
 _SIZES = {F16: 2, BF16: 2, F32: 4, I32: 4, F64: 8}
 
 
+class _Device:
+    type = "cuda"
+
+    def __init__(self, index):
+        self.index = index
+
+
 class DeviceArray:
     """A typed, shaped view of device memory of the library (``buf``: an
     ``ops.DeviceBuffer``; ``offset`` in bytes; contiguous)."""
@@ -38,6 +45,10 @@ class DeviceArray:
         size = _SIZES[_code(dtype)]
         if self.offset < 0 or self.offset + int(np.prod(self.shape, dtype=np.int64)) * size > buf.nbytes:
             raise ValueError("the view ends behind its buffer")
+
+    @property
+    def device(self):
+        return _Device(self.buf.ctx.device)
 
     def data_ptr(self):
         return self.buf.h.value + self.offset
@@ -79,7 +90,7 @@ def _array(a, what, codes, ndim, device=None):
             if getattr(dev, "type", "cuda") != "cuda":
                 raise ValueError(f"{what} must be on a CUDA device")
             if device is not None and dev.index is not None and dev.index != device:
-                raise ValueError(f"{what} is on device {dev.index}, the context on device {device}")
+                raise ValueError(f"{what} is on device {dev.index}, not on device {device}")
         p, shape, stride, code = a.data_ptr(), a.shape, a.stride(), _code(a.dtype)
     elif hasattr(a, "__cuda_array_interface__"):
         i = a.__cuda_array_interface__
@@ -161,9 +172,13 @@ def _on(ctx, *views):
             raise ValueError(f"the {type(v).__name__} is on device {v.device}, the context on device {ctx.device}")
 
 
-def _device_of(a):
-    dev = getattr(a, "device", None)
-    return getattr(dev, "index", None)
+def _device_of(*arrays):
+    """The device of the first array that tells one."""
+    for a in arrays:
+        index = getattr(getattr(a, "device", None), "index", None)
+        if index is not None:
+            return index
+    return None
 
 
 class PagedKV:
@@ -171,6 +186,7 @@ class PagedKV:
     contiguous, fp16 or bf16.  ``DeviceKV.view(layer)`` gives a model's own."""
 
     def __init__(self, k, v, device=None):
+        self.device = device = _device_of(k, v) if device is None else device
         kp, code, shape = _contiguous(k, "k", (F16, BF16), 4, device)
         vp, vcode, vshape = _contiguous(v, "v", (F16, BF16), 4, device)
         if vcode != code or tuple(vshape) != tuple(shape):
@@ -179,7 +195,6 @@ class PagedKV:
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = (int(n) for n in shape)
         self.c = PagedKVView(kp, vp, code, self.n_pages, self.page_size, self.kv_heads, self.head_dim)
         self.ref = ctypes.addressof(self.c)
-        self.device = _device_of(k) if device is None else device
         self._keep = (k, v)
 
     @classmethod
@@ -198,8 +213,8 @@ class PageTable:
     """The page table of a model's cache (``DeviceKV.page_table()``): row s
     holds slot s's page numbers."""
 
-    def __init__(self, pointer, rows, pages, keep):
-        self.pointer, self.rows, self.pages, self._keep = pointer, rows, pages, keep
+    def __init__(self, pointer, rows, pages, keep, device=None):
+        self.pointer, self.rows, self.pages, self._keep, self.device = pointer, rows, pages, keep, _Device(device)
 
 
 class SeqBatch:
@@ -214,12 +229,15 @@ class SeqBatch:
     can be replayed with new contents."""
 
     def __init__(self, row_start, kv_len, page_table, n_rows, max_rows=None, slots=None, device=None):
+        self.device = device = _device_of(row_start, kv_len, page_table, slots) if device is None else device
         rp, _, rs = _contiguous(row_start, "row_start", (I32,), 1, device)
         lp, _, ls = _contiguous(kv_len, "kv_len", (I32,), 1, device)
         n_seq = int(ls[0])
         if rs[0] != n_seq + 1:
             raise ValueError("row_start must have one entry more than kv_len")
         if isinstance(page_table, PageTable):
+            if page_table.device.index not in (None, device):
+                raise ValueError(f"page_table is on device {page_table.device.index}, not on device {device}")
             tp, rows, pages, step = page_table.pointer, page_table.rows, page_table.pages, page_table.pages
         else:
             tp, _, shape, stride = _array(page_table, "page_table", (I32,), 2, device)
@@ -242,7 +260,6 @@ class SeqBatch:
         most = self.n_rows if max_rows is None else int(max_rows)
         self.c = SeqBatchView(n_seq, self.n_rows, most, rows, pages, step, rp, lp, tp, sp)
         self.ref = ctypes.addressof(self.c)
-        self.device = _device_of(row_start) if device is None else device
         self._keep = (row_start, kv_len, page_table, slots)
 
 

@@ -240,3 +240,48 @@ def test_packed_arguments_are_the_structs(args, pack):
 
 def test_empty_arrays_are_contiguous():
     assert paged._dense((2, 0), (1, 1)) and paged._dense((0, 5), (7, 1)) and not paged._dense((2, 3), (4, 1))
+
+
+class Gpu0:
+    type, index = "cuda", 0
+
+
+class Buffer:
+    """Memory of a context, in name only."""
+
+    def __init__(self, device):
+        class Ctx:
+            pass
+
+        class Handle:
+            value = P
+        self.ctx, self.h, self.nbytes = Ctx(), Handle(), 1 << 20
+        self.ctx.device = device
+
+
+@pytest.mark.parametrize("make", [
+    lambda: paged.PagedKV(Fake((4, 2, 16, 64), device=Gpu0), Fake((4, 2, 16, 64), device=Gpu1)),
+    lambda: _seqs(row_start=Fake((3,), "int32", device=Gpu0), kv_len=Fake((2,), "int32", device=Gpu1)),
+    lambda: _seqs(row_start=Fake((3,), "int32", device=Gpu0), page_table=Fake((2, 4), "int32", device=Gpu1)),
+    lambda: _seqs(row_start=Fake((3,), "int32", device=Gpu1), slots=Fake((2,), "int32", device=Gpu0)),
+    lambda: _seqs(row_start=Fake((3,), "int32", device=Gpu0), page_table=paged.PageTable(P, 2, 4, None, device=1)),
+    lambda: _seqs(row_start=Fake((3,), "int32", device=Gpu0), kv_len=paged.DeviceArray(Buffer(1), (2,), "int32")),
+    lambda: paged.PagedKV(paged.DeviceArray(Buffer(0), (1, 2, 16, 64), "float16"), Fake((1, 2, 16, 64), device=Gpu1)),
+])
+def test_views_refuse_arrays_of_different_devices(make):
+    with pytest.raises(ValueError, match="device"):
+        make()
+
+
+def test_views_know_their_device():
+    kv = paged.PagedKV(Fake((4, 2, 16, 64)), Fake((4, 2, 16, 64), device=Gpu1))
+    assert kv.device == 1
+    assert paged.PagedKV(*[paged.DeviceArray(Buffer(1), (1, 2, 16, 64), "float16")] * 2).device == 1
+    seqs = _seqs(page_table=paged.PageTable(P, 2, 4, None, device=1))
+    assert seqs.device == 1
+    with pytest.raises(ValueError, match="device"):      # NoContext is on device 0
+        paged.rope_append(NoContext, kv, _seqs(), Fake((5, 4, 64)), Fake((5, 2, 64)), Fake((5, 2, 64)), Fake((9, 64)),
+                          Fake((5, 4, 64)))
+    with pytest.raises(ValueError, match="device"):
+        paged.rope_append(NoContext, _cache(), seqs, Fake((5, 4, 64)), Fake((5, 2, 64)), Fake((5, 2, 64)), Fake((9, 64)),
+                          Fake((5, 4, 64)))
