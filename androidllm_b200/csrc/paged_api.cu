@@ -233,6 +233,8 @@ ALM_API int alm_attn_paged(alm_ctx* ctx, const alm_paged_kv* kv_, const alm_seq_
   int device, n_sms, *err;
   cudaStream_t st;
   TRY(alm_internal_ctx_paged(ctx, &device, &n_sms, &st, &err));
+  // (a row can be made again from its q, when its place in out has been written)
+  REQ(none || v->q_dev != v->out_dev, "out_dev must not be q_dev");
   REQ(v->work_bytes >= attn_paged_work_bytes(n_sms, kv.head_dim), "the work area is too small (alm_attn_paged_work)");
   if (none) return ALM_OK;
   AttnPaged a;

@@ -319,9 +319,10 @@ def rope_append(ctx, kv, seqs, q, k, v, rope, q_out, q_norm=None, k_norm=None, e
 def attn_paged(ctx, kv, seqs, q, out, work, scale=None, window=0, lse=None):
     """alm_attn_paged: out[r] = softmax(scale q[r] . K) V over the positions of
     row r's sequence up to its own (the last ``window`` of them when window >
-    0).  q, out (n_rows, heads, head_dim) of the cache's type; scale defaults
-    to head_dim ** -0.5; lse (n_rows, heads) fp32 receives the log of the sum
-    of exponentials.  Rows that see nothing get zeros and -inf."""
+    0).  q, out (n_rows, heads, head_dim) of the cache's type, not the same
+    memory; scale defaults to head_dim ** -0.5; lse (n_rows, heads) fp32
+    receives the log of the sum of exponentials.  Rows that see nothing get
+    zeros and -inf."""
     dev, n, d, code = ctx.device, seqs.n_rows, kv.head_dim, kv.code
     if kv.device != dev or seqs.device != dev or work.device != dev:
         _on(ctx, kv, seqs, work)

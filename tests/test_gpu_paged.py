@@ -1326,3 +1326,13 @@ def test_verify_denormal_temperatures(ctx, dtype):
         for min_p in (0.0, 0.3, 1.0):
             check_verify(ctx, start, torch.tensor(lg, device="cuda").to(DT[dtype]), draft, q, u, np.full(6, temp),
                          np.full(6, min_p))
+
+
+def test_attend_refuses_q_as_its_output(ctx):
+    b = Batch([3], [20], 16, 2, 64, torch.float16, seed=50)
+    q = b.randn(b.n_rows, 4, 64)
+    kept = q.clone()
+    with pytest.raises(ALMError, match="must not be q_dev"):
+        attend(ctx, b, q, out=q)
+    ctx.sync()
+    assert torch.equal(q, kept)
