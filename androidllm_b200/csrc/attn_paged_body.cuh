@@ -389,6 +389,7 @@ __device__ __noinline__ void mend_rows(const AttnPaged& a_, const PagedKV& kv_, 
                                        int r0, int step, unsigned todo, float m, float inv, int p0, int p1, float* part,
                                        volatile Waits* waits) {
   constexpr int V = HD / 32;
+  if (todo == 0) return;
   const AttnPaged a = a_;   // (in registers: the loops would load them from the arguments every time)
   const PagedKV kv = kv_;
   const int lane = threadIdx.x % kWarp;

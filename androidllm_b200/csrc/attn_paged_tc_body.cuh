@@ -8,6 +8,10 @@
 //   P = 2^(c S - c m), written over S as 16-bit values
 //   O (128 x head_dim, tensor memory) += P (tensor memory) . V
 //
+// P is of the cache's type because the product's operands have one type; its half
+// step is the output's own, averaged over the row.  The sum of weights is taken in
+// fp32 before that rounding.
+//
 // Two streams alternate, so that one's softmax runs under the other's
 // products: with kNQ = 2 they are two 128-row blocks over the same K and V
 // tiles, with kNQ = 1 (at most 128 rows in a sequence) the even and the odd
@@ -26,10 +30,11 @@
 // 1024 cycles of an SM, so the streams take turns at the exponential unit
 // (without turns both wait for it at once and the tensor core idles: 351 us
 // against 285 us at 4 x 2047 rows, 28 heads over 4 of 128).  4 x 2047 rows
-// take 268 us (935 TFLOP/s, 56% of a large library product's rate): a stream's
+// take 272 us replayed from a graph (920 TFLOP/s, 55% of a large library product's
+// rate), 309 us called back to back, at the power limit (810 TFLOP/s): a stream's
 // chain of product, tensor-memory read, maximum, exponentials, write and
 // product is 3540 cycles a step of both streams, 2048 of them tensor work.
-// 1 x 7 rows over 131 thousand positions (HBM-bound): 65 us, 4.1 TB/s, 60 us
+// 1 x 7 rows over 131 thousand positions (HBM-bound): 66 us, 4.1 TB/s, 60 us
 // of it this kernel.
 #pragma once
 

@@ -1,6 +1,6 @@
 // Operators of a batched step on device data: argument structs and launchers
 // shared by paged_api.cu (entry points and checks), rope_append.cu,
-// attn_paged.cu, attn_paged_tc.cu and verify.cu.
+// attn_paged_body.cuh, attn_paged_tc_body.cuh and verify.cu.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

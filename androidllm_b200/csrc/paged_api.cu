@@ -47,7 +47,8 @@ cudaError_t paged_init_attrs() {
 //   64 x 1000   36.9 / 50.9    39.0 / 51.2    69.4 / 53.1    72.1 / 54.3   104.1 / 57.9
 // (With its TMA producer at 64 rows too the mma.sync kernel takes as long as
 // the tcgen05 kernel there, and 16% longer at 49 rows of 131 thousand
-// positions.)
+// positions.)  max_rows, the host's bound, picks one kernel for all sequences: a
+// prompt chunk takes the single rows of its batch to the tcgen05 kernel too.
 constexpr long long kTcMinRows = 32;
 
 // Sequences of at most this many rows: the last of a unit's CTAs joins their
@@ -55,7 +56,9 @@ constexpr long long kTcMinRows = 32;
 // partials a row), are joined by a kernel of their own, which spreads them over
 // more CTAs but costs a launch (4 us of the host's time).  Joined there against
 // by the kernel, 8 rows a K/V head, 4 heads of 128: 3 x 100 7.4 / 9.1 us, 64 x
-// 1000 36.3 / 36.8 us, 2 x 4000 14.0 / 13.5 us, 1 x 16000 20.0 / 17.0 us.
+// 1000 36.3 / 36.8 us, 2 x 4000 14.0 / 13.5 us, 1 x 16000 20.0 / 17.0 us.  The
+// host knows the table's width, not the lengths: few short sequences under a
+// table of kLongTable positions or more pay for the second kernel.
 constexpr long long kJoinHere = 8, kFewUnits = 8, kLongTable = 4096;
 
 // The work area: a counter and a record a CTA, at the same place for every head

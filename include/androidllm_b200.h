@@ -484,7 +484,10 @@ ALM_API int alm_rope_append(alm_ctx* ctx, const alm_paged_kv* kv, const alm_seq_
  * sequence's end and of pages of other sequences never reach a result, NaN
  * and infinities included; nor does a value at a position that a row does not
  * see.  A page outside the pool is read as zeros and recorded for
- * alm_ctx_sync.  scale is positive, at most 1e30.  work_dev: alm_attn_paged_work
+ * alm_ctx_sync.  A row that sees an infinity or NaN of V has it in that column,
+ * however small its weight.  Scores, weights, sums and statistics are fp32; the
+ * weights are rounded to the cache's type for their product with V (after their
+ * sum was taken), and the output once.  scale is positive, at most 1e30.  work_dev: alm_attn_paged_work
  * bytes, 256-byte aligned, set to zeros before the first call that uses them
  * (a call leaves the counters in it zero again; after ALM_ERR_CUDA from
  * alm_ctx_sync set them to zeros again); calls that can overlap on the GPU,
