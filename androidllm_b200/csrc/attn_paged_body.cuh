@@ -35,9 +35,9 @@ constexpr int kPagedThreads = 256;
 constexpr int kJoinThreads = 128;
 constexpr int kPagedWarps = kPagedThreads / kWarp;
 // A weight is 2^(c s - round(c m)), one multiply-add a score.  What round()
-// leaves scales a chunk's weights by up to 2^(2^-24 c m): 2^-14 at this
-// |c m|, a quarter of fp16's half step.  Beyond it (at 2^28 every weight would be
-// 0 or infinite) m is taken off the scores first: c (s - m) is 0 at the maximum
+// leaves scales a chunk's weights by up to 2^(2^-24 c m): by 2^-14 at this |c m|,
+// an eighth of fp16's half step.  Beyond it (at 2^28 every weight would be 0 or
+// infinite) m is taken off the scores first: c (s - m) is 0 at the maximum
 // whatever c is.
 constexpr float kFarScore = 1024.f;
 

@@ -34,8 +34,8 @@
 // rate), 309 us called back to back, at the power limit (810 TFLOP/s): a stream's
 // chain of product, tensor-memory read, maximum, exponentials, write and
 // product is 3540 cycles a step of both streams, 2048 of them tensor work.
-// 1 x 7 rows over 131 thousand positions (HBM-bound): 66 us, 4.1 TB/s, 60 us
-// of it this kernel.
+// 1 x 7 rows over 131 thousand positions (HBM-bound): 66 us, 4.1 TB/s, 61
+// to 63 us of it this kernel.
 #pragma once
 
 #include "attn_paged_body.cuh"
@@ -236,9 +236,9 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
   // not finite though their weights were, with zeros for the infinities and NaN of
   // V, which the rows that see them then get; or when scores were beyond kFarScore,
   // and takes the maximum off them before they are scaled.  The barriers' phases
-  // and the counters go on.  512 rows over 30,512 positions, 28 heads over 4 of 128: 243 us, 1400 us
-  // with one infinity.  (Two copies of the code: a flag instead costs the first
-  // pass 8%.)
+  // and the counters go on.  512 rows over 30,512 positions, 28 heads over 4 of
+  // 128: 243 us, 1400 us with one infinity.  (Two copies of the code: a flag
+  // instead costs the first pass 8%.)
   auto again = [&] {
     bar_sync(4, kTcPagedThreads);
     return *static_cast<volatile int*>(&sh.lost) != 0;
@@ -488,7 +488,8 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
             tc_ld32(t_s + 32, sr[1]);
             const int p0 = (cu.t0 + t) * S::kTile;
             const bool mask = p0 + S::kTile - 1 > pos_a || (a.window > 0 && p0 <= pos_b - a.window);
-            const int n_hi = hi - p0, n_lo = max(n_hi, -1) - a.window;   // columns > n_hi, and with a window <= n_lo, are hidden
+            // columns > n_hi, and with a window <= n_lo, are hidden
+            const int n_hi = hi - p0, n_lo = max(n_hi, -1) - a.window;
             auto hide = [&](int h) {
 #pragma unroll
               for (int i = 64 * h; i < 64 * h + 64; ++i)
@@ -536,7 +537,8 @@ attn_paged_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
               }
             }
             const float base = m == kNegInf ? 0.f : m, mc = base * a.scale_log2;
-            const uint64_t c2 = pair(a.scale_log2, a.scale_log2), m2 = decltype(careful)::value ? pair(-base, -base) : pair(-mc, -mc);
+            const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
+            const uint64_t m2 = decltype(careful)::value ? pair(-base, -base) : pair(-mc, -mc);
             uint64_t sum[2] = {0, 0};   // (+0, +0)
             uint32_t pr[2][32];
             auto weights = [&](int h, int j0, int j1) {
