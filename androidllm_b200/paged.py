@@ -247,6 +247,8 @@ class SeqBatch:
             step = int(stride[0]) if rows > 1 else pages
             if step < pages:
                 raise ValueError("page_table rows must not overlap")
+            if step > _INT_MAX:
+                raise ValueError("page_table rows must lie less than 2^31 elements apart")
         sp = None
         if slots is not None:
             sp, _, ss = _contiguous(slots, "slots", (I32,), 1, device)
@@ -255,9 +257,9 @@ class SeqBatch:
         elif rows < n_seq:
             raise ValueError("page_table must have a row for every sequence")
         self.n_seq, self.n_rows = n_seq, int(n_rows)
-        if self.n_rows < 0:
-            raise ValueError("n_rows must not be negative")
-        most = self.n_rows if max_rows is None else int(max_rows)
+        if not 0 <= self.n_rows <= _INT_MAX:
+            raise ValueError("n_rows must not be negative and be below 2^31")
+        most = self.n_rows if max_rows is None else min(int(max_rows), _INT_MAX)
         self.c = SeqBatchView(n_seq, self.n_rows, most, rows, pages, step, rp, lp, tp, sp)
         self.ref = ctypes.addressof(self.c)
         self._keep = (row_start, kv_len, page_table, slots)
@@ -280,6 +282,14 @@ class AttnWorkspace:
 _ROPE_ARGS = struct.Struct("@PPPqqqqqqPqqiPPfPiiii").pack
 _ATTN_ARGS = struct.Struct("@PqqPqqPqiifPN").pack
 _VERIFY_ARGS = struct.Struct("@iiiiPPiqPPqqPPPPPP").pack
+_INT_MAX = 2 ** 31 - 1
+
+
+def _packed(pack, what, *args):
+    try:
+        return pack(*args)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"{what}: an argument is no number of its type ({e})") from None
 
 
 def _heads_of(q, what, n_rows, dim):
@@ -311,9 +321,9 @@ def rope_append(ctx, kv, seqs, q, k, v, rope, q_out, q_norm=None, k_norm=None, e
     rp, rcode, rs = _contiguous(rope, "rope", (F16, BF16, F32), 2, dev)
     qw = _flat(q_norm, "q_norm", code, (d,), dev) if q_norm is not None else 0
     kw = _flat(k_norm, "k_norm", code, (d,), dev) if k_norm is not None else 0
-    check(lib.alm_rope_append(ctx.h, kv.ref, seqs.ref, _ROPE_ARGS(
-        qp, kp, vp, qr, qh, kr, kh, vr, vh, op, o_r, oh, heads, qw, kw, eps, rp, rcode, rs[0], rs[1],
-        1 if interleaved else 0)))
+    check(lib.alm_rope_append(ctx.h, kv.ref, seqs.ref, _packed(
+        _ROPE_ARGS, "rope_append", qp, kp, vp, qr, qh, kr, kh, vr, vh, op, o_r, oh, heads, qw, kw, eps, rp, rcode,
+        rs[0], rs[1], 1 if interleaved else 0)))
 
 
 def attn_paged(ctx, kv, seqs, q, out, work, scale=None, window=0, lse=None):
@@ -335,9 +345,9 @@ def attn_paged(ctx, kv, seqs, q, out, work, scale=None, window=0, lse=None):
         if tuple(got) != shape[:2] or (shape[1] > 1 and stride[1] != 1):
             raise ValueError("lse must be (n_rows, heads), contiguous in its last dimension")
         ls = stride[0]
-    check(lib.alm_attn_paged(ctx.h, kv.ref, seqs.ref, _ATTN_ARGS(
-        qp, qr, qh, op, o_r, oh, lp, ls, shape[1], window, d ** -0.5 if scale is None else scale, work.pointer,
-        work.nbytes)))
+    check(lib.alm_attn_paged(ctx.h, kv.ref, seqs.ref, _packed(
+        _ATTN_ARGS, "attn_paged", qp, qr, qh, op, o_r, oh, lp, ls, shape[1], window,
+        d ** -0.5 if scale is None else scale, work.pointer, work.nbytes)))
 
 
 def verify(ctx, row_start, logits, draft_tokens, draft_probs, uniforms, temperature, tokens, n_accepted,
@@ -371,6 +381,6 @@ def verify(ctx, row_start, logits, draft_tokens, draft_probs, uniforms, temperat
     ap = _flat(n_accepted, "n_accepted", I32, (n_seq,), dev)
     mp = _flat(min_p, "min_p", F32, (n_seq,), dev) if min_p is not None else 0
     pp = _flat(p_draft, "p_draft", F32, (n_seq, k), dev) if p_draft is not None else 0
-    check(lib.alm_verify(ctx.h, _VERIFY_ARGS(
-        n_seq, n_rows, k, vocab, rp, lp, lcode, lstride[0] if n_rows > 1 else vocab, dp, qp, q_seq, q_step, up, tp, mp,
-        op, ap, pp)))
+    check(lib.alm_verify(ctx.h, _packed(
+        _VERIFY_ARGS, "verify", n_seq, n_rows, k, vocab, rp, lp, lcode, lstride[0] if n_rows > 1 else vocab, dp, qp,
+        q_seq, q_step, up, tp, mp, op, ap, pp)))

@@ -285,3 +285,31 @@ def test_views_know_their_device():
     with pytest.raises(ValueError, match="device"):
         paged.rope_append(NoContext, _cache(), seqs, Fake((5, 4, 64)), Fake((5, 2, 64)), Fake((5, 2, 64)), Fake((9, 64)),
                           Fake((5, 4, 64)))
+
+
+@pytest.mark.parametrize("kw", [dict(window=2 ** 31), dict(window=-2 ** 40), dict(window=1.5)])
+def test_python_attention_refuses_numbers_outside_their_types(kw):
+    class Work:
+        pointer, nbytes, device = P, 1 << 30, None
+    with pytest.raises(ValueError, match="attn_paged"):
+        paged.attn_paged(NoContext, _cache(), _seqs(), Fake((5, 4, 64)), Fake((5, 4, 64)), Work, **kw)
+
+
+def test_python_refuses_floats_outside_their_type():
+    from androidllm_b200._lib import ALMError
+
+    class Work:
+        pointer, nbytes, device = P, 1 << 30, None
+    with pytest.raises(ALMError, match="scale"):         # an infinity in 32 bits
+        paged.attn_paged(NoContext, _cache(), _seqs(), Fake((5, 4, 64)), Fake((5, 4, 64)), Work, scale=1e60)
+    with pytest.raises(ALMError, match="eps"):
+        paged.rope_append(NoContext, _cache(), _seqs(), Fake((5, 4, 64)), Fake((5, 2, 64)), Fake((5, 2, 64)),
+                          Fake((9, 64)), Fake((5, 4, 64)), eps=1e60)
+
+
+def test_batches_refuse_or_clamp_numbers_outside_their_types():
+    with pytest.raises(ValueError, match="page_table"):
+        _seqs(page_table=Fake((2, 4), "int32", stride=(2 ** 31, 1)))
+    with pytest.raises(ValueError, match="n_rows"):
+        _seqs(n_rows=2 ** 32 + 5)
+    assert _seqs(max_rows=2 ** 40).c.max_rows == 2 ** 31 - 1       # a bound, and this one holds too
